@@ -3,12 +3,17 @@
 ``B200Sampler`` keeps the reference's ``SamplerBase.select`` /
 ``select_batch`` call signature and runs the whole path (penalties,
 temperature, top-k, top-p, inverse-CDF draw) in hand-written sm_100a CUDA
-kernels behind a C ABI (``include/ns_sampler.h``).  The CUDA library is loaded
-on first use; there is no CPU fallback.
+kernels behind a C ABI (``include/ns_sampler.h``).  ``token_logprobs``,
+``policy_loss`` and ``preference_loss`` score and train on the tokens it draws
+(``include/ns_losses.h``).  The CUDA library is loaded on first use; there is
+no CPU fallback.
 """
 from .params import SamplingParams
 
-__all__ = ["SamplingParams", "B200Sampler", "SamplerBase", "VocabParallelSampler"]
+_LOSSES = ("token_logprobs", "policy_loss", "policy_loss_and_grad", "PolicyLoss",
+           "preference_loss", "preference_loss_and_grad", "PreferenceLoss")
+
+__all__ = ["SamplingParams", "B200Sampler", "SamplerBase", "VocabParallelSampler", *_LOSSES]
 
 
 def __getattr__(name):
@@ -18,4 +23,7 @@ def __getattr__(name):
     if name == "VocabParallelSampler":
         from . import vocab_parallel
         return vocab_parallel.VocabParallelSampler
+    if name in _LOSSES:
+        from . import losses
+        return getattr(losses, name)
     raise AttributeError(name)

@@ -1,4 +1,5 @@
-"""ctypes binding of the C ABI declared in ``include/ns_sampler.h``.
+"""ctypes binding of the C ABI declared in ``include/ns_sampler.h`` and
+``include/ns_losses.h``.
 
 The library is loaded from the package directory (built in-tree by
 ``b200_sampler.build``).  There is no fallback: if it is missing, loading
@@ -30,12 +31,16 @@ NS_DTYPE_F32 = 0
 NS_DTYPE_BF16 = 1
 NS_DTYPE_F16 = 2
 
-# name -> (restype, argtypes); mirrors include/ns_sampler.h
+# name -> (restype, argtypes); mirrors include/ns_sampler.h and include/ns_losses.h
 _c_i64 = ctypes.c_int64
 _c_u64 = ctypes.c_uint64
 _c_int = ctypes.c_int
 _c_vp = ctypes.c_void_p
 _c_sz = ctypes.c_size_t
+_c_f32 = ctypes.c_float
+
+# logits, dtype, rows, vocab, row_stride, targets, temperature, temperature_all
+_ROWS = [_c_vp, _c_int, _c_i64, _c_i64, _c_i64, _c_vp, _c_vp, _c_f32]
 
 PROTOTYPES = {
     "ns_status_string": (ctypes.c_char_p, [_c_int]),
@@ -96,6 +101,25 @@ PROTOTYPES = {
     "ns_ipc_handle": (_c_int, [_c_vp, _c_vp]),
     "ns_ipc_open": (_c_int, [_c_vp, ctypes.POINTER(_c_vp)]),
     "ns_ipc_close": (_c_int, [_c_vp]),
+    "ns_token_logprobs": (_c_int, [
+        *_ROWS, _c_vp, _c_vp, _c_vp, _c_vp,          # logprobs, entropy, stats, stream
+    ]),
+    "ns_token_logprobs_grad": (_c_int, [
+        *_ROWS, _c_vp, _c_vp,                        # stats, entropy
+        _c_vp, _c_vp, _c_vp, _c_i64, _c_vp,          # grad_logprobs, grad_entropy, grad_logits, grad_stride, stream
+    ]),
+    "ns_policy_loss": (_c_int, [
+        *_ROWS, _c_vp, _c_vp, _c_vp, _c_vp,          # old_logprobs, ref_logprobs, advantages, weights
+        _c_f32, _c_f32, _c_f32, _c_f32,              # clip_low, clip_high, kl_coef, entropy_coef
+        _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp,    # loss, row_loss, logprobs, entropy, kl, stats
+        _c_vp, _c_vp, _c_i64, _c_vp,                 # row_grad, grad_logits, grad_stride, stream
+    ]),
+    "ns_preference_loss": (_c_int, [
+        *_ROWS, _c_vp, _c_i64, _c_vp,                # seq_offsets, pairs, ref_logprobs
+        _c_f32, _c_f32, _c_int,                      # beta, label_smoothing, average
+        _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp,    # loss, pair_loss, rewards, logprobs, stats, row_grad
+        _c_vp, _c_i64, _c_vp,                        # grad_logits, grad_stride, stream
+    ]),
 }
 
 _lock = threading.Lock()

@@ -3,8 +3,10 @@
     python -m b200_sampler.build          (from nano-inference_b200/)
 
 nvcc cross-compiles for sm_100a only; no GPU is needed to build.  The library
-is a plain shared object with a C ABI (``include/ns_sampler.h``); it links the
-CUDA runtime statically and uses no torch headers.
+is a plain shared object with a C ABI (``include/ns_sampler.h``,
+``include/ns_losses.h``); it links the CUDA runtime statically and uses no
+torch headers.  Every source has its own object under ``build/``, so a change
+to one compiles that one alone.
 """
 from __future__ import annotations
 
@@ -13,6 +15,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG_DIR)                     # nano-inference_b200/
@@ -26,8 +29,8 @@ NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-std=c++17", "-lineinfo",
     "-Xcompiler", "-fPIC,-O2",
-    "-shared",
 ]
+OBJ_DIR = os.path.join(ROOT, "build")
 
 
 def nvcc_path() -> str:
@@ -70,8 +73,12 @@ def build_histpack(force: bool = False) -> str:
     return out
 
 
+def _headers():
+    return glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(INCLUDE, "*.h"))
+
+
 def _deps():
-    return sources() + glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(INCLUDE, "*.h"))
+    return sources() + _headers()
 
 
 def needs_build() -> bool:
@@ -81,22 +88,40 @@ def needs_build() -> bool:
     return any(os.path.getmtime(p) > t for p in _deps())
 
 
-def build(force: bool = False, verbose: bool = False) -> str:
-    """Compile csrc/*.cu into the in-tree shared library (and the history
-    packer); returns the library's path."""
-    build_histpack(force)
-    if not force and not needs_build():
-        return LIB_PATH
-    tmp = LIB_PATH + ".tmp"
-    cmd = [nvcc_path(), *NVCC_FLAGS, "-I", INCLUDE, "-I", CSRC, "-o", tmp, *sources()]
+def _run(cmd, verbose: bool = False) -> None:
     if verbose:
-        cmd.insert(1, "-Xptxas=-v")
         print(" ".join(cmd), flush=True)
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError("nvcc failed:\n" + r.stdout + r.stderr)
     if verbose:
         print(r.stdout + r.stderr)
+
+
+def _compile(src: str, force: bool, verbose: bool) -> str:
+    obj = os.path.join(OBJ_DIR, os.path.basename(src) + ".o")
+    if not force and os.path.exists(obj) and all(os.path.getmtime(obj) >= os.path.getmtime(p)
+                                                 for p in [src, *_headers()]):
+        return obj
+    cmd = [nvcc_path(), *NVCC_FLAGS, "-I", INCLUDE, "-I", CSRC, "-c", "-o", obj + ".tmp", src]
+    if verbose:
+        cmd.insert(1, "-Xptxas=-v")
+    _run(cmd, verbose)
+    os.replace(obj + ".tmp", obj)
+    return obj
+
+
+def build(force: bool = False, verbose: bool = False) -> str:
+    """Compile csrc/*.cu into the in-tree shared library (and the history
+    packer); returns the library's path."""
+    build_histpack(force)
+    if not force and not needs_build():
+        return LIB_PATH
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    with ThreadPoolExecutor() as pool:
+        objs = list(pool.map(lambda src: _compile(src, force, verbose), sources()))
+    tmp = LIB_PATH + ".tmp"
+    _run([nvcc_path(), *NVCC_FLAGS, "-shared", "-o", tmp, *objs], verbose)
     os.replace(tmp, LIB_PATH)
     return LIB_PATH
 

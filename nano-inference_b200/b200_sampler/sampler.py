@@ -404,6 +404,21 @@ class DeviceBatch:
             None if self.uniforms is None else self.uniforms.data_ptr(), self.seed, offset,
             out.data_ptr(), ws_ptr, ws_bytes, s.cuda_stream)
 
+    def logprobs(self, logits: torch.Tensor, ids: torch.Tensor, out: torch.Tensor,
+                 stream: Optional[torch.cuda.Stream] = None) -> int:
+        """ln softmax(logits / T)[id] of the ids a ``launch`` drew from these
+        logits, into ``out`` (fp32 [batch]): one ``ns_token_logprobs`` call
+        with each row's own temperature (a greedy row counts as 1), without
+        penalties, top-k and top-p.  A failed row (negative id) gets 0, a row
+        of negative temperature NaN."""
+        B, V = logits.shape
+        assert B == self.batch and logits.stride(1) == 1 and ids.numel() >= B and out.numel() >= B
+        assert ids.dtype == torch.int64 and out.dtype == torch.float32 and ids.is_contiguous() and out.is_contiguous()
+        s = stream if stream is not None else torch.cuda.current_stream(self.device)
+        return self.lib.ns_token_logprobs(
+            logits.data_ptr(), _DTYPES[logits.dtype], B, V, int(logits.stride(0)) if B > 1 else V,
+            ids.data_ptr(), self.params.data_ptr(), 1.0, out.data_ptr(), None, None, s.cuda_stream)
+
 
 class DeviceHistory:
     """Token histories (prompt + outputs per row) kept on the device for a
