@@ -33,7 +33,7 @@
  *     equal bits.  No call needs a workspace or leaves state for the next.
  *
  *   stats fp32 [rows][2], written by the forward calls and read by the
- *   gradient: the row's largest logit and log2 of sum exp((x - largest) / T).
+ *   gradient: an offset c (a logit of the row) and log2 of sum exp((x - c) / T).
  */
 #ifndef NS_LOSSES_H
 #define NS_LOSSES_H

@@ -2,18 +2,23 @@
 // and entropies with their gradient, the clipped policy loss and the preference
 // loss (include/ns_losses.h).
 //
-// Mathematics.  With s = log2(e) / T, m the row's largest logit and
-//   t_j = (x_j - m) s,   S = sum_j 2^t_j,   U = sum_j 2^t_j t_j
-// (t_j <= 0, so nothing overflows, and x_j - m is taken before the scale, so a
-// row whose logits are all the type's lowest value still gets its uniform
-// distribution), ln p_j = ln2 (t_j - log2 S) and the entropy is
-// ln2 (log2 S - U / S).  One pass over the row keeps a running (m, S, U) per
-// thread and rescales it when m rises; partial rows join by the same rule.  The
+// Mathematics.  With s = log2(e) / T, c the target's logit and
+//   t_j = (x_j - c) s,   S = sum_j 2^t_j,   U = sum_j 2^t_j t_j,
+// ln p_j = ln2 (t_j - log2 S), so the target's log-probability is -ln S, and
+// the entropy is ln2 (log2 S - U / S).  Any offset near the row's largest logit
+// would do in fp32; the target's is known before the row is read and is the
+// same for every thread and block of the row, so no maximum is kept and no sum
+// is ever rescaled: the exponential's error (2^-22, and -5e-8 on average,
+// measured over 4 M arguments) enters once.  The difference is taken before the
+// scale, so a row whose logits are all the type's lowest value still gets its
+// uniform distribution.  A row whose S leaves [2^-60, 2^100] (a target less
+// likely than 2^-100, or barred) is added up again with a running maximum.  The
 // gradient of a * logprob + h * entropy is
 //   dx_j = (a 1{j = target} - p_j (a + h (ln p_j + H))) / T.
 //
 // Bound: HBM.  A forward reads the logits once, a gradient reads them and
-// writes as many bytes.
+// writes as many bytes; the policy loss keeps a row in shared memory between
+// its sums and its gradient, and reads it once.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -32,9 +37,11 @@ namespace cg = cooperative_groups;
 namespace ns {
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
+constexpr int kBatch = 4;          // 16-byte loads a thread has in flight
+constexpr int kKeepBytes = 48 << 10;   // of a row, in a block's shared memory
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr double kLn2 = 0.6931471805599453;
 
@@ -111,6 +118,30 @@ struct Elem<NS_DTYPE_F16> {
   }
 };
 
+// Two fp32 values in a 64-bit register: one instruction for both.
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 f2(float lo, float hi) {
+  F2 d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+__device__ __forceinline__ void split(F2 v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+
 struct LossArgs {
   const void* logits;
   int64_t rows, vocab, row_stride;
@@ -130,6 +161,7 @@ struct LossArgs {
   const float *grad_logprobs, *grad_entropy;
   void* grad_logits;
   int64_t grad_stride;
+  int keep;              // vectors a thread keeps in shared memory for the gradient
 };
 
 // The row's scale log2(e) / T and 1 / T; NaN for a temperature that gives no
@@ -205,31 +237,23 @@ __device__ __forceinline__ Span row_span(const void* row, int64_t vocab) {
   return {head, (vocab - head) / E};
 }
 
-// Block `rank` of `blocks` adds its share of the row; every thread returns the block's part.
+// Block `rank` of `blocks` adds its share of the row with a running maximum:
+// the part of a thread whose columns rise is rescaled.
 template <int DT, bool ENT>
-__device__ __forceinline__ Part block_part(const void* base, int64_t vocab, float scale, int rank, int blocks,
-                                           Part* shared) {
+__device__ __noinline__ Part running_part(const void* base, int64_t vocab, float scale, int rank, int blocks,
+                                          Part* shared) {
   using D = Elem<DT>;
   using T = typename D::T;
-  constexpr int E = D::E, U = 4;
+  constexpr int E = D::E;
   const T* row = static_cast<const T*>(base);
   const Span sp = row_span<E>(row, vocab);
   const int64_t v0 = sp.nv * rank / blocks, v1 = sp.nv * (rank + 1) / blocks;
   const uint4* vec = reinterpret_cast<const uint4*>(row + sp.head);
   Part p = {-INFINITY, 0.0f, 0.0f};
-  for (int64_t v = v0 + threadIdx.x; v < v1; v += U * kThreads) {
-    uint4 q[U];
-#pragma unroll
-    for (int k = 0; k < U; ++k) {
-      const int64_t at = v + k * kThreads;
-      q[k] = at < v1 ? vec[at] : make_uint4(D::kNegInf2, D::kNegInf2, D::kNegInf2, D::kNegInf2);
-    }
-#pragma unroll
-    for (int k = 0; k < U; ++k) {
-      float x[E];
-      D::unpack(q[k], x);
-      add<ENT>(p, x, scale);
-    }
+  for (int64_t v = v0 + threadIdx.x; v < v1; v += kThreads) {
+    float x[E];
+    D::unpack(vec[v], x);
+    add<ENT>(p, x, scale);
   }
   if (rank == 0 && threadIdx.x < sp.head) {
     const float x[1] = {D::load(row + threadIdx.x)};
@@ -241,6 +265,7 @@ __device__ __forceinline__ Part block_part(const void* base, int64_t vocab, floa
     add<ENT>(p, x, scale);
   }
   p = warp_join<ENT>(p, scale);
+  __syncthreads();
   if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = p;
   __syncthreads();
   const int lane = threadIdx.x & 31;
@@ -248,26 +273,146 @@ __device__ __forceinline__ Part block_part(const void* base, int64_t vocab, floa
   return warp_join<ENT>(p, scale);
 }
 
-// What a row's (m, S, U) and target give.  Sums are taken in 64 bits, so that
-// differences from a reference's log-probability keep their digits; the
-// logarithm is split as exponent * ln2 + ln(mantissa), whose second part lies
-// in [0, ln2) and is exact to 2^-25.
+// Adds a vector's 2^t, and 2^t t, to the sums.  t is held above -200, where
+// 2^t is 0, so that 0 * -inf does not arise; a NaN t has made 2^t NaN.
+template <int DT, bool ENT>
+__device__ __forceinline__ void add_vector(const uint4& q, F2 minus_c, F2 scale, F2& s, F2& u) {
+  using D = Elem<DT>;
+  float x[D::E];
+  D::unpack(q, x);
+#pragma unroll
+  for (int i = 0; i < D::E; i += 2) {
+    float a, b;
+    const F2 t = mul2(add2(f2(x[i], x[i + 1]), minus_c), scale);
+    split(t, a, b);
+    const F2 e = f2(ex2_approx(a), ex2_approx(b));
+    s = add2(s, e);
+    if (ENT) u = fma2(e, f2(fmaxf(a, -200.0f), fmaxf(b, -200.0f)), u);
+  }
+}
+
+struct RowShared {
+  Part warp[kWarps];
+  Part block[kMaxCluster];
+};
+
+// Whether S says that c lies too far from the row's largest logit.  NaN: the
+// row holds one, and no offset helps.
+__device__ __forceinline__ bool sums_far(float s) { return s < 0x1p-60f || s > 0x1p100f; }
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+  return v;
+}
+
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// The row's sums around c over the whole cluster, the same in every thread of it.  The
+// block's first `keep` vectors of each thread stay in `kept`.
+template <int DT, bool ENT, bool GRAD>
+__device__ __forceinline__ Part row_sums(const void* base, int64_t vocab, float c, float scale, int keep,
+                                         uint4* kept, RowShared& sh, cg::cluster_group& cluster) {
+  using D = Elem<DT>;
+  using T = typename D::T;
+  constexpr int E = D::E;
+  const int blocks = int(cluster.num_blocks()), rank = int(cluster.block_rank());
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const T* row = static_cast<const T*>(base);
+  const Span sp = row_span<E>(row, vocab);
+  const int v0 = int(sp.nv * rank / blocks), n = int(sp.nv * (rank + 1) / blocks) - v0;
+  const uint4* vec = reinterpret_cast<const uint4*>(row + sp.head) + v0;
+  const uint4 none = make_uint4(D::kNegInf2, D::kNegInf2, D::kNegInf2, D::kNegInf2);
+  if (blocks > 1) cluster_arrive();
+  uint4 q[kBatch];
+#pragma unroll
+  for (int k = 0; k < kBatch; ++k) {
+    const int v = int(threadIdx.x) + k * kThreads;
+    q[k] = v < n ? vec[v] : none;
+  }
+  // the elements before the first 16-byte boundary and after the last whole vector
+  const int64_t tail = sp.head + sp.nv * E + threadIdx.x;
+  const float edge[2] = {threadIdx.x < sp.head ? D::load(row + threadIdx.x) : -INFINITY,
+                         tail < vocab ? D::load(row + tail) : -INFINITY};
+  const F2 minus_c = f2(-c, -c), scale2 = f2(scale, scale);
+  F2 s[2] = {0, 0}, u[2] = {0, 0};
+  for (int v = threadIdx.x, i = 0; v < n; v += kBatch * kThreads, i += kBatch) {
+    uint4 next[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int at = v + (kBatch + k) * kThreads;
+      next[k] = at < n ? vec[at] : none;
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      if (GRAD && i + k < keep) kept[(i + k) * kThreads + threadIdx.x] = q[k];
+      add_vector<DT, ENT>(q[k], minus_c, scale2, s[k & 1], u[k & 1]);
+      q[k] = next[k];
+    }
+  }
+  Part p;
+  p.m = c;
+  {
+    float a, b;
+    split(add2(s[0], s[1]), a, b);
+    p.s = a + b;
+    split(add2(u[0], u[1]), a, b);
+    p.u = a + b;
+  }
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    if (rank == (k == 0 ? 0 : blocks - 1)) {
+      const float t = (edge[k] - c) * scale, e = ex2_approx(t);
+      p.s += e;
+      if (ENT) p.u = fmaf(e, fmaxf(t, -200.0f), p.u);
+    }
+  p.s = warp_sum(p.s);
+  if (ENT) p.u = warp_sum(p.u);
+  if (lane == 0) sh.warp[warp] = p;
+  __syncthreads();
+  p.s = warp_sum(lane < kWarps ? sh.warp[lane].s : 0.0f);
+  if (ENT) p.u = warp_sum(lane < kWarps ? sh.warp[lane].u : 0.0f);
+  if (blocks > 1) {
+    cluster_wait();                    // every block has started: its shared memory may be written
+    if (int(threadIdx.x) < blocks) *cluster.map_shared_rank(&sh.block[rank], threadIdx.x) = p;
+    cluster.sync();
+    p.s = warp_sum(lane < blocks ? sh.block[lane].s : 0.0f);
+    if (ENT) p.u = warp_sum(lane < blocks ? sh.block[lane].u : 0.0f);
+  }
+  if (!sums_far(p.s)) return p;      // the same for the whole cluster
+  p = running_part<DT, ENT>(base, vocab, scale, rank, blocks, sh.warp);
+  if (blocks > 1) {
+    cluster.sync();                    // every block has read the first sums
+    if (int(threadIdx.x) < blocks) *cluster.map_shared_rank(&sh.block[rank], threadIdx.x) = p;
+    cluster.sync();
+    p = lane < blocks ? sh.block[lane] : Part{-INFINITY, 0.0f, 0.0f};
+    p = warp_join<ENT>(p, scale);
+  }
+  return p;
+}
+
+// What a row's sums and target give, in 64 bits, so that differences from a
+// reference's log-probability keep their digits.  The target's t uses the same
+// rounded scale as the sums.  The logarithm is split as exponent * ln2 +
+// ln(mantissa), whose second part lies in [0, ln2) and is exact to 2^-25.
 struct RowResult {
   double logprob;
   float entropy, log2s;
 };
 template <bool ENT>
-__device__ __forceinline__ RowResult finish(const Part& p, float x_target, double inv_t) {
+__device__ __forceinline__ RowResult finish(const Part& p, float x_target, float scale) {
   int ex;
-  const float mant = 2.0f * frexpf(p.s, &ex);       // S >= 1 for a row with a distribution
+  const float mant = 2.0f * frexpf(p.s, &ex);
   const double ln_s = p.s < INFINITY && p.s > 0.0f ? double(ex - 1) * kLn2 + double(logf(mant)) : double(NAN);
   RowResult r;
-  r.logprob = (double(x_target) - double(p.m)) * inv_t - ln_s;
-  r.log2s = float(ln_s / kLn2);
-  r.entropy = ENT ? float(ln_s - kLn2 * double(p.u) / double(p.s)) : 0.0f;
-  if (!isfinite(inv_t)) r.logprob = NAN;
+  r.logprob = (double(x_target) - double(p.m)) * double(scale) * kLn2 - ln_s;
+  r.log2s = float(ln_s * (1.0 / kLn2));
+  r.entropy = ENT ? float(ln_s) - float(kLn2) * (p.u / p.s) : 0.0f;
   return r;
 }
+
+__device__ __forceinline__ float row_offset(float x_target) { return isfinite(x_target) ? x_target : 0.0f; }
 
 struct PolicyRow {
   float loss, kl, a, h;
@@ -313,16 +458,112 @@ __device__ __forceinline__ bool row_alive(const LossArgs& a, int64_t row, float&
   return true;
 }
 
-// One cluster of blocks per row.
-template <int DT, bool ENT, int OP>
+// Gradient of one value: g = p (A + B log2 p), log2 p = (x - c) s - log2 S.
+struct GradRow {
+  float c, log2s, scale, ca, cb;
+  float at;                  // the value at the target
+  bool zero;
+  int64_t target;
+};
+template <bool ENT>
+__device__ __forceinline__ float grad_value(const GradRow& g, float x) {
+  const float t = fmaf(x - g.c, g.scale, -g.log2s);
+  return ex2_approx(t) * (ENT ? fmaf(g.cb, fmaxf(t, -200.0f), g.ca) : g.ca);
+}
+// a and h: dloss/dlogprob and dloss/dentropy of the row
+template <bool ENT>
+__device__ __forceinline__ GradRow grad_row(float c, float log2s, float scale, double inv_t, float a, float h,
+                                            float entropy, int64_t target, float x_target) {
+  GradRow g;
+  g.c = c == -INFINITY ? 0.0f : c;      // no distribution: log2 S is NaN
+  g.log2s = log2s;
+  g.scale = scale;
+  g.ca = -float((double(a) + (ENT ? double(h) * double(entropy) : 0.0)) * inv_t);
+  g.cb = ENT ? -float(double(h) * kLn2 * inv_t) : 0.0f;
+  g.at = grad_value<ENT>(g, x_target) + float(double(a) * inv_t);
+  g.zero = a == 0.0f && h == 0.0f;
+  g.target = target;
+  return g;
+}
+// Writes a vector of gradients at out + j, j its first column.
+template <int DT, bool ENT>
+__device__ __forceinline__ void grad_vector(const GradRow& g, const uint4& q, typename Elem<DT>::T* out, int64_t j) {
+  using D = Elem<DT>;
+  float x[D::E];
+  D::unpack(q, x);
+  const F2 minus_c = f2(-g.c, -g.c), scale = f2(g.scale, g.scale), minus_l = f2(-g.log2s, -g.log2s);
+  const F2 ca = f2(g.ca, g.ca), cb = f2(g.cb, g.cb);
+#pragma unroll
+  for (int i = 0; i < D::E; i += 2) {
+    float a, b;
+    const F2 t = fma2(add2(f2(x[i], x[i + 1]), minus_c), scale, minus_l);
+    split(t, a, b);
+    const F2 p = f2(ex2_approx(a), ex2_approx(b));
+    const F2 w = ENT ? fma2(cb, f2(fmaxf(a, -200.0f), fmaxf(b, -200.0f)), ca) : ca;
+    split(mul2(p, w), x[i], x[i + 1]);
+  }
+  *reinterpret_cast<uint4*>(out + j) = D::pack(x);
+  if (uint64_t(g.target - j) < uint64_t(D::E)) D::store(out + g.target, g.at);   // one thread of the row
+}
+template <int DT, bool ENT>
+__device__ __forceinline__ void grad_element(const GradRow& g, float x, typename Elem<DT>::T* out, int64_t j) {
+  Elem<DT>::store(out + j, j == g.target ? g.at : grad_value<ENT>(g, x));
+}
+
+// Block `rank`'s share of a row's gradient, whose first vectors the block has
+// kept; the rest is read again.
+template <int DT, bool ENT>
+__device__ __forceinline__ void write_gradient(const GradRow& g, const void* base, void* grad, int64_t vocab, int keep,
+                                               const uint4* kept, int rank, int blocks) {
+  using D = Elem<DT>;
+  using T = typename D::T;
+  constexpr int E = D::E;
+  const T* row = static_cast<const T*>(base);
+  T* out = static_cast<T*>(grad);
+  const Span sp = row_span<E>(row, vocab);
+  const int v0 = int(sp.nv * rank / blocks), n = int(sp.nv * (rank + 1) / blocks) - v0;
+  const uint4* vec = reinterpret_cast<const uint4*>(row + sp.head) + v0;
+  const int64_t j0 = sp.head + int64_t(v0) * E;
+  if (((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0) {
+    for (int v = threadIdx.x, i = 0; v < n; v += kThreads, ++i)
+      grad_vector<DT, ENT>(g, i < keep ? kept[i * kThreads + threadIdx.x] : vec[v], out, j0 + int64_t(v) * E);
+  } else {      // the rows start on different 16-byte phases: element by element
+    for (int64_t j = j0 + threadIdx.x; j < j0 + int64_t(n) * E; j += kThreads)
+      grad_element<DT, ENT>(g, D::load(row + j), out, j);
+  }
+  const int64_t tail = sp.head + sp.nv * E + threadIdx.x;
+  if (rank == 0 && threadIdx.x < sp.head)
+    grad_element<DT, ENT>(g, D::load(row + threadIdx.x), out, threadIdx.x);
+  if (rank == blocks - 1 && tail < vocab) grad_element<DT, ENT>(g, D::load(row + tail), out, tail);
+}
+
+// Zeros in block `rank`'s share of a row.
+template <int DT>
+__device__ __forceinline__ void write_zeros(void* grad, int64_t vocab, int rank, int blocks) {
+  using T = typename Elem<DT>::T;
+  constexpr int E = Elem<DT>::E;
+  T* out = static_cast<T*>(grad);
+  const Span sp = row_span<E>(out, vocab);
+  uint4* dst = reinterpret_cast<uint4*>(out + sp.head);
+  const int v1 = int(sp.nv * (rank + 1) / blocks);
+  for (int v = int(sp.nv * rank / blocks) + threadIdx.x; v < v1; v += kThreads) dst[v] = make_uint4(0, 0, 0, 0);
+  const int64_t tail = sp.head + sp.nv * E + threadIdx.x;
+  if (rank == 0 && threadIdx.x < sp.head) Elem<DT>::store(out + threadIdx.x, 0.0f);
+  if (rank == blocks - 1 && tail < vocab) Elem<DT>::store(out + tail, 0.0f);
+}
+
+// One cluster of blocks per row.  GRAD (policy only): the gradient as well.
+template <int DT, bool ENT, int OP, bool GRAD>
 __global__ void __launch_bounds__(kThreads) forward_kernel(const LossArgs a) {
   using D = Elem<DT>;
   using T = typename D::T;
-  __shared__ Part warp_parts[kWarps];
-  __shared__ Part block_parts[kMaxCluster];
+  __shared__ RowShared sh;
+  __shared__ GradRow coef;
+  extern __shared__ uint4 kept[];
   cg::cluster_group cluster = cg::this_cluster();
   const int blocks = int(cluster.num_blocks()), rank = int(cluster.block_rank());
   const int64_t row = blockIdx.x / blocks;
+  void* grad = GRAD ? static_cast<T*>(a.grad_logits) + row * a.grad_stride : nullptr;
   float w;
   const bool alive = row_alive<OP>(a, row, w);
   if (!alive) {            // the same for every block of the cluster
@@ -337,6 +578,7 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const LossArgs a) {
       }
       if (OP == kPreference) a.row_grad[row] = 0.0f;
     }
+    if (GRAD) write_zeros<DT>(grad, a.vocab, rank, blocks);
     return;
   }
   float scale;
@@ -345,33 +587,39 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const LossArgs a) {
   const T* x = static_cast<const T*>(a.logits) + row * a.row_stride;
   const int64_t target = a.targets[row];
   const float x_target = target < a.vocab ? D::load(x + target) : NAN;
-  Part p = block_part<DT, ENT>(x, a.vocab, scale, rank, blocks, warp_parts);
-  if (blocks > 1) {
-    if (threadIdx.x == 0) *cluster.map_shared_rank(&block_parts[rank], 0) = p;
-    cluster.sync();
+  const Part p = row_sums<DT, ENT, GRAD>(x, a.vocab, row_offset(x_target), scale, a.keep, kept, sh, cluster);
+  if (threadIdx.x == 0 && (GRAD || rank == 0)) {
+    const RowResult r = finish<ENT>(p, x_target, scale);
+    const float log2s = isnan(r.logprob) ? NAN : r.log2s, entropy = isnan(r.logprob) ? NAN : r.entropy;
+    PolicyRow l;
+    if (OP == kPolicy) {
+      l = policy_row(a, row, r.logprob, entropy, w);
+      if (GRAD) coef = grad_row<ENT>(p.m, log2s, scale, inv_t, l.a, l.h, entropy, target, x_target);
+    }
     if (rank == 0) {
-      const int lane = threadIdx.x & 31;
-      p = lane < blocks ? block_parts[lane] : Part{-INFINITY, 0.0f, 0.0f};
-      p = warp_join<ENT>(p, scale);
+      a.logprobs[row] = float(r.logprob);
+      if (ENT) a.entropy[row] = entropy;
+      if (a.stats) {
+        a.stats[2 * row] = p.m;
+        a.stats[2 * row + 1] = log2s;
+      }
+      if (OP == kPolicy) {
+        a.row_loss[row] = l.loss;
+        if (a.kl) a.kl[row] = l.kl;
+        a.row_grad[row] = l.a;
+        a.row_grad[a.rows + row] = l.h;
+      }
+      if (OP == kPreference)   // the row's gain; the pair kernel turns it into the coefficient
+        a.row_grad[row] = float(r.logprob - (a.ref_logprobs ? double(a.ref_logprobs[row]) : 0.0));
     }
   }
-  if (rank != 0 || threadIdx.x != 0) return;
-  const RowResult r = finish<ENT>(p, x_target, inv_t);
-  a.logprobs[row] = float(r.logprob);
-  if (ENT) a.entropy[row] = isnan(r.logprob) ? NAN : r.entropy;
-  if (a.stats) {
-    a.stats[2 * row] = p.m;
-    a.stats[2 * row + 1] = isnan(r.logprob) ? NAN : r.log2s;
+  if (GRAD) {
+    __syncthreads();
+    if (coef.zero)
+      write_zeros<DT>(grad, a.vocab, rank, blocks);
+    else
+      write_gradient<DT, ENT>(coef, x, grad, a.vocab, a.keep, kept, rank, blocks);
   }
-  if (OP == kPolicy) {
-    const PolicyRow l = policy_row(a, row, r.logprob, r.entropy, w);
-    a.row_loss[row] = l.loss;
-    if (a.kl) a.kl[row] = l.kl;
-    a.row_grad[row] = l.a;
-    a.row_grad[a.rows + row] = l.h;
-  }
-  if (OP == kPreference)   // the row's gain; the pair kernel turns it into the coefficient
-    a.row_grad[row] = float(r.logprob - (a.ref_logprobs ? double(a.ref_logprobs[row]) : 0.0));
 }
 
 __device__ __forceinline__ double block_sum(double v, double* shared) {
@@ -450,21 +698,9 @@ __global__ void __launch_bounds__(1024) pair_kernel(const LossArgs a, float beta
   if (threadIdx.x == 0) *loss = a.pairs ? float(total / double(a.pairs)) : 0.0f;
 }
 
-// Gradient of one value: g = -p (A + B t') with t' = log2 p.
-struct GradRow {
-  float m, log2s, scale, ca, cb, at;   // at: added at the target
-  int64_t target;
-};
-template <bool ENT>
-__device__ __forceinline__ float grad_value(const GradRow& g, float x) {
-  const float t = fmaf(x - g.m, g.scale, -g.log2s);
-  const float p = ex2_approx(t);
-  return ENT ? -p * fmaf(g.cb, fmaxf(t, -200.0f), g.ca) : -p * g.ca;
-}
-
 constexpr int kGradVecs = 8;    // vectors of a thread
 
-// One block per (row, chunk of 512 x 8 vectors).
+// The gradient alone: one block per (row, chunk of kThreads x kGradVecs vectors).
 template <int DT, bool ENT>
 __global__ void __launch_bounds__(kThreads) grad_kernel(const LossArgs a, int chunks) {
   using D = Elem<DT>;
@@ -476,75 +712,40 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(const LossArgs a, int ch
   T* out = static_cast<T*>(a.grad_logits) + row * a.grad_stride;
   const float ga = a.grad_logprobs ? a.grad_logprobs[row] : 0.0f;
   const float gh = ENT ? a.grad_entropy[row] : 0.0f;
-  const bool zero = a.targets[row] < 0 || (ga == 0.0f && gh == 0.0f);
-  GradRow g = {};
-  if (!zero) {
-    double inv_t;
-    row_scale(a, row, g.scale, inv_t);
-    g.m = a.stats[2 * row];
-    if (g.m == -INFINITY) g.m = 0.0f;        // no distribution: log2 S is NaN
-    g.log2s = a.stats[2 * row + 1];
-    g.target = a.targets[row];
-    g.at = float(double(ga) * inv_t);
-    g.ca = float((double(ga) + (ENT ? double(gh) * double(a.entropy[row]) : 0.0)) * inv_t);
-    g.cb = ENT ? float(double(gh) * kLn2 * inv_t) : 0.0f;
-  }
-  const Span sp = row_span<E>(out, a.vocab);
-  if (((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(out)) & 15) != 0) {
-    // the rows start on different 16-byte phases: element by element
-    const int64_t per = int64_t(kThreads) * kGradVecs * E;
-    const int64_t end = min(a.vocab, (chunk + 1) * per);
-    for (int64_t j = chunk * per + threadIdx.x; j < end; j += kThreads) {
-      float v = 0.0f;
-      if (!zero) {
-        v = grad_value<ENT>(g, D::load(x + j));
-        if (j == g.target) v += g.at;
-      }
-      D::store(out + j, v);
-    }
+  if (a.targets[row] < 0 || (ga == 0.0f && gh == 0.0f)) {
+    write_zeros<DT>(out, a.vocab, chunk, chunks);
     return;
   }
-  const uint4* src = reinterpret_cast<const uint4*>(x + sp.head);
-  uint4* dst = reinterpret_cast<uint4*>(out + sp.head);
-  const int64_t base = int64_t(chunk) * kThreads * kGradVecs + threadIdx.x;
-  if (zero) {
-#pragma unroll
-    for (int k = 0; k < kGradVecs; ++k)
-      if (base + k * kThreads < sp.nv) dst[base + k * kThreads] = make_uint4(0, 0, 0, 0);
-  } else {
-    uint4 q[kGradVecs];
-#pragma unroll
-    for (int k = 0; k < kGradVecs; ++k)
-      if (base + k * kThreads < sp.nv) q[k] = src[base + k * kThreads];
-#pragma unroll
-    for (int k = 0; k < kGradVecs; ++k) {
-      const int64_t v = base + k * kThreads;
-      if (v >= sp.nv) continue;
-      float f[E];
-      D::unpack(q[k], f);
-#pragma unroll
-      for (int i = 0; i < E; ++i) f[i] = grad_value<ENT>(g, f[i]);
-      const int64_t j = g.target - (sp.head + v * E);
-      if (uint64_t(j) < uint64_t(E)) {
-#pragma unroll
-        for (int i = 0; i < E; ++i)
-          if (i == int(j)) f[i] += g.at;
-      }
-      dst[v] = D::pack(f);
-    }
+  float scale;
+  double inv_t;
+  row_scale(a, row, scale, inv_t);
+  // every thread reads the target's logit before it writes; in place, the one that uses it is its writer
+  const int64_t target = a.targets[row];
+  const GradRow g = grad_row<ENT>(a.stats[2 * row], a.stats[2 * row + 1], scale, inv_t, ga, gh,
+                                  ENT ? a.entropy[row] : 0.0f, target, target < a.vocab ? D::load(x + target) : NAN);
+  const Span sp = row_span<E>(x, a.vocab);
+  if (((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(out)) & 15) != 0) {
+    write_gradient<DT, ENT>(g, x, out, a.vocab, 0, nullptr, chunk, chunks);
+    return;
   }
-  if (chunk == 0) {     // the elements before the first whole vector and after the last
-    const int64_t rest = sp.head + sp.nv * E, edge = sp.head + (a.vocab - rest);
-    if (threadIdx.x < edge) {
-      const int64_t j = threadIdx.x < sp.head ? threadIdx.x : rest + (threadIdx.x - sp.head);
-      float v = 0.0f;
-      if (!zero) {
-        v = grad_value<ENT>(g, D::load(x + j));
-        if (j == g.target) v += g.at;
-      }
-      D::store(out + j, v);
-    }
+  const int v0 = int(sp.nv * chunk / chunks), n = int(sp.nv * (chunk + 1) / chunks) - v0;
+  const int64_t j0 = sp.head + int64_t(v0) * E;
+  const uint4* src = reinterpret_cast<const uint4*>(x + j0);
+  uint4 q[kGradVecs];
+#pragma unroll
+  for (int k = 0; k < kGradVecs; ++k) {
+    const int v = int(threadIdx.x) + k * kThreads;
+    if (v < n) q[k] = src[v];
   }
+#pragma unroll
+  for (int k = 0; k < kGradVecs; ++k) {
+    const int v = int(threadIdx.x) + k * kThreads;
+    if (v < n) grad_vector<DT, ENT>(g, q[k], out, j0 + int64_t(v) * E);
+  }
+  const int64_t tail = sp.head + sp.nv * E + threadIdx.x;
+  if (chunk == 0 && threadIdx.x < sp.head)
+    grad_element<DT, ENT>(g, D::load(x + threadIdx.x), out, threadIdx.x);
+  if (chunk == chunks - 1 && tail < a.vocab) grad_element<DT, ENT>(g, D::load(x + tail), out, tail);
 }
 
 // ---------------------------------------------------------------------------
@@ -562,17 +763,38 @@ int sm_count(int* out) {
   return NS_OK;
 }
 
-template <int DT, bool ENT, int OP>
-int launch_forward(const LossArgs& a, cudaStream_t stream) {
+template <int DT, bool ENT, int OP, bool GRAD>
+int launch_forward(const LossArgs& base, cudaStream_t stream) {
   int sms = 0;
   if (const int rc = sm_count(&sms)) return rc;
+  LossArgs a = base;
+  const int64_t vectors = a.vocab / Elem<DT>::E;
   // blocks per row: enough to give every SM two, each thread at least one vector
   int blocks = 1;
-  while (blocks < kMaxCluster && a.rows * blocks < 2 * sms && a.vocab >= int64_t(2) * blocks * kThreads * Elem<DT>::E)
-    blocks *= 2;
+  while (blocks < kMaxCluster && a.rows * blocks < 2 * sms && vectors >= int64_t(2) * blocks * kThreads) blocks *= 2;
+  size_t smem = 0;
+  if (GRAD) {
+    // the row stays in the cluster's shared memory, as far as kKeepBytes of a block go
+    while (blocks < kMaxCluster && vectors * 16 > int64_t(blocks) * kKeepBytes) blocks *= 2;
+    const int64_t per = (vectors + blocks - 1) / blocks;
+    a.keep = int(std::min<int64_t>((per + kThreads - 1) / kThreads, kKeepBytes / (16 * kThreads)));
+    smem = size_t(a.keep) * kThreads * 16;
+    static std::mutex mu;
+    static bool configured[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return NS_ERR_CUDA;
+    std::lock_guard<std::mutex> lk(mu);
+    if (!configured[dev]) {
+      if (cudaFuncSetAttribute(forward_kernel<DT, ENT, OP, GRAD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               kKeepBytes) != cudaSuccess)
+        return NS_ERR_CUDA;
+      configured[dev] = true;
+    }
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(a.rows * blocks));
   cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -580,25 +802,29 @@ int launch_forward(const LossArgs& a, cudaStream_t stream) {
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, forward_kernel<DT, ENT, OP>, a) == cudaSuccess ? NS_OK : NS_ERR_CUDA;
+  return cudaLaunchKernelEx(&cfg, forward_kernel<DT, ENT, OP, GRAD>, a) == cudaSuccess ? NS_OK : NS_ERR_CUDA;
 }
 
-template <int OP>
+template <int OP, bool GRAD, int DT>
+int forward_typed(const LossArgs& a, cudaStream_t stream) {
+  if constexpr (OP == kPreference)
+    return launch_forward<DT, false, OP, GRAD>(a, stream);
+  else
+    return a.entropy ? launch_forward<DT, true, OP, GRAD>(a, stream) : launch_forward<DT, false, OP, GRAD>(a, stream);
+}
+
+template <int OP, bool GRAD = false>
 int forward(const LossArgs& a, int dtype, cudaStream_t stream) {
-  const bool ent = a.entropy != nullptr;
   switch (dtype) {
-    case NS_DTYPE_F32:
-      return ent ? launch_forward<NS_DTYPE_F32, true, OP>(a, stream) : launch_forward<NS_DTYPE_F32, false, OP>(a, stream);
-    case NS_DTYPE_BF16:
-      return ent ? launch_forward<NS_DTYPE_BF16, true, OP>(a, stream) : launch_forward<NS_DTYPE_BF16, false, OP>(a, stream);
-    default:
-      return ent ? launch_forward<NS_DTYPE_F16, true, OP>(a, stream) : launch_forward<NS_DTYPE_F16, false, OP>(a, stream);
+    case NS_DTYPE_F32: return forward_typed<OP, GRAD, NS_DTYPE_F32>(a, stream);
+    case NS_DTYPE_BF16: return forward_typed<OP, GRAD, NS_DTYPE_BF16>(a, stream);
+    default: return forward_typed<OP, GRAD, NS_DTYPE_F16>(a, stream);
   }
 }
 
 template <int DT>
 int launch_grad(const LossArgs& a, cudaStream_t stream) {
-  const int64_t per = int64_t(kThreads) * kGradVecs * Elem<DT>::E;
+  const int64_t per = int64_t(kThreads) * kGradVecs * Elem<DT>::E;    // shares differ by one vector at most
   const int chunks = int((a.vocab + per - 1) / per);
   const int64_t blocks = a.rows * chunks;
   if (blocks > 0x7FFFFFFF) return NS_ERR_INVALID_ARGUMENT;
@@ -714,15 +940,12 @@ int ns_policy_loss(const void* logits, int dtype, int64_t rows, int64_t vocab, i
   a.row_loss = row_loss;
   a.kl = kl;
   a.row_grad = row_grad;
-  if (const int rc = ns::forward<ns::kPolicy>(a, dtype, s)) return rc;
-  ns::policy_sum_kernel<<<1, 1024, 0, s>>>(a, loss);
-  if (cudaGetLastError() != cudaSuccess) return NS_ERR_CUDA;
-  if (!grad_logits) return NS_OK;
-  a.grad_logprobs = row_grad;
-  a.grad_entropy = entropy_coef != 0.0f ? row_grad + rows : nullptr;
   a.grad_logits = grad_logits;
   a.grad_stride = grad_stride;
-  return ns::gradient(a, dtype, s);
+  if (const int rc = grad_logits ? ns::forward<ns::kPolicy, true>(a, dtype, s) : ns::forward<ns::kPolicy>(a, dtype, s))
+    return rc;
+  ns::policy_sum_kernel<<<1, 1024, 0, s>>>(a, loss);
+  return cudaGetLastError() == cudaSuccess ? NS_OK : NS_ERR_CUDA;
 }
 
 int ns_preference_loss(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t row_stride,

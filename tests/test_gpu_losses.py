@@ -63,7 +63,7 @@ def _check_logprobs(x, targets, temperature, entropy=True, grads=True, seed=0):
     assert got_lp.dtype == torch.float32
     close(got_lp, lp, logprob_bound(ln_p, lp), "logprobs")
     if entropy:
-        close(got_ent, ent, entropy_bound(ln_p, ent), "entropy")
+        close(got_ent, ent, entropy_bound(ln_p, lp, ent), "entropy")
     # the call without a graph gives the same bits
     with torch.no_grad():
         again = token_logprobs(x, targets, temperature=temperature, entropy=entropy)
@@ -76,7 +76,7 @@ def _check_logprobs(x, targets, temperature, entropy=True, grads=True, seed=0):
     hh = h if entropy else torch.zeros_like(h)
     want = O.gradient(ln_p, ent, alive, t, targets, a, hh)
     aa = torch.where(alive, a.cpu().double(), torch.zeros_like(lp))
-    bound = grad_bound(ln_p, t, ent, targets.cpu(), want, aa, torch.zeros_like(lp),
+    bound = grad_bound(ln_p, lp, t, ent, targets.cpu(), want, aa, torch.zeros_like(lp),
                        torch.where(alive, hh.cpu().double(), torch.zeros_like(lp)), x.dtype)
     assert grad.dtype == x.dtype and grad.shape == x.shape
     close(grad, want, torch.nan_to_num(bound), "grad")
@@ -171,7 +171,7 @@ def test_gradient_of_broadcast_rows():
     ln_p, lp, ent, alive, t = O.rows(base.detach().expand(6, 777), targets)
     want = O.gradient(ln_p, ent, alive, t, targets, a)
     zero = torch.zeros_like(lp)
-    bound = grad_bound(ln_p, t, ent, targets.cpu(), want, a.cpu().double(), zero, zero, torch.float32)
+    bound = grad_bound(ln_p, lp, t, ent, targets.cpu(), want, a.cpu().double(), zero, zero, torch.float32)
     close(grad, want.sum(0, keepdim=True), bound.sum(0, keepdim=True) + 6 * U * want.abs().sum(0), "grad")
 
 
@@ -225,18 +225,18 @@ def _check_policy(got, grad, want, x, targets, old, ref, adv, weights, kl_coef):
     ratio = torch.nan_to_num(torch.exp(lp - old.cpu().double()) * adv.cpu().double()).abs()
     rel = lp_off + 6 * U
     up = torch.zeros_like(lp) if ref is None else torch.nan_to_num(torch.exp(ref.cpu().double() - lp))
-    ent_off = torch.nan_to_num(entropy_bound(ln_p, ent)) * want["h"].abs() / w.clamp(min=1e-30)
+    ent_off = torch.nan_to_num(entropy_bound(ln_p, lp, ent)) * want["h"].abs() / w.clamp(min=1e-30)
     row_off = ratio * rel + abs(kl_coef) * (up + 1) * rel + ent_off + 6 * U * torch.nan_to_num(want["row_loss"]).abs()
     close(got.logprobs, lp, torch.nan_to_num(logprob_bound(ln_p, lp)), "logprobs")
     close(got.row_loss, want["row_loss"], row_off, "row_loss")
     if ref is not None:
         close(got.kl, want["kl"], (up + 1) * rel + 4 * U * torch.nan_to_num(want["kl"]), "kl")
     if got.entropy is not None:
-        close(got.entropy, ent, torch.nan_to_num(entropy_bound(ln_p, ent)), "entropy")
+        close(got.entropy, ent, torch.nan_to_num(entropy_bound(ln_p, lp, ent)), "entropy")
     close(got.loss, want["loss"], (w * row_off).sum() + 2 * U * want["loss"].abs().nan_to_num(), "loss")
     if grad is not None:
         a_off = w * (ratio + abs(kl_coef) * up) * rel
-        bound = grad_bound(ln_p, want["t"], ent, targets.cpu(), want["grad"], want["a"], a_off, want["h"], x.dtype)
+        bound = grad_bound(ln_p, lp, want["t"], ent, targets.cpu(), want["grad"], want["a"], a_off, want["h"], x.dtype)
         close(grad, want["grad"], torch.nan_to_num(bound), "grad")
 
 
@@ -336,7 +336,7 @@ def _check_preference(got, grad, want, x, targets, ref, beta):
         pairs = len(want["pair_loss"])
         zero = torch.zeros_like(lp)
         a_off = want["a"].abs().nan_to_num() * 8 * U + torch.where(want["alive"], abs(beta) / pairs * 2 * total, zero)
-        bound = grad_bound(ln_p, want["t"], zero, targets.cpu(), want["grad"], want["a"], a_off, zero, x.dtype)
+        bound = grad_bound(ln_p, lp, want["t"], zero, targets.cpu(), want["grad"], want["a"], a_off, zero, x.dtype)
         close(grad, want["grad"], torch.nan_to_num(bound), "grad")
 
 
@@ -511,7 +511,7 @@ def test_backward_twice_and_upstream_gradients():
     one64, zero = torch.ones_like(lp64) * alive, torch.zeros_like(lp64)
     for got, a, h in ((only_h, zero, one64), (only_a, one64, zero)):
         want = O.gradient(ln_p, ent64, alive, t, targets, a, h)
-        close(got, want, grad_bound(ln_p, t, ent64, targets.cpu(), want, a, zero, h, torch.float32), "grad")
+        close(got, want, grad_bound(ln_p, lp64, t, ent64, targets.cpu(), want, a, zero, h, torch.float32), "grad")
 
 
 def test_changed_logits_stop_the_backward_pass():
