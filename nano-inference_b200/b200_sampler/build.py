@@ -77,6 +77,12 @@ def _headers():
     return glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(INCLUDE, "*.h"))
 
 
+def _included(src: str):
+    """The headers that a source names."""
+    text = open(src).read()
+    return [h for h in _headers() if os.path.basename(h) in text]
+
+
 def _deps():
     return sources() + _headers()
 
@@ -101,7 +107,7 @@ def _run(cmd, verbose: bool = False) -> None:
 def _compile(src: str, force: bool, verbose: bool) -> str:
     obj = os.path.join(OBJ_DIR, os.path.basename(src) + ".o")
     if not force and os.path.exists(obj) and all(os.path.getmtime(obj) >= os.path.getmtime(p)
-                                                 for p in [src, *_headers()]):
+                                                 for p in [src, *_included(src)]):
         return obj
     cmd = [nvcc_path(), *NVCC_FLAGS, "-I", INCLUDE, "-I", CSRC, "-c", "-o", obj + ".tmp", src]
     if verbose:

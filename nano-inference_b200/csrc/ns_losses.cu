@@ -41,7 +41,6 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kBatch = 4;          // 16-byte loads a thread has in flight
-constexpr int kKeepBytes = 48 << 10;   // of a row, in a block's shared memory
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr double kLn2 = 0.6931471805599453;
 
@@ -161,7 +160,6 @@ struct LossArgs {
   const float *grad_logprobs, *grad_entropy;
   void* grad_logits;
   int64_t grad_stride;
-  int keep;              // vectors a thread keeps in shared memory for the gradient
 };
 
 // The row's scale log2(e) / T and 1 / T; NaN for a temperature that gives no
@@ -309,11 +307,10 @@ __device__ __forceinline__ float warp_sum(float v) {
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
-// The row's sums around c over the whole cluster, the same in every thread of it.  The
-// block's first `keep` vectors of each thread stay in `kept`.
-template <int DT, bool ENT, bool GRAD>
-__device__ __forceinline__ Part row_sums(const void* base, int64_t vocab, float c, float scale, int keep,
-                                         uint4* kept, RowShared& sh, cg::cluster_group& cluster) {
+// The row's sums around c over the whole cluster, the same in every thread of it.
+template <int DT, bool ENT>
+__device__ __forceinline__ Part row_sums(const void* base, int64_t vocab, float c, float scale, RowShared& sh,
+                                         cg::cluster_group& cluster) {
   using D = Elem<DT>;
   using T = typename D::T;
   constexpr int E = D::E;
@@ -337,7 +334,7 @@ __device__ __forceinline__ Part row_sums(const void* base, int64_t vocab, float 
                          tail < vocab ? D::load(row + tail) : -INFINITY};
   const F2 minus_c = f2(-c, -c), scale2 = f2(scale, scale);
   F2 s[2] = {0, 0}, u[2] = {0, 0};
-  for (int v = threadIdx.x, i = 0; v < n; v += kBatch * kThreads, i += kBatch) {
+  for (int v = threadIdx.x; v < n; v += kBatch * kThreads) {
     uint4 next[kBatch];
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
@@ -346,7 +343,6 @@ __device__ __forceinline__ Part row_sums(const void* base, int64_t vocab, float 
     }
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
-      if (GRAD && i + k < keep) kept[(i + k) * kThreads + threadIdx.x] = q[k];
       add_vector<DT, ENT>(q[k], minus_c, scale2, s[k & 1], u[k & 1]);
       q[k] = next[k];
     }
@@ -409,27 +405,33 @@ __device__ __forceinline__ RowResult finish(const Part& p, float x_target, float
   r.logprob = (double(x_target) - double(p.m)) * double(scale) * kLn2 - ln_s;
   r.log2s = float(ln_s * (1.0 / kLn2));
   r.entropy = ENT ? float(ln_s) - float(kLn2) * (p.u / p.s) : 0.0f;
+  if (isnan(r.logprob)) r.log2s = r.entropy = NAN;
   return r;
 }
 
 __device__ __forceinline__ float row_offset(float x_target) { return isfinite(x_target) ? x_target : 0.0f; }
 
+struct PolicyIn {
+  float old, adv, ref, w;
+};
 struct PolicyRow {
   float loss, kl, a, h;
 };
-__device__ __forceinline__ PolicyRow policy_row(const LossArgs& a, int64_t row, double logprob, float entropy, float w) {
-  const float adv = a.advantages[row];
-  const float ratio = expf(float(logprob - double(a.old_logprobs[row])));
-  const float inside = ratio * adv;
-  const float clipped = fminf(fmaxf(ratio, 1.0f - a.clip_low), 1.0f + a.clip_high) * adv;
+__device__ __forceinline__ PolicyIn policy_in(const LossArgs& a, int64_t row, float w) {
+  return {a.old_logprobs[row], a.advantages[row], a.ref_logprobs ? a.ref_logprobs[row] : 0.0f, w};
+}
+__device__ __forceinline__ PolicyRow policy_row(const LossArgs& a, const PolicyIn& in, double logprob, float entropy) {
+  const float ratio = expf(float(logprob - double(in.old)));
+  const float inside = ratio * in.adv;
+  const float clipped = fminf(fmaxf(ratio, 1.0f - a.clip_low), 1.0f + a.clip_high) * in.adv;
   PolicyRow r = {0.0f, 0.0f, 0.0f, 0.0f};
   // fmin drops a NaN, so the comparison keeps it; without an advantage there is no term (0 * inf is NaN)
-  if (adv != 0.0f || isnan(ratio)) {
+  if (in.adv != 0.0f || isnan(ratio)) {
     r.loss = -(clipped < inside ? clipped : inside);
     r.a = clipped < inside ? 0.0f : -inside;
   }
   if (a.ref_logprobs) {
-    const float d = float(double(a.ref_logprobs[row]) - logprob);
+    const float d = float(double(in.ref) - logprob);
     const float g = expm1f(d);
     r.kl = g - d;
     if (a.kl_coef != 0.0f) {
@@ -439,10 +441,16 @@ __device__ __forceinline__ PolicyRow policy_row(const LossArgs& a, int64_t row, 
   }
   if (a.entropy_coef != 0.0f) {
     r.loss = fmaf(-a.entropy_coef, entropy, r.loss);
-    r.h = -a.entropy_coef * w;
+    r.h = -a.entropy_coef * in.w;
   }
-  r.a *= w;
+  r.a *= in.w;
   return r;
+}
+__device__ __forceinline__ void write_policy_row(const LossArgs& a, int64_t row, const PolicyRow& l) {
+  a.row_loss[row] = l.loss;
+  if (a.kl) a.kl[row] = l.kl;
+  a.row_grad[row] = l.a;
+  a.row_grad[a.rows + row] = l.h;
 }
 
 // Whether the row holds a token, by operator.
@@ -510,31 +518,15 @@ __device__ __forceinline__ void grad_element(const GradRow& g, float x, typename
   Elem<DT>::store(out + j, j == g.target ? g.at : grad_value<ENT>(g, x));
 }
 
-// Block `rank`'s share of a row's gradient, whose first vectors the block has
-// kept; the rest is read again.
+// Block `rank`'s share of a row's gradient where the rows start on different 16-byte phases: element by element.
 template <int DT, bool ENT>
-__device__ __forceinline__ void write_gradient(const GradRow& g, const void* base, void* grad, int64_t vocab, int keep,
-                                               const uint4* kept, int rank, int blocks) {
-  using D = Elem<DT>;
-  using T = typename D::T;
-  constexpr int E = D::E;
+__device__ __forceinline__ void write_elements(const GradRow& g, const void* base, void* grad, int64_t vocab, int rank,
+                                               int blocks) {
+  using T = typename Elem<DT>::T;
   const T* row = static_cast<const T*>(base);
-  T* out = static_cast<T*>(grad);
-  const Span sp = row_span<E>(row, vocab);
-  const int v0 = int(sp.nv * rank / blocks), n = int(sp.nv * (rank + 1) / blocks) - v0;
-  const uint4* vec = reinterpret_cast<const uint4*>(row + sp.head) + v0;
-  const int64_t j0 = sp.head + int64_t(v0) * E;
-  if (((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0) {
-    for (int v = threadIdx.x, i = 0; v < n; v += kThreads, ++i)
-      grad_vector<DT, ENT>(g, i < keep ? kept[i * kThreads + threadIdx.x] : vec[v], out, j0 + int64_t(v) * E);
-  } else {      // the rows start on different 16-byte phases: element by element
-    for (int64_t j = j0 + threadIdx.x; j < j0 + int64_t(n) * E; j += kThreads)
-      grad_element<DT, ENT>(g, D::load(row + j), out, j);
-  }
-  const int64_t tail = sp.head + sp.nv * E + threadIdx.x;
-  if (rank == 0 && threadIdx.x < sp.head)
-    grad_element<DT, ENT>(g, D::load(row + threadIdx.x), out, threadIdx.x);
-  if (rank == blocks - 1 && tail < vocab) grad_element<DT, ENT>(g, D::load(row + tail), out, tail);
+  const int64_t end = vocab * (rank + 1) / blocks;
+  for (int64_t j = vocab * rank / blocks + threadIdx.x; j < end; j += kThreads)
+    grad_element<DT, ENT>(g, Elem<DT>::load(row + j), static_cast<T*>(grad), j);
 }
 
 // Zeros in block `rank`'s share of a row.
@@ -552,33 +544,32 @@ __device__ __forceinline__ void write_zeros(void* grad, int64_t vocab, int rank,
   if (rank == blocks - 1 && tail < vocab) Elem<DT>::store(out + tail, 0.0f);
 }
 
-// One cluster of blocks per row.  GRAD (policy only): the gradient as well.
-template <int DT, bool ENT, int OP, bool GRAD>
+// The numbers of a row that holds no token.
+template <int OP>
+__device__ __forceinline__ void write_dead_row(const LossArgs& a, int64_t row) {
+  a.logprobs[row] = 0.0f;
+  if (a.entropy) a.entropy[row] = 0.0f;
+  if (a.stats) a.stats[2 * row] = a.stats[2 * row + 1] = 0.0f;
+  if (OP == kPolicy) {
+    a.row_loss[row] = 0.0f;
+    if (a.kl) a.kl[row] = 0.0f;
+    a.row_grad[row] = a.row_grad[a.rows + row] = 0.0f;
+  }
+  if (OP == kPreference) a.row_grad[row] = 0.0f;
+}
+
+// One cluster of blocks per row.
+template <int DT, bool ENT, int OP>
 __global__ void __launch_bounds__(kThreads) forward_kernel(const LossArgs a) {
   using D = Elem<DT>;
   using T = typename D::T;
   __shared__ RowShared sh;
-  __shared__ GradRow coef;
-  extern __shared__ uint4 kept[];
   cg::cluster_group cluster = cg::this_cluster();
   const int blocks = int(cluster.num_blocks()), rank = int(cluster.block_rank());
   const int64_t row = blockIdx.x / blocks;
-  void* grad = GRAD ? static_cast<T*>(a.grad_logits) + row * a.grad_stride : nullptr;
   float w;
-  const bool alive = row_alive<OP>(a, row, w);
-  if (!alive) {            // the same for every block of the cluster
-    if (rank == 0 && threadIdx.x == 0) {
-      a.logprobs[row] = 0.0f;
-      if (a.entropy) a.entropy[row] = 0.0f;
-      if (a.stats) a.stats[2 * row] = a.stats[2 * row + 1] = 0.0f;
-      if (OP == kPolicy) {
-        a.row_loss[row] = 0.0f;
-        if (a.kl) a.kl[row] = 0.0f;
-        a.row_grad[row] = a.row_grad[a.rows + row] = 0.0f;
-      }
-      if (OP == kPreference) a.row_grad[row] = 0.0f;
-    }
-    if (GRAD) write_zeros<DT>(grad, a.vocab, rank, blocks);
+  if (!row_alive<OP>(a, row, w)) {            // the same for every block of the cluster
+    if (rank == 0 && threadIdx.x == 0) write_dead_row<OP>(a, row);
     return;
   }
   float scale;
@@ -587,39 +578,18 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const LossArgs a) {
   const T* x = static_cast<const T*>(a.logits) + row * a.row_stride;
   const int64_t target = a.targets[row];
   const float x_target = target < a.vocab ? D::load(x + target) : NAN;
-  const Part p = row_sums<DT, ENT, GRAD>(x, a.vocab, row_offset(x_target), scale, a.keep, kept, sh, cluster);
-  if (threadIdx.x == 0 && (GRAD || rank == 0)) {
-    const RowResult r = finish<ENT>(p, x_target, scale);
-    const float log2s = isnan(r.logprob) ? NAN : r.log2s, entropy = isnan(r.logprob) ? NAN : r.entropy;
-    PolicyRow l;
-    if (OP == kPolicy) {
-      l = policy_row(a, row, r.logprob, entropy, w);
-      if (GRAD) coef = grad_row<ENT>(p.m, log2s, scale, inv_t, l.a, l.h, entropy, target, x_target);
-    }
-    if (rank == 0) {
-      a.logprobs[row] = float(r.logprob);
-      if (ENT) a.entropy[row] = entropy;
-      if (a.stats) {
-        a.stats[2 * row] = p.m;
-        a.stats[2 * row + 1] = log2s;
-      }
-      if (OP == kPolicy) {
-        a.row_loss[row] = l.loss;
-        if (a.kl) a.kl[row] = l.kl;
-        a.row_grad[row] = l.a;
-        a.row_grad[a.rows + row] = l.h;
-      }
-      if (OP == kPreference)   // the row's gain; the pair kernel turns it into the coefficient
-        a.row_grad[row] = float(r.logprob - (a.ref_logprobs ? double(a.ref_logprobs[row]) : 0.0));
-    }
+  const Part p = row_sums<DT, ENT>(x, a.vocab, row_offset(x_target), scale, sh, cluster);
+  if (threadIdx.x != 0 || rank != 0) return;
+  const RowResult r = finish<ENT>(p, x_target, scale);
+  a.logprobs[row] = float(r.logprob);
+  if (ENT) a.entropy[row] = r.entropy;
+  if (a.stats) {
+    a.stats[2 * row] = p.m;
+    a.stats[2 * row + 1] = r.log2s;
   }
-  if (GRAD) {
-    __syncthreads();
-    if (coef.zero)
-      write_zeros<DT>(grad, a.vocab, rank, blocks);
-    else
-      write_gradient<DT, ENT>(coef, x, grad, a.vocab, a.keep, kept, rank, blocks);
-  }
+  if (OP == kPolicy) write_policy_row(a, row, policy_row(a, policy_in(a, row, w), r.logprob, r.entropy));
+  if (OP == kPreference)   // the row's gain; the pair kernel turns it into the coefficient
+    a.row_grad[row] = float(r.logprob - (a.ref_logprobs ? double(a.ref_logprobs[row]) : 0.0));
 }
 
 __device__ __forceinline__ double block_sum(double v, double* shared) {
@@ -698,6 +668,354 @@ __global__ void __launch_bounds__(1024) pair_kernel(const LossArgs a, float beta
   if (threadIdx.x == 0) *loss = a.pairs ? float(total / double(a.pairs)) : 0.0f;
 }
 
+// ---------------------------------------------------------------------------
+// Policy loss and gradient from one reading of the logits
+// ---------------------------------------------------------------------------
+// Persistent clusters; cluster i takes rows i, i + clusters, ...  Block r of a
+// cluster holds columns of every one of its rows, and each of its kRowWarps row
+// warps a contiguous share of those, which it streams by bulk copies of
+// kChunkVecs vectors into its own ring in shared memory.  A chunk is read
+// twice there, for the row's sums and then for its gradient, and only then
+// refilled, so DRAM sees the logits once.  The scalar warp joins the sums over
+// the block and, through the peers' shared memory, over the cluster, and turns
+// them into the row's loss and coefficients; that chain of latencies (some 2 us)
+// passes while the row warps write the gradient of the row before and add up
+// the row behind, so a ring holds two rows and what is in flight.  One block
+// barrier per row:
+//   row warps     sums(k) | barrier(k) | gradient(k - 1), sums(k + 1) | barrier(k + 1) | ...
+//   scalar warp            barrier(k) | join and finish row k, load row k + 2's numbers | barrier(k + 1) | ...
+constexpr int kRowWarps = 16;
+constexpr int kPipeThreads = (kRowWarps + 1) * 32;
+constexpr int kChunkVecs = 64;
+constexpr int kChunkBytes = kChunkVecs * 16;
+constexpr int kMaxSlots = 14;                 // chunks of a warp's ring
+constexpr uint32_t kPipeSmem = uint32_t(kRowWarps) * kMaxSlots * (kChunkBytes + 8);
+
+struct RowInfo {
+  float c, scale;
+  int alive;
+};
+struct PipeShared {
+  uint64_t bar[2];                // sums of the cluster's blocks, by row parity
+  uint64_t far_bar;               // the same for a row that is added up again
+  float2 part[2][kMaxCluster];    // (S, U) of each block
+  float4 far_part[kMaxCluster];   // (m, S, U)
+  float2 warp_part[2][kRowWarps];
+  RowInfo info[2];
+  GradRow coef[2];
+  int coef_alive[2];
+};
+
+__device__ __forceinline__ uint32_t peer_addr(const void* p, int rank) {
+  uint32_t d;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(d) : "r"(smem_addr(p)), "r"(rank));
+  return d;
+}
+// Stores 8 bytes in a peer block's shared memory and counts them on its barrier.
+__device__ __forceinline__ void send(uint32_t dst, float a, float b, uint32_t bar) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(dst), "f"(a),
+               "f"(b), "r"(bar)
+               : "memory");
+}
+
+// What the scalar warp loads of a row, ahead of its turn.
+struct RowIn {
+  bool alive;
+  int64_t target;
+  float x_target, scale, edge;
+  double inv_t;
+  PolicyIn in;
+};
+
+// The barrier of both kinds of warps.
+__device__ __forceinline__ void row_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(kPipeThreads) : "memory"); }
+
+template <int DT, bool ENT>
+__global__ void __launch_bounds__(kPipeThreads, 1) policy_kernel(const LossArgs a) {
+  using D = Elem<DT>;
+  using T = typename D::T;
+  constexpr int E = D::E;
+  __shared__ PipeShared sh;
+  extern __shared__ __align__(128) unsigned char dyn[];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int blocks = int(cluster.num_blocks()), rank = int(cluster.block_rank());
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t first_row = blockIdx.x / blocks, clusters = gridDim.x / blocks;
+  const int64_t rows = (a.rows - first_row + clusters - 1) / clusters;     // of this cluster
+  uint64_t* full_all = reinterpret_cast<uint64_t*>(dyn + kRowWarps * kMaxSlots * kChunkBytes);
+  if (threadIdx.x < kRowWarps * kMaxSlots) mbar_init(full_all + threadIdx.x, 1);
+  if (threadIdx.x == 0) {
+    mbar_init(&sh.bar[0], 1);
+    mbar_init(&sh.bar[1], 1);
+    mbar_init(&sh.far_bar, 1);
+  }
+  fence_mbar_init();
+  __syncthreads();
+  cluster.sync();                       // the peers' barriers exist
+
+  if (warp == kRowWarps) {
+    // ------------------------------------------------------------ scalar warp
+    bool bad = false;
+    uint32_t joined = 0, far_phase = 0;      // rows joined over the cluster so far
+    auto load_target = [&](int64_t k) { return k < rows ? a.targets[first_row + k * clusters] : int64_t(-1); };
+    auto load_row = [&](int64_t k, int64_t target) {
+      RowIn r = {};
+      r.target = target;
+      if (k >= rows || target < 0) return r;
+      const int64_t row = first_row + k * clusters;
+      float w;
+      r.alive = row_alive<kPolicy>(a, row, w);
+      const T* x = static_cast<const T*>(a.logits) + row * a.row_stride;
+      r.x_target = target < a.vocab ? D::load(x + target) : NAN;
+      row_scale(a, row, r.scale, r.inv_t);
+      r.in = policy_in(a, row, w);
+      // the first block's lanes 0.. hold the elements before the first vector, the last one's lanes 16.. those after
+      const Span sp = row_span<E>(x, a.vocab);
+      const int64_t tail = sp.head + sp.nv * E + lane - 16;
+      r.edge = -INFINITY;
+      if (rank == 0 && lane < sp.head) r.edge = D::load(x + lane);
+      if (rank == blocks - 1 && lane >= 16 && tail < a.vocab) r.edge = D::load(x + tail);
+      return r;
+    };
+    auto publish = [&](int64_t k, const RowIn& r) {
+      if (lane == 0) sh.info[k & 1] = {row_offset(r.x_target), r.scale, r.alive};
+    };
+    auto finish_row = [&](int64_t k, const RowIn& r) {
+      const int par = int(k & 1);
+      const int64_t row = first_row + k * clusters;
+      if (!r.alive) {
+        if (lane == 0) {
+          sh.coef_alive[par] = 0;
+          if (rank == 0) write_dead_row<kPolicy>(a, row);
+        }
+        return;
+      }
+      const T* x = static_cast<const T*>(a.logits) + row * a.row_stride;
+      Part p;
+      p.m = row_offset(r.x_target);
+      {
+        const float2 v = lane < kRowWarps ? sh.warp_part[par][lane] : make_float2(0.0f, 0.0f);
+        const float t = (r.edge - p.m) * r.scale, e = ex2_approx(t);
+        p.s = warp_sum(v.x + e);
+        p.u = ENT ? warp_sum(v.y + e * fmaxf(t, -200.0f)) : 0.0f;
+      }
+      if (blocks > 1) {
+        // a peer may be one join ahead of this block, never two: two barriers take turns
+        const int turn = int(joined & 1);
+        if (lane == 0) mbar_arrive_expect_tx(&sh.bar[turn], uint32_t(blocks) * 8);
+        __syncwarp();
+        if (lane < blocks) send(peer_addr(&sh.part[turn][rank], lane), p.s, p.u, peer_addr(&sh.bar[turn], lane));
+        if (!bad) bad = __any_sync(~0u, !mbar_wait_bounded(&sh.bar[turn], (joined >> 1) & 1));
+        ++joined;
+        const float2 v = lane < blocks ? sh.part[turn][lane] : make_float2(0.0f, 0.0f);
+        p.s = warp_sum(v.x);
+        if (ENT) p.u = warp_sum(v.y);
+      }
+      if (bad) p.s = NAN;               // a wait ran out: the row has no result
+      if (sums_far(p.s)) {
+        // one warp per block: a row whose target is all but impossible is rare
+        Part q = {-INFINITY, 0.0f, 0.0f};
+        const Span sp = row_span<E>(x, a.vocab);
+        const uint4* vec = reinterpret_cast<const uint4*>(x + sp.head);
+        const int64_t v1 = sp.nv * (rank + 1) / blocks;
+        for (int64_t v = sp.nv * rank / blocks + lane; v < v1; v += 32) {
+          float f[E];
+          D::unpack(vec[v], f);
+          add<ENT>(q, f, r.scale);
+        }
+        const float f[1] = {r.edge};
+        add<ENT>(q, f, r.scale);
+        p = warp_join<ENT>(q, r.scale);
+        if (blocks > 1) {
+          if (lane == 0) mbar_arrive_expect_tx(&sh.far_bar, uint32_t(blocks) * 16);
+          __syncwarp();
+          if (lane < blocks) {
+            const uint32_t dst = peer_addr(&sh.far_part[rank], lane), bar = peer_addr(&sh.far_bar, lane);
+            send(dst, p.m, p.s, bar);
+            send(dst + 8, p.u, 0.0f, bar);
+          }
+          bad = __any_sync(~0u, !mbar_wait_bounded(&sh.far_bar, far_phase));
+          far_phase ^= 1;
+          const float4 v = lane < blocks ? sh.far_part[lane] : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+          p = warp_join<ENT>(Part{v.x, v.y, v.z}, r.scale);
+        }
+      }
+      if (bad) p.s = NAN;
+      const RowResult res = finish<ENT>(p, r.x_target, r.scale);
+      const PolicyRow l = policy_row(a, r.in, res.logprob, res.entropy);
+      const GradRow g = grad_row<ENT>(p.m, res.log2s, r.scale, r.inv_t, l.a, l.h, res.entropy, r.target, r.x_target);
+      if (lane == 0) {
+        sh.coef[par] = g;
+        sh.coef_alive[par] = 1;
+        if (rank == 0) {
+          a.logprobs[row] = float(res.logprob);
+          if (ENT) a.entropy[row] = res.entropy;
+          a.stats[2 * row] = p.m;
+          a.stats[2 * row + 1] = res.log2s;
+          write_policy_row(a, row, l);
+        }
+      }
+      // the gradient of the elements outside the vectors
+      T* out = static_cast<T*>(a.grad_logits) + row * a.grad_stride;
+      const Span sp = row_span<E>(x, a.vocab);
+      const int64_t tail = sp.head + sp.nv * E + lane - 16;
+      const bool head = rank == 0 && lane < sp.head, last = rank == blocks - 1 && lane >= 16 && tail < a.vocab;
+      if (head || last) {
+        const int64_t j = head ? lane : tail;
+        if (g.zero)
+          D::store(out + j, 0.0f);
+        else
+          grad_element<DT, ENT>(g, r.edge, out, j);
+      }
+    };
+    int64_t target_ahead = load_target(1);
+    RowIn prev = {}, cur = load_row(0, load_target(0));
+    publish(0, cur);
+    row_barrier();
+    for (int64_t k = 0; k < rows; ++k) {
+      const RowIn next = load_row(k + 1, target_ahead);
+      target_ahead = load_target(k + 2);
+      if (k > 0) finish_row(k - 1, prev);
+      publish(k + 1, next);
+      prev = cur;
+      cur = next;
+      row_barrier();
+    }
+    finish_row(rows - 1, prev);
+    row_barrier();
+  } else {
+    // -------------------------------------------------------------- row warps
+    uint4* ring = reinterpret_cast<uint4*>(dyn) + warp * kMaxSlots * kChunkVecs;
+    uint64_t* full = full_all + warp * kMaxSlots;
+    const uint64_t policy = l2_policy_evict_first();
+    // this warp's vectors [v0, v0 + n) of a row whose first vector lies `head` elements in
+    struct Share {
+      int64_t head;
+      int v0, n;
+    };
+    auto share = [&](const void* base) {
+      const Span sp = row_span<E>(base, a.vocab);
+      const int b0 = int(sp.nv * rank / blocks), bn = int(sp.nv * (rank + 1) / blocks) - b0;
+      const int w0 = bn * warp / kRowWarps;
+      return Share{sp.head, b0 + w0, bn * (warp + 1) / kRowWarps - w0};
+    };
+    // producer: the next chunk to copy is chunk `pj` of `pn` vectors at `psrc`, of row `pk`
+    int64_t pk = -1, window = -1;
+    uint32_t window_alive = 0;
+    const uint4* psrc = nullptr;
+    int pj = 0, pn = 0, pslot = 0, in_ring = 0;
+    bool bad = false;
+    auto produce = [&]() {
+      while (in_ring < kMaxSlots && pk < rows && !bad) {
+        if (pj >= pn) {
+          if (++pk >= rows) return;
+          if ((pk >> 5) != window) {        // which of the next 32 rows hold a token
+            window = pk >> 5;
+            const int64_t k = (window << 5) + lane;
+            float w;
+            window_alive = __ballot_sync(~0u, k < rows && row_alive<kPolicy>(a, first_row + k * clusters, w));
+          }
+          pj = pn = 0;
+          if (!((window_alive >> (pk & 31)) & 1)) continue;
+          const T* x = static_cast<const T*>(a.logits) + (first_row + pk * clusters) * a.row_stride;
+          const Share s = share(x);
+          psrc = reinterpret_cast<const uint4*>(x + s.head) + s.v0;
+          pn = s.n;
+          continue;
+        }
+        if (lane == 0) {
+          const uint32_t bytes = uint32_t(min(kChunkVecs, pn - pj)) * 16;
+          mbar_arrive_expect_tx(full + pslot, bytes);
+          bulk_g2s(ring + pslot * kChunkVecs, psrc + pj, bytes, full + pslot, policy);
+        }
+        pj += kChunkVecs;
+        pslot = pslot + 1 == kMaxSlots ? 0 : pslot + 1;
+        ++in_ring;
+      }
+    };
+    int sslot = 0, gslot = 0;
+    uint32_t sphase = 0;
+    auto sums = [&](int64_t k) {
+      const RowInfo info = sh.info[k & 1];
+      if (!info.alive) return;
+      const Share s = share(static_cast<const T*>(a.logits) + (first_row + k * clusters) * a.row_stride);
+      const F2 minus_c = f2(-info.c, -info.c), scale = f2(info.scale, info.scale);
+      const uint4 none = make_uint4(D::kNegInf2, D::kNegInf2, D::kNegInf2, D::kNegInf2);
+      F2 sum[2] = {0, 0}, u[2] = {0, 0};
+      for (int j = 0; j < s.n; j += kChunkVecs) {
+        if (!bad) bad = __any_sync(~0u, !mbar_wait_bounded(full + sslot, sphase));
+        const uint4* q = ring + sslot * kChunkVecs;
+        const uint4 q0 = j + lane < s.n ? q[lane] : none, q1 = j + 32 + lane < s.n ? q[32 + lane] : none;
+        add_vector<DT, ENT>(q0, minus_c, scale, sum[0], u[0]);
+        add_vector<DT, ENT>(q1, minus_c, scale, sum[1], u[1]);
+        if (++sslot == kMaxSlots) {
+          sslot = 0;
+          sphase ^= 1;
+        }
+      }
+      float lo, hi;
+      split(add2(sum[0], sum[1]), lo, hi);
+      const float total = warp_sum(lo + hi);
+      split(add2(u[0], u[1]), lo, hi);
+      const float mean = ENT ? warp_sum(lo + hi) : 0.0f;
+      if (lane == 0) sh.warp_part[k & 1][warp] = make_float2(bad ? NAN : total, mean);
+    };
+    auto gradient = [&](int64_t k) {
+      const int64_t row = first_row + k * clusters;
+      T* out = static_cast<T*>(a.grad_logits) + row * a.grad_stride;
+      if (!sh.coef_alive[k & 1]) {
+        const Share s = share(out);
+        uint4* dst = reinterpret_cast<uint4*>(out + s.head) + s.v0;
+        for (int v = lane; v < s.n; v += 32) dst[v] = make_uint4(0, 0, 0, 0);
+        const Span sp = row_span<E>(out, a.vocab);
+        const int64_t tail = sp.head + sp.nv * E + lane;
+        if (rank == 0 && warp == 0 && lane < sp.head) D::store(out + lane, 0.0f);
+        if (rank == blocks - 1 && warp == 0 && tail < a.vocab) D::store(out + tail, 0.0f);
+        return;
+      }
+      const GradRow g = sh.coef[k & 1];
+      const T* x = static_cast<const T*>(a.logits) + row * a.row_stride;
+      const Share s = share(x);
+      const bool same = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+      for (int j = 0; j < s.n; j += kChunkVecs) {
+        const uint4* q = ring + gslot * kChunkVecs;
+        const int n = min(kChunkVecs, s.n - j);
+        const int64_t col = s.head + int64_t(s.v0 + j) * E;
+        if (!same) {            // the rows start on different 16-byte phases: element by element
+          const T* e = reinterpret_cast<const T*>(q);
+          for (int i = lane; i < n * E; i += 32)
+            if (g.zero)
+              D::store(out + col + i, 0.0f);
+            else
+              grad_element<DT, ENT>(g, D::load(e + i), out, col + i);
+        } else if (g.zero) {
+          for (int v = lane; v < n; v += 32) *reinterpret_cast<uint4*>(out + col + v * E) = make_uint4(0, 0, 0, 0);
+        } else {
+          if (lane < n) grad_vector<DT, ENT>(g, q[lane], out, col + lane * E);
+          if (lane + 32 < n) grad_vector<DT, ENT>(g, q[lane + 32], out, col + (lane + 32) * E);
+        }
+        gslot = gslot + 1 == kMaxSlots ? 0 : gslot + 1;
+        __syncwarp();             // the chunk has been read: its slot may be filled again
+        --in_ring;
+        produce();
+      }
+    };
+    produce();
+    row_barrier();
+    for (int64_t k = 0; k < rows; ++k) {
+      sums(k);
+      row_barrier();
+      if (k > 0) gradient(k - 1);
+    }
+    row_barrier();
+    gradient(rows - 1);
+    // after a wait that ran out, copies may still be on their way into this block
+    if (bad)
+      for (int i = 0; i < kMaxSlots; ++i) mbar_wait_bounded(full + i, sphase);
+  }
+  cluster.sync();        // no block leaves while a peer may still write to it
+}
+
 constexpr int kGradVecs = 8;    // vectors of a thread
 
 // The gradient alone: one block per (row, chunk of kThreads x kGradVecs vectors).
@@ -725,7 +1043,7 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(const LossArgs a, int ch
                                   ENT ? a.entropy[row] : 0.0f, target, target < a.vocab ? D::load(x + target) : NAN);
   const Span sp = row_span<E>(x, a.vocab);
   if (((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(out)) & 15) != 0) {
-    write_gradient<DT, ENT>(g, x, out, a.vocab, 0, nullptr, chunk, chunks);
+    write_elements<DT, ENT>(g, x, out, a.vocab, chunk, chunks);
     return;
   }
   const int v0 = int(sp.nv * chunk / chunks), n = int(sp.nv * (chunk + 1) / chunks) - v0;
@@ -763,37 +1081,12 @@ int sm_count(int* out) {
   return NS_OK;
 }
 
-template <int DT, bool ENT, int OP, bool GRAD>
-int launch_forward(const LossArgs& base, cudaStream_t stream) {
-  int sms = 0;
-  if (const int rc = sm_count(&sms)) return rc;
-  LossArgs a = base;
-  const int64_t vectors = a.vocab / Elem<DT>::E;
-  // blocks per row: enough to give every SM two, each thread at least one vector
-  int blocks = 1;
-  while (blocks < kMaxCluster && a.rows * blocks < 2 * sms && vectors >= int64_t(2) * blocks * kThreads) blocks *= 2;
-  size_t smem = 0;
-  if (GRAD) {
-    // the row stays in the cluster's shared memory, as far as kKeepBytes of a block go
-    while (blocks < kMaxCluster && vectors * 16 > int64_t(blocks) * kKeepBytes) blocks *= 2;
-    const int64_t per = (vectors + blocks - 1) / blocks;
-    a.keep = int(std::min<int64_t>((per + kThreads - 1) / kThreads, kKeepBytes / (16 * kThreads)));
-    smem = size_t(a.keep) * kThreads * 16;
-    static std::mutex mu;
-    static bool configured[64];
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return NS_ERR_CUDA;
-    std::lock_guard<std::mutex> lk(mu);
-    if (!configured[dev]) {
-      if (cudaFuncSetAttribute(forward_kernel<DT, ENT, OP, GRAD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               kKeepBytes) != cudaSuccess)
-        return NS_ERR_CUDA;
-      configured[dev] = true;
-    }
-  }
+template <typename... Args>
+int launch_clusters(void (*kernel)(Args...), int64_t grid, int threads, int blocks, size_t smem, cudaStream_t stream,
+                    Args... args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(a.rows * blocks));
-  cfg.blockDim = dim3(kThreads);
+  cfg.gridDim = dim3(unsigned(grid));
+  cfg.blockDim = dim3(unsigned(threads));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute at[1];
@@ -802,23 +1095,94 @@ int launch_forward(const LossArgs& base, cudaStream_t stream) {
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, forward_kernel<DT, ENT, OP, GRAD>, a) == cudaSuccess ? NS_OK : NS_ERR_CUDA;
+  return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? NS_OK : NS_ERR_CUDA;
 }
 
-template <int OP, bool GRAD, int DT>
+template <int DT, bool ENT, int OP>
+int launch_forward(const LossArgs& a, cudaStream_t stream) {
+  int sms = 0;
+  if (const int rc = sm_count(&sms)) return rc;
+  const int64_t vectors = a.vocab / Elem<DT>::E;
+  // blocks per row: enough to give every SM two, each thread at least one vector
+  int blocks = 1;
+  while (blocks < kMaxCluster && a.rows * blocks < 2 * sms && vectors >= int64_t(2) * blocks * kThreads) blocks *= 2;
+  return launch_clusters(forward_kernel<DT, ENT, OP>, a.rows * blocks, kThreads, blocks, 0, stream, a);
+}
+
+template <int OP, int DT>
 int forward_typed(const LossArgs& a, cudaStream_t stream) {
   if constexpr (OP == kPreference)
-    return launch_forward<DT, false, OP, GRAD>(a, stream);
+    return launch_forward<DT, false, OP>(a, stream);
   else
-    return a.entropy ? launch_forward<DT, true, OP, GRAD>(a, stream) : launch_forward<DT, false, OP, GRAD>(a, stream);
+    return a.entropy ? launch_forward<DT, true, OP>(a, stream) : launch_forward<DT, false, OP>(a, stream);
 }
 
-template <int OP, bool GRAD = false>
+template <int OP>
 int forward(const LossArgs& a, int dtype, cudaStream_t stream) {
   switch (dtype) {
-    case NS_DTYPE_F32: return forward_typed<OP, GRAD, NS_DTYPE_F32>(a, stream);
-    case NS_DTYPE_BF16: return forward_typed<OP, GRAD, NS_DTYPE_BF16>(a, stream);
-    default: return forward_typed<OP, GRAD, NS_DTYPE_F16>(a, stream);
+    case NS_DTYPE_F32: return forward_typed<OP, NS_DTYPE_F32>(a, stream);
+    case NS_DTYPE_BF16: return forward_typed<OP, NS_DTYPE_BF16>(a, stream);
+    default: return forward_typed<OP, NS_DTYPE_F16>(a, stream);
+  }
+}
+
+// Blocks per row of policy_kernel: the fewest whose rings hold two rows and two
+// chunks more; 0 when even kMaxCluster blocks do not.
+int pipe_blocks(int64_t vectors) {
+  for (int blocks = 1; blocks <= kMaxCluster; blocks *= 2) {
+    const int64_t block = (vectors + blocks - 1) / blocks, warp = (block + kRowWarps - 1) / kRowWarps;
+    const int64_t chunks = (warp + kChunkVecs - 1) / kChunkVecs;
+    if (2 * chunks + 2 <= kMaxSlots) return blocks;
+  }
+  return 0;
+}
+
+// The clusters of policy_kernel that the current device holds at once.
+template <int DT, bool ENT>
+int pipe_clusters(int blocks, int* out) {
+  static std::mutex mu;
+  static int known[64][kMaxCluster + 1];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return NS_ERR_CUDA;
+  std::lock_guard<std::mutex> lk(mu);
+  if (known[dev][blocks] == 0) {
+    if (cudaFuncSetAttribute(policy_kernel<DT, ENT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPipeSmem) != cudaSuccess)
+      return NS_ERR_CUDA;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned(blocks) * 64);
+    cfg.blockDim = dim3(kPipeThreads);
+    cfg.dynamicSmemBytes = kPipeSmem;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = unsigned(blocks);
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, policy_kernel<DT, ENT>, &cfg) != cudaSuccess || n < 1) return NS_ERR_CUDA;
+    known[dev][blocks] = n;
+  }
+  *out = known[dev][blocks];
+  return NS_OK;
+}
+
+template <int DT, bool ENT>
+int launch_policy(const LossArgs& a, int blocks, cudaStream_t stream) {
+  int clusters = 0;
+  if (const int rc = pipe_clusters<DT, ENT>(blocks, &clusters)) return rc;
+  const int64_t grid = std::min<int64_t>(a.rows, clusters) * blocks;
+  return launch_clusters(policy_kernel<DT, ENT>, grid, kPipeThreads, blocks, kPipeSmem, stream, a);
+}
+
+int policy_with_gradient(const LossArgs& a, int dtype, int blocks, cudaStream_t stream) {
+  const bool ent = a.entropy != nullptr;
+  switch (dtype) {
+    case NS_DTYPE_F32:
+      return ent ? launch_policy<NS_DTYPE_F32, true>(a, blocks, stream) : launch_policy<NS_DTYPE_F32, false>(a, blocks, stream);
+    case NS_DTYPE_BF16:
+      return ent ? launch_policy<NS_DTYPE_BF16, true>(a, blocks, stream) : launch_policy<NS_DTYPE_BF16, false>(a, blocks, stream);
+    default:
+      return ent ? launch_policy<NS_DTYPE_F16, true>(a, blocks, stream) : launch_policy<NS_DTYPE_F16, false>(a, blocks, stream);
   }
 }
 
@@ -940,10 +1304,18 @@ int ns_policy_loss(const void* logits, int dtype, int64_t rows, int64_t vocab, i
   a.row_loss = row_loss;
   a.kl = kl;
   a.row_grad = row_grad;
+  a.grad_logprobs = row_grad;
+  a.grad_entropy = entropy_coef != 0.0f ? row_grad + rows : nullptr;
   a.grad_logits = grad_logits;
   a.grad_stride = grad_stride;
-  if (const int rc = grad_logits ? ns::forward<ns::kPolicy, true>(a, dtype, s) : ns::forward<ns::kPolicy>(a, dtype, s))
-    return rc;
+  const int blocks = grad_logits ? ns::pipe_blocks(vocab / (dtype == NS_DTYPE_F32 ? 4 : 8)) : 0;
+  if (blocks) {
+    if (const int rc = ns::policy_with_gradient(a, dtype, blocks, s)) return rc;
+  } else {
+    if (const int rc = ns::forward<ns::kPolicy>(a, dtype, s)) return rc;
+    if (grad_logits)
+      if (const int rc = ns::gradient(a, dtype, s)) return rc;
+  }
   ns::policy_sum_kernel<<<1, 1024, 0, s>>>(a, loss);
   return cudaGetLastError() == cudaSuccess ? NS_OK : NS_ERR_CUDA;
 }
