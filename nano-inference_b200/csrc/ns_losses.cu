@@ -17,8 +17,8 @@
 //   dx_j = (a 1{j = target} - p_j (a + h (ln p_j + H))) / T.
 //
 // Bound: HBM.  A forward reads the logits once, a gradient reads them and
-// writes as many bytes; the policy loss keeps a row in shared memory between
-// its sums and its gradient, and reads it once.
+// writes as many bytes; the policy loss reads a row for its gradient while L2
+// still holds it from its sums.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -165,12 +165,14 @@ struct LossArgs {
 // The row's scale log2(e) / T and 1 / T; NaN for a temperature that gives no
 // distribution.  0 stands for 1.  A denormal T would make the scale infinite
 // and 0 * inf of the largest logit NaN, so it stops at the largest float.
-__device__ __forceinline__ void row_scale(const LossArgs& a, int64_t row, float& s, double& inv_t) {
-  float t = a.temperature ? a.temperature[row] : a.temperature_all;
+__device__ __forceinline__ void row_scale(float t, float& s, double& inv_t) {
   if (t == 0.0f) t = 1.0f;
   const bool ok = t > 0.0f && t < INFINITY;
   s = ok ? fminf(kLog2e / t, 3.402823466e38f) : NAN;
   inv_t = ok ? 1.0 / double(t) : double(NAN);
+}
+__device__ __forceinline__ void row_scale(const LossArgs& a, int64_t row, float& s, double& inv_t) {
+  row_scale(a.temperature ? a.temperature[row] : a.temperature_all, s, inv_t);
 }
 
 // Running (m, S, U) of a part of a row.  m = -inf: nothing but -inf so far.
@@ -304,24 +306,19 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-
-// The row's sums around c over the whole cluster, the same in every thread of it.
+// The sums around c over part `rank` of `parts` of a row, in every thread.
 template <int DT, bool ENT>
-__device__ __forceinline__ Part row_sums(const void* base, int64_t vocab, float c, float scale, RowShared& sh,
-                                         cg::cluster_group& cluster) {
+__device__ __forceinline__ Part part_sums(const void* base, int64_t vocab, float c, float scale, int rank, int parts,
+                                          Part* shared) {
   using D = Elem<DT>;
   using T = typename D::T;
   constexpr int E = D::E;
-  const int blocks = int(cluster.num_blocks()), rank = int(cluster.block_rank());
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const T* row = static_cast<const T*>(base);
   const Span sp = row_span<E>(row, vocab);
-  const int v0 = int(sp.nv * rank / blocks), n = int(sp.nv * (rank + 1) / blocks) - v0;
+  const int v0 = int(sp.nv * rank / parts), n = int(sp.nv * (rank + 1) / parts) - v0;
   const uint4* vec = reinterpret_cast<const uint4*>(row + sp.head) + v0;
   const uint4 none = make_uint4(D::kNegInf2, D::kNegInf2, D::kNegInf2, D::kNegInf2);
-  if (blocks > 1) cluster_arrive();
   uint4 q[kBatch];
 #pragma unroll
   for (int k = 0; k < kBatch; ++k) {
@@ -330,8 +327,8 @@ __device__ __forceinline__ Part row_sums(const void* base, int64_t vocab, float 
   }
   // the elements before the first 16-byte boundary and after the last whole vector
   const int64_t tail = sp.head + sp.nv * E + threadIdx.x;
-  const float edge[2] = {threadIdx.x < sp.head ? D::load(row + threadIdx.x) : -INFINITY,
-                         tail < vocab ? D::load(row + tail) : -INFINITY};
+  const float edge[2] = {rank == 0 && threadIdx.x < sp.head ? D::load(row + threadIdx.x) : -INFINITY,
+                         rank == parts - 1 && tail < vocab ? D::load(row + tail) : -INFINITY};
   const F2 minus_c = f2(-c, -c), scale2 = f2(scale, scale);
   F2 s[2] = {0, 0}, u[2] = {0, 0};
   for (int v = threadIdx.x; v < n; v += kBatch * kThreads) {
@@ -357,18 +354,30 @@ __device__ __forceinline__ Part row_sums(const void* base, int64_t vocab, float 
     p.u = a + b;
   }
 #pragma unroll
-  for (int k = 0; k < 2; ++k)
-    if (rank == (k == 0 ? 0 : blocks - 1)) {
-      const float t = (edge[k] - c) * scale, e = ex2_approx(t);
-      p.s += e;
-      if (ENT) p.u = fmaf(e, fmaxf(t, -200.0f), p.u);
-    }
+  for (int k = 0; k < 2; ++k) {
+    const float t = (edge[k] - c) * scale, e = ex2_approx(t);
+    p.s += e;
+    if (ENT) p.u = fmaf(e, fmaxf(t, -200.0f), p.u);
+  }
   p.s = warp_sum(p.s);
   if (ENT) p.u = warp_sum(p.u);
-  if (lane == 0) sh.warp[warp] = p;
+  if (lane == 0) shared[warp] = p;
   __syncthreads();
-  p.s = warp_sum(lane < kWarps ? sh.warp[lane].s : 0.0f);
-  if (ENT) p.u = warp_sum(lane < kWarps ? sh.warp[lane].u : 0.0f);
+  p.s = warp_sum(lane < kWarps ? shared[lane].s : 0.0f);
+  if (ENT) p.u = warp_sum(lane < kWarps ? shared[lane].u : 0.0f);
+  return p;
+}
+
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// The row's sums around c over the whole cluster, the same in every thread of it.
+template <int DT, bool ENT>
+__device__ __forceinline__ Part row_sums(const void* base, int64_t vocab, float c, float scale, RowShared& sh,
+                                         cg::cluster_group& cluster) {
+  const int blocks = int(cluster.num_blocks()), rank = int(cluster.block_rank()), lane = threadIdx.x & 31;
+  if (blocks > 1) cluster_arrive();
+  Part p = part_sums<DT, ENT>(base, vocab, c, scale, rank, blocks, sh.warp);
   if (blocks > 1) {
     cluster_wait();                    // every block has started: its shared memory may be written
     if (int(threadIdx.x) < blocks) *cluster.map_shared_rank(&sh.block[rank], threadIdx.x) = p;
@@ -467,11 +476,11 @@ __device__ __forceinline__ bool row_alive(const LossArgs& a, int64_t row, float&
 }
 
 // Gradient of one value: g = p (A + B log2 p), log2 p = (x - c) s - log2 S.
-struct GradRow {
+struct alignas(16) GradRow {
   float c, log2s, scale, ca, cb;
   float at;                  // the value at the target
-  bool zero;
-  int64_t target;
+  int zero;
+  int target;                // past the vocabulary: none
 };
 template <bool ENT>
 __device__ __forceinline__ float grad_value(const GradRow& g, float x) {
@@ -490,28 +499,31 @@ __device__ __forceinline__ GradRow grad_row(float c, float log2s, float scale, d
   g.cb = ENT ? -float(double(h) * kLn2 * inv_t) : 0.0f;
   g.at = grad_value<ENT>(g, x_target) + float(double(a) * inv_t);
   g.zero = a == 0.0f && h == 0.0f;
-  g.target = target;
+  g.target = int(target < (int64_t(1) << 24) ? target : int64_t(1) << 24);
   return g;
 }
-// Writes a vector of gradients at out + j, j its first column.
+// The same for a vector; the constants of the row are in pairs.
+struct GradPairs {
+  F2 minus_c, scale, minus_l, ca, cb;
+};
+__device__ __forceinline__ GradPairs grad_pairs(const GradRow& g) {
+  return {f2(-g.c, -g.c), f2(g.scale, g.scale), f2(-g.log2s, -g.log2s), f2(g.ca, g.ca), f2(g.cb, g.cb)};
+}
 template <int DT, bool ENT>
-__device__ __forceinline__ void grad_vector(const GradRow& g, const uint4& q, typename Elem<DT>::T* out, int64_t j) {
+__device__ __forceinline__ uint4 grad_vector(const GradPairs& g, const uint4& q) {
   using D = Elem<DT>;
   float x[D::E];
   D::unpack(q, x);
-  const F2 minus_c = f2(-g.c, -g.c), scale = f2(g.scale, g.scale), minus_l = f2(-g.log2s, -g.log2s);
-  const F2 ca = f2(g.ca, g.ca), cb = f2(g.cb, g.cb);
 #pragma unroll
   for (int i = 0; i < D::E; i += 2) {
     float a, b;
-    const F2 t = fma2(add2(f2(x[i], x[i + 1]), minus_c), scale, minus_l);
+    const F2 t = fma2(add2(f2(x[i], x[i + 1]), g.minus_c), g.scale, g.minus_l);
     split(t, a, b);
     const F2 p = f2(ex2_approx(a), ex2_approx(b));
-    const F2 w = ENT ? fma2(cb, f2(fmaxf(a, -200.0f), fmaxf(b, -200.0f)), ca) : ca;
+    const F2 w = ENT ? fma2(g.cb, f2(fmaxf(a, -200.0f), fmaxf(b, -200.0f)), g.ca) : g.ca;
     split(mul2(p, w), x[i], x[i + 1]);
   }
-  *reinterpret_cast<uint4*>(out + j) = D::pack(x);
-  if (uint64_t(g.target - j) < uint64_t(D::E)) D::store(out + g.target, g.at);   // one thread of the row
+  return D::pack(x);
 }
 template <int DT, bool ENT>
 __device__ __forceinline__ void grad_element(const GradRow& g, float x, typename Elem<DT>::T* out, int64_t j) {
@@ -604,18 +616,6 @@ __device__ __forceinline__ double block_sum(double v, double* shared) {
   return v;
 }
 
-// The policy loss: the rows' losses by their weights, in 64 bits and in one order.
-__global__ void __launch_bounds__(1024) policy_sum_kernel(const LossArgs a, float* loss) {
-  __shared__ double shared[32];
-  double v = 0.0;
-  for (int64_t i = threadIdx.x; i < a.rows; i += 1024) {
-    const double w = a.weights ? double(a.weights[i]) : 1.0 / double(a.rows);
-    if (a.targets[i] >= 0 && w != 0.0) v += w * double(a.row_loss[i]);
-  }
-  v = block_sum(v, shared);
-  if (threadIdx.x == 0) *loss = float(v);
-}
-
 // The pairs: one warp sums a sequence's gains, then the pair's loss, and the
 // rows' coefficients over the gains.
 __global__ void __launch_bounds__(1024) pair_kernel(const LossArgs a, float beta, float smoothing, int average,
@@ -668,402 +668,240 @@ __global__ void __launch_bounds__(1024) pair_kernel(const LossArgs a, float beta
   if (threadIdx.x == 0) *loss = a.pairs ? float(total / double(a.pairs)) : 0.0f;
 }
 
-// ---------------------------------------------------------------------------
-// Policy loss and gradient from one reading of the logits
-// ---------------------------------------------------------------------------
-// Persistent clusters; cluster i takes rows i, i + clusters, ...  Block r of a
-// cluster holds columns of every one of its rows, and each of its kRowWarps row
-// warps a contiguous share of those, which it streams by bulk copies of
-// kChunkVecs vectors into its own ring in shared memory.  A chunk is read
-// twice there, for the row's sums and then for its gradient, and only then
-// refilled, so DRAM sees the logits once.  The scalar warp joins the sums over
-// the block and, through the peers' shared memory, over the cluster, and turns
-// them into the row's loss and coefficients; that chain of latencies (some 2 us)
-// passes while the row warps write the gradient of the row before and add up
-// the row behind, so a ring holds two rows and what is in flight.  One block
-// barrier per row:
-//   row warps     sums(k) | barrier(k) | gradient(k - 1), sums(k + 1) | barrier(k + 1) | ...
-//   scalar warp            barrier(k) | join and finish row k, load row k + 2's numbers | barrier(k + 1) | ...
-constexpr int kRowWarps = 16;
-constexpr int kPipeThreads = (kRowWarps + 1) * 32;
-constexpr int kChunkVecs = 64;
-constexpr int kChunkBytes = kChunkVecs * 16;
-constexpr int kMaxSlots = 14;                 // chunks of a warp's ring
-constexpr uint32_t kPipeSmem = uint32_t(kRowWarps) * kMaxSlots * (kChunkBytes + 8);
+constexpr int kGradVecs = 8;    // vectors of a thread
 
-struct RowInfo {
-  float c, scale;
-  int alive;
-};
-struct PipeShared {
-  uint64_t bar[2];                // sums of the cluster's blocks, by row parity
-  uint64_t far_bar;               // the same for a row that is added up again
-  float2 part[2][kMaxCluster];    // (S, U) of each block
-  float4 far_part[kMaxCluster];   // (m, S, U)
-  float2 warp_part[2][kRowWarps];
-  RowInfo info[2];
-  GradRow coef[2];
-  int coef_alive[2];
-};
-
-__device__ __forceinline__ uint32_t peer_addr(const void* p, int rank) {
-  uint32_t d;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(d) : "r"(smem_addr(p)), "r"(rank));
-  return d;
-}
-// Stores 8 bytes in a peer block's shared memory and counts them on its barrier.
-__device__ __forceinline__ void send(uint32_t dst, float a, float b, uint32_t bar) {
-  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(dst), "f"(a),
-               "f"(b), "r"(bar)
-               : "memory");
-}
-
-// What the scalar warp loads of a row, ahead of its turn.
-struct RowIn {
-  bool alive;
-  int64_t target;
-  float x_target, scale, edge;
-  double inv_t;
-  PolicyIn in;
-};
-
-// The barrier of both kinds of warps.
-__device__ __forceinline__ void row_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(kPipeThreads) : "memory"); }
-
+// Chunk `chunk` of `chunks` of a row's gradient.
 template <int DT, bool ENT>
-__global__ void __launch_bounds__(kPipeThreads, 1) policy_kernel(const LossArgs a) {
+__device__ __forceinline__ void write_chunk(const GradRow& g, const void* base, void* grad, int64_t vocab, int chunk,
+                                            int chunks) {
   using D = Elem<DT>;
   using T = typename D::T;
   constexpr int E = D::E;
-  __shared__ PipeShared sh;
-  extern __shared__ __align__(128) unsigned char dyn[];
-  cg::cluster_group cluster = cg::this_cluster();
-  const int blocks = int(cluster.num_blocks()), rank = int(cluster.block_rank());
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t first_row = blockIdx.x / blocks, clusters = gridDim.x / blocks;
-  const int64_t rows = (a.rows - first_row + clusters - 1) / clusters;     // of this cluster
-  uint64_t* full_all = reinterpret_cast<uint64_t*>(dyn + kRowWarps * kMaxSlots * kChunkBytes);
-  if (threadIdx.x < kRowWarps * kMaxSlots) mbar_init(full_all + threadIdx.x, 1);
-  if (threadIdx.x == 0) {
-    mbar_init(&sh.bar[0], 1);
-    mbar_init(&sh.bar[1], 1);
-    mbar_init(&sh.far_bar, 1);
+  const T* x = static_cast<const T*>(base);
+  T* out = static_cast<T*>(grad);
+  if (g.zero) {
+    write_zeros<DT>(out, vocab, chunk, chunks);
+    return;
   }
-  fence_mbar_init();
-  __syncthreads();
-  cluster.sync();                       // the peers' barriers exist
-
-  if (warp == kRowWarps) {
-    // ------------------------------------------------------------ scalar warp
-    bool bad = false;
-    uint32_t joined = 0, far_phase = 0;      // rows joined over the cluster so far
-    auto load_target = [&](int64_t k) { return k < rows ? a.targets[first_row + k * clusters] : int64_t(-1); };
-    auto load_row = [&](int64_t k, int64_t target) {
-      RowIn r = {};
-      r.target = target;
-      if (k >= rows || target < 0) return r;
-      const int64_t row = first_row + k * clusters;
-      float w;
-      r.alive = row_alive<kPolicy>(a, row, w);
-      const T* x = static_cast<const T*>(a.logits) + row * a.row_stride;
-      r.x_target = target < a.vocab ? D::load(x + target) : NAN;
-      row_scale(a, row, r.scale, r.inv_t);
-      r.in = policy_in(a, row, w);
-      // the first block's lanes 0.. hold the elements before the first vector, the last one's lanes 16.. those after
-      const Span sp = row_span<E>(x, a.vocab);
-      const int64_t tail = sp.head + sp.nv * E + lane - 16;
-      r.edge = -INFINITY;
-      if (rank == 0 && lane < sp.head) r.edge = D::load(x + lane);
-      if (rank == blocks - 1 && lane >= 16 && tail < a.vocab) r.edge = D::load(x + tail);
-      return r;
-    };
-    auto publish = [&](int64_t k, const RowIn& r) {
-      if (lane == 0) sh.info[k & 1] = {row_offset(r.x_target), r.scale, r.alive};
-    };
-    auto finish_row = [&](int64_t k, const RowIn& r) {
-      const int par = int(k & 1);
-      const int64_t row = first_row + k * clusters;
-      if (!r.alive) {
-        if (lane == 0) {
-          sh.coef_alive[par] = 0;
-          if (rank == 0) write_dead_row<kPolicy>(a, row);
-        }
-        return;
-      }
-      const T* x = static_cast<const T*>(a.logits) + row * a.row_stride;
-      Part p;
-      p.m = row_offset(r.x_target);
-      {
-        const float2 v = lane < kRowWarps ? sh.warp_part[par][lane] : make_float2(0.0f, 0.0f);
-        const float t = (r.edge - p.m) * r.scale, e = ex2_approx(t);
-        p.s = warp_sum(v.x + e);
-        p.u = ENT ? warp_sum(v.y + e * fmaxf(t, -200.0f)) : 0.0f;
-      }
-      if (blocks > 1) {
-        // a peer may be one join ahead of this block, never two: two barriers take turns
-        const int turn = int(joined & 1);
-        if (lane == 0) mbar_arrive_expect_tx(&sh.bar[turn], uint32_t(blocks) * 8);
-        __syncwarp();
-        if (lane < blocks) send(peer_addr(&sh.part[turn][rank], lane), p.s, p.u, peer_addr(&sh.bar[turn], lane));
-        if (!bad) bad = __any_sync(~0u, !mbar_wait_bounded(&sh.bar[turn], (joined >> 1) & 1));
-        ++joined;
-        const float2 v = lane < blocks ? sh.part[turn][lane] : make_float2(0.0f, 0.0f);
-        p.s = warp_sum(v.x);
-        if (ENT) p.u = warp_sum(v.y);
-      }
-      if (bad) p.s = NAN;               // a wait ran out: the row has no result
-      if (sums_far(p.s)) {
-        // one warp per block: a row whose target is all but impossible is rare
-        Part q = {-INFINITY, 0.0f, 0.0f};
-        const Span sp = row_span<E>(x, a.vocab);
-        const uint4* vec = reinterpret_cast<const uint4*>(x + sp.head);
-        const int64_t v1 = sp.nv * (rank + 1) / blocks;
-        for (int64_t v = sp.nv * rank / blocks + lane; v < v1; v += 32) {
-          float f[E];
-          D::unpack(vec[v], f);
-          add<ENT>(q, f, r.scale);
-        }
-        const float f[1] = {r.edge};
-        add<ENT>(q, f, r.scale);
-        p = warp_join<ENT>(q, r.scale);
-        if (blocks > 1) {
-          if (lane == 0) mbar_arrive_expect_tx(&sh.far_bar, uint32_t(blocks) * 16);
-          __syncwarp();
-          if (lane < blocks) {
-            const uint32_t dst = peer_addr(&sh.far_part[rank], lane), bar = peer_addr(&sh.far_bar, lane);
-            send(dst, p.m, p.s, bar);
-            send(dst + 8, p.u, 0.0f, bar);
-          }
-          bad = __any_sync(~0u, !mbar_wait_bounded(&sh.far_bar, far_phase));
-          far_phase ^= 1;
-          const float4 v = lane < blocks ? sh.far_part[lane] : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
-          p = warp_join<ENT>(Part{v.x, v.y, v.z}, r.scale);
-        }
-      }
-      if (bad) p.s = NAN;
-      const RowResult res = finish<ENT>(p, r.x_target, r.scale);
-      const PolicyRow l = policy_row(a, r.in, res.logprob, res.entropy);
-      const GradRow g = grad_row<ENT>(p.m, res.log2s, r.scale, r.inv_t, l.a, l.h, res.entropy, r.target, r.x_target);
-      if (lane == 0) {
-        sh.coef[par] = g;
-        sh.coef_alive[par] = 1;
-        if (rank == 0) {
-          a.logprobs[row] = float(res.logprob);
-          if (ENT) a.entropy[row] = res.entropy;
-          a.stats[2 * row] = p.m;
-          a.stats[2 * row + 1] = res.log2s;
-          write_policy_row(a, row, l);
-        }
-      }
-      // the gradient of the elements outside the vectors
-      T* out = static_cast<T*>(a.grad_logits) + row * a.grad_stride;
-      const Span sp = row_span<E>(x, a.vocab);
-      const int64_t tail = sp.head + sp.nv * E + lane - 16;
-      const bool head = rank == 0 && lane < sp.head, last = rank == blocks - 1 && lane >= 16 && tail < a.vocab;
-      if (head || last) {
-        const int64_t j = head ? lane : tail;
-        if (g.zero)
-          D::store(out + j, 0.0f);
-        else
-          grad_element<DT, ENT>(g, r.edge, out, j);
-      }
-    };
-    int64_t target_ahead = load_target(1);
-    RowIn prev = {}, cur = load_row(0, load_target(0));
-    publish(0, cur);
-    row_barrier();
-    for (int64_t k = 0; k < rows; ++k) {
-      const RowIn next = load_row(k + 1, target_ahead);
-      target_ahead = load_target(k + 2);
-      if (k > 0) finish_row(k - 1, prev);
-      publish(k + 1, next);
-      prev = cur;
-      cur = next;
-      row_barrier();
-    }
-    finish_row(rows - 1, prev);
-    row_barrier();
-  } else {
-    // -------------------------------------------------------------- row warps
-    uint4* ring = reinterpret_cast<uint4*>(dyn) + warp * kMaxSlots * kChunkVecs;
-    uint64_t* full = full_all + warp * kMaxSlots;
-    const uint64_t policy = l2_policy_evict_first();
-    // this warp's vectors [v0, v0 + n) of a row whose first vector lies `head` elements in
-    struct Share {
-      int64_t head;
-      int v0, n;
-    };
-    auto share = [&](const void* base) {
-      const Span sp = row_span<E>(base, a.vocab);
-      const int b0 = int(sp.nv * rank / blocks), bn = int(sp.nv * (rank + 1) / blocks) - b0;
-      const int w0 = bn * warp / kRowWarps;
-      return Share{sp.head, b0 + w0, bn * (warp + 1) / kRowWarps - w0};
-    };
-    // producer: the next chunk to copy is chunk `pj` of `pn` vectors at `psrc`, of row `pk`
-    int64_t pk = -1, window = -1;
-    uint32_t window_alive = 0;
-    const uint4* psrc = nullptr;
-    int pj = 0, pn = 0, pslot = 0, in_ring = 0;
-    bool bad = false;
-    auto produce = [&]() {
-      while (in_ring < kMaxSlots && pk < rows && !bad) {
-        if (pj >= pn) {
-          if (++pk >= rows) return;
-          if ((pk >> 5) != window) {        // which of the next 32 rows hold a token
-            window = pk >> 5;
-            const int64_t k = (window << 5) + lane;
-            float w;
-            window_alive = __ballot_sync(~0u, k < rows && row_alive<kPolicy>(a, first_row + k * clusters, w));
-          }
-          pj = pn = 0;
-          if (!((window_alive >> (pk & 31)) & 1)) continue;
-          const T* x = static_cast<const T*>(a.logits) + (first_row + pk * clusters) * a.row_stride;
-          const Share s = share(x);
-          psrc = reinterpret_cast<const uint4*>(x + s.head) + s.v0;
-          pn = s.n;
-          continue;
-        }
-        if (lane == 0) {
-          const uint32_t bytes = uint32_t(min(kChunkVecs, pn - pj)) * 16;
-          mbar_arrive_expect_tx(full + pslot, bytes);
-          bulk_g2s(ring + pslot * kChunkVecs, psrc + pj, bytes, full + pslot, policy);
-        }
-        pj += kChunkVecs;
-        pslot = pslot + 1 == kMaxSlots ? 0 : pslot + 1;
-        ++in_ring;
-      }
-    };
-    int sslot = 0, gslot = 0;
-    uint32_t sphase = 0;
-    auto sums = [&](int64_t k) {
-      const RowInfo info = sh.info[k & 1];
-      if (!info.alive) return;
-      const Share s = share(static_cast<const T*>(a.logits) + (first_row + k * clusters) * a.row_stride);
-      const F2 minus_c = f2(-info.c, -info.c), scale = f2(info.scale, info.scale);
-      const uint4 none = make_uint4(D::kNegInf2, D::kNegInf2, D::kNegInf2, D::kNegInf2);
-      F2 sum[2] = {0, 0}, u[2] = {0, 0};
-      for (int j = 0; j < s.n; j += kChunkVecs) {
-        if (!bad) bad = __any_sync(~0u, !mbar_wait_bounded(full + sslot, sphase));
-        const uint4* q = ring + sslot * kChunkVecs;
-        const uint4 q0 = j + lane < s.n ? q[lane] : none, q1 = j + 32 + lane < s.n ? q[32 + lane] : none;
-        add_vector<DT, ENT>(q0, minus_c, scale, sum[0], u[0]);
-        add_vector<DT, ENT>(q1, minus_c, scale, sum[1], u[1]);
-        if (++sslot == kMaxSlots) {
-          sslot = 0;
-          sphase ^= 1;
-        }
-      }
-      float lo, hi;
-      split(add2(sum[0], sum[1]), lo, hi);
-      const float total = warp_sum(lo + hi);
-      split(add2(u[0], u[1]), lo, hi);
-      const float mean = ENT ? warp_sum(lo + hi) : 0.0f;
-      if (lane == 0) sh.warp_part[k & 1][warp] = make_float2(bad ? NAN : total, mean);
-    };
-    auto gradient = [&](int64_t k) {
-      const int64_t row = first_row + k * clusters;
-      T* out = static_cast<T*>(a.grad_logits) + row * a.grad_stride;
-      if (!sh.coef_alive[k & 1]) {
-        const Share s = share(out);
-        uint4* dst = reinterpret_cast<uint4*>(out + s.head) + s.v0;
-        for (int v = lane; v < s.n; v += 32) dst[v] = make_uint4(0, 0, 0, 0);
-        const Span sp = row_span<E>(out, a.vocab);
-        const int64_t tail = sp.head + sp.nv * E + lane;
-        if (rank == 0 && warp == 0 && lane < sp.head) D::store(out + lane, 0.0f);
-        if (rank == blocks - 1 && warp == 0 && tail < a.vocab) D::store(out + tail, 0.0f);
-        return;
-      }
-      const GradRow g = sh.coef[k & 1];
-      const T* x = static_cast<const T*>(a.logits) + row * a.row_stride;
-      const Share s = share(x);
-      const bool same = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
-      for (int j = 0; j < s.n; j += kChunkVecs) {
-        const uint4* q = ring + gslot * kChunkVecs;
-        const int n = min(kChunkVecs, s.n - j);
-        const int64_t col = s.head + int64_t(s.v0 + j) * E;
-        if (!same) {            // the rows start on different 16-byte phases: element by element
-          const T* e = reinterpret_cast<const T*>(q);
-          for (int i = lane; i < n * E; i += 32)
-            if (g.zero)
-              D::store(out + col + i, 0.0f);
-            else
-              grad_element<DT, ENT>(g, D::load(e + i), out, col + i);
-        } else if (g.zero) {
-          for (int v = lane; v < n; v += 32) *reinterpret_cast<uint4*>(out + col + v * E) = make_uint4(0, 0, 0, 0);
-        } else {
-          if (lane < n) grad_vector<DT, ENT>(g, q[lane], out, col + lane * E);
-          if (lane + 32 < n) grad_vector<DT, ENT>(g, q[lane + 32], out, col + (lane + 32) * E);
-        }
-        gslot = gslot + 1 == kMaxSlots ? 0 : gslot + 1;
-        __syncwarp();             // the chunk has been read: its slot may be filled again
-        --in_ring;
-        produce();
-      }
-    };
-    produce();
-    row_barrier();
-    for (int64_t k = 0; k < rows; ++k) {
-      sums(k);
-      row_barrier();
-      if (k > 0) gradient(k - 1);
-    }
-    row_barrier();
-    gradient(rows - 1);
-    // after a wait that ran out, copies may still be on their way into this block
-    if (bad)
-      for (int i = 0; i < kMaxSlots; ++i) mbar_wait_bounded(full + i, sphase);
+  if (((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(out)) & 15) != 0) {
+    write_elements<DT, ENT>(g, x, out, vocab, chunk, chunks);
+    return;
   }
-  cluster.sync();        // no block leaves while a peer may still write to it
+  const Span sp = row_span<E>(x, vocab);
+  const int v0 = int(sp.nv * chunk / chunks), n = int(sp.nv * (chunk + 1) / chunks) - v0;
+  const int j0 = int(sp.head) + v0 * E;
+  const uint4* src = reinterpret_cast<const uint4*>(x + j0) + threadIdx.x;
+  uint4* dst = reinterpret_cast<uint4*>(out + j0) + threadIdx.x;
+  const GradPairs pairs = grad_pairs(g);
+  uint4 q[kGradVecs];
+#pragma unroll
+  for (int k = 0; k < kGradVecs; ++k)
+    if (int(threadIdx.x) + k * kThreads < n) q[k] = src[k * kThreads];
+#pragma unroll
+  for (int k = 0; k < kGradVecs; ++k)
+    if (int(threadIdx.x) + k * kThreads < n) dst[k * kThreads] = grad_vector<DT, ENT>(pairs, q[k]);
+  // the target's value over its vector, by the thread that wrote it
+  const unsigned at = unsigned(g.target - j0);
+  if (at < unsigned(n) * E && int(at / E) % kThreads == int(threadIdx.x)) D::store(out + g.target, g.at);
+  const int64_t tail = sp.head + sp.nv * E + threadIdx.x;
+  if (chunk == 0 && threadIdx.x < sp.head)
+    grad_element<DT, ENT>(g, D::load(x + threadIdx.x), out, threadIdx.x);
+  if (chunk == chunks - 1 && tail < vocab) grad_element<DT, ENT>(g, D::load(x + tail), out, tail);
 }
-
-constexpr int kGradVecs = 8;    // vectors of a thread
 
 // The gradient alone: one block per (row, chunk of kThreads x kGradVecs vectors).
 template <int DT, bool ENT>
 __global__ void __launch_bounds__(kThreads) grad_kernel(const LossArgs a, int chunks) {
   using D = Elem<DT>;
   using T = typename D::T;
-  constexpr int E = D::E;
   const int64_t row = blockIdx.x / chunks;
   const int chunk = int(blockIdx.x % chunks);
   const T* x = static_cast<const T*>(a.logits) + row * a.row_stride;
   T* out = static_cast<T*>(a.grad_logits) + row * a.grad_stride;
   const float ga = a.grad_logprobs ? a.grad_logprobs[row] : 0.0f;
   const float gh = ENT ? a.grad_entropy[row] : 0.0f;
-  if (a.targets[row] < 0 || (ga == 0.0f && gh == 0.0f)) {
-    write_zeros<DT>(out, a.vocab, chunk, chunks);
-    return;
+  const int64_t target = a.targets[row];
+  GradRow g = {};
+  g.zero = target < 0 || (ga == 0.0f && gh == 0.0f);
+  if (!g.zero) {
+    float scale;
+    double inv_t;
+    row_scale(a, row, scale, inv_t);
+    // every thread reads the target's logit before it writes; in place, the one that uses it is its writer
+    g = grad_row<ENT>(a.stats[2 * row], a.stats[2 * row + 1], scale, inv_t, ga, gh, ENT ? a.entropy[row] : 0.0f, target,
+                      target < a.vocab ? D::load(x + target) : NAN);
+  }
+  write_chunk<DT, ENT>(g, x, out, a.vocab, chunk, chunks);
+}
+
+// ---------------------------------------------------------------------------
+// Policy loss and gradient from one reading of the logits
+// ---------------------------------------------------------------------------
+// A row's gradient needs the row's sums first, so its logits are read twice;
+// the second reading comes soon enough after the first to find them in L2.
+// Blocks take items by a ticket: the sums of row t, in `parts`, then the
+// gradient of row t - lead, in `chunks`.  The block that adds a row's last part
+// joins them in the parts' order and releases the row; a gradient block waits
+// for that.  An item waits only for items of lower tickets, which running
+// blocks hold and which do not wait themselves, so every wait ends; it is
+// bounded all the same.  The lead keeps a gradient from waiting for sums still
+// under way, and with it kLeadBytes of logits between their two readings.
+constexpr int64_t kLeadBytes = 32 << 20;
+constexpr int64_t kPartBytes = 80 << 10;
+constexpr uint32_t kReady = 0x80000000u;
+
+struct PolicyPlan {
+  int parts, chunks;
+  int64_t lead;
+  // in the caller's workspace; the counters are zeroed before the launch
+  uint32_t *ticket, *rows_done, *state;     // state [rows]: parts added, then kReady
+  float2* part;                             // [rows][parts] (S, U)
+  GradRow* coef;                            // [rows]
+  float* loss;
+};
+
+__device__ __forceinline__ uint32_t ld_acquire(const uint32_t* p) {
+  uint32_t v;
+  asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ void st_release(uint32_t* p, uint32_t v) {
+  asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
+}
+
+// The policy loss: the rows' losses by their weights, in 64 bits and in one order.
+__device__ __forceinline__ void sum_rows(const LossArgs& a, float* loss, double* shared) {
+  double v = 0.0;
+  for (int64_t i = threadIdx.x; i < a.rows; i += blockDim.x) {
+    const double w = a.weights ? double(a.weights[i]) : 1.0 / double(a.rows);
+    if (a.targets[i] >= 0 && w != 0.0) v += w * double(__ldcg(a.row_loss + i));
+  }
+  v = block_sum(v, shared);
+  if (threadIdx.x == 0) *loss = float(v);
+}
+__global__ void __launch_bounds__(1024) policy_sum_kernel(const LossArgs a, float* loss) {
+  __shared__ double shared[32];
+  sum_rows(a, loss, shared);
+}
+
+// Part `rank` of a row's sums, and the row when it is the last one.  True: every row is done.
+template <int DT, bool ENT>
+__device__ __forceinline__ bool policy_part(const LossArgs& a, const PolicyPlan& plan, int64_t row, int rank,
+                                            Part* shared, int* flag) {
+  using D = Elem<DT>;
+  using T = typename D::T;
+  float w;
+  if (!row_alive<kPolicy>(a, row, w)) {
+    if (rank != 0) return false;
+    if (threadIdx.x == 0) {
+      write_dead_row<kPolicy>(a, row);
+      __threadfence();
+      *flag = atomicAdd(plan.rows_done, 1u) == uint32_t(a.rows - 1);
+    }
+    __syncthreads();
+    return *flag != 0;
   }
   float scale;
   double inv_t;
   row_scale(a, row, scale, inv_t);
-  // every thread reads the target's logit before it writes; in place, the one that uses it is its writer
+  const T* x = static_cast<const T*>(a.logits) + row * a.row_stride;
   const int64_t target = a.targets[row];
-  const GradRow g = grad_row<ENT>(a.stats[2 * row], a.stats[2 * row + 1], scale, inv_t, ga, gh,
-                                  ENT ? a.entropy[row] : 0.0f, target, target < a.vocab ? D::load(x + target) : NAN);
-  const Span sp = row_span<E>(x, a.vocab);
-  if (((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(out)) & 15) != 0) {
-    write_elements<DT, ENT>(g, x, out, a.vocab, chunk, chunks);
+  const float x_target = target < a.vocab ? D::load(x + target) : NAN;
+  Part p = part_sums<DT, ENT>(x, a.vocab, row_offset(x_target), scale, rank, plan.parts, shared);
+  if (plan.parts > 1) {
+    if (threadIdx.x == 0) {
+      __stcg(plan.part + row * plan.parts + rank, make_float2(p.s, p.u));
+      __threadfence();
+      *flag = atomicAdd(plan.state + row, 1u) == uint32_t(plan.parts - 1);
+      __threadfence();
+    }
+    __syncthreads();
+    if (!*flag) return false;
+    const int lane = threadIdx.x & 31;
+    p.s = p.u = 0.0f;
+    for (int i = lane; i < plan.parts; i += 32) {
+      const float2 v = __ldcg(plan.part + row * plan.parts + i);
+      p.s += v.x;
+      p.u += v.y;
+    }
+    p.s = warp_sum(p.s);
+    if (ENT) p.u = warp_sum(p.u);
+  }
+  if (sums_far(p.s)) p = running_part<DT, ENT>(x, a.vocab, scale, 0, 1, shared);
+  __syncthreads();                     // the flag has been read
+  if (threadIdx.x == 0) {
+    const RowResult r = finish<ENT>(p, x_target, scale);
+    const PolicyRow l = policy_row(a, policy_in(a, row, w), r.logprob, r.entropy);
+    plan.coef[row] = grad_row<ENT>(p.m, r.log2s, scale, inv_t, l.a, l.h, r.entropy, target, x_target);
+    a.row_loss[row] = l.loss;
+    __threadfence();
+    st_release(plan.state + row, kReady);
+    *flag = atomicAdd(plan.rows_done, 1u) == uint32_t(a.rows - 1);
+    __threadfence();
+    a.logprobs[row] = float(r.logprob);
+    if (ENT) a.entropy[row] = r.entropy;
+    a.stats[2 * row] = p.m;
+    a.stats[2 * row + 1] = r.log2s;
+    write_policy_row(a, row, l);
+  }
+  __syncthreads();
+  return *flag != 0;
+}
+
+template <int DT, bool ENT>
+__global__ void __launch_bounds__(kThreads) policy_kernel(const LossArgs a, const PolicyPlan plan) {
+  using T = typename Elem<DT>::T;
+  __shared__ Part shared[kWarps];
+  __shared__ double sums[32];
+  __shared__ GradRow coef;
+  __shared__ uint32_t ticket;
+  __shared__ int flag;
+  if (threadIdx.x == 0) ticket = atomicAdd(plan.ticket, 1u);
+  __syncthreads();
+  // rows of sums before the first gradient, then both, then gradients alone
+  const int64_t lead = min(plan.lead, a.rows), alone = lead * plan.parts, both = plan.parts + plan.chunks;
+  int64_t row, i = ticket;
+  int part = -1, chunk = 0;
+  if (i < alone) {
+    row = i / plan.parts;
+    part = int(i - row * plan.parts);
+  } else {
+    i -= alone;
+    const int64_t mixed = (a.rows - lead) * both;
+    if (i < mixed) {
+      const int64_t t = i / both;
+      const int at = int(i - t * both);
+      row = at < plan.parts ? lead + t : t;
+      part = at < plan.parts ? at : -1;
+      chunk = at - plan.parts;
+    } else {
+      i -= mixed;
+      row = a.rows - lead + i / plan.chunks;
+      chunk = int(i % plan.chunks);
+    }
+  }
+  if (part >= 0) {
+    if (policy_part<DT, ENT>(a, plan, row, part, shared, &flag)) sum_rows(a, plan.loss, sums);
     return;
   }
-  const int v0 = int(sp.nv * chunk / chunks), n = int(sp.nv * (chunk + 1) / chunks) - v0;
-  const int64_t j0 = sp.head + int64_t(v0) * E;
-  const uint4* src = reinterpret_cast<const uint4*>(x + j0);
-  uint4 q[kGradVecs];
-#pragma unroll
-  for (int k = 0; k < kGradVecs; ++k) {
-    const int v = int(threadIdx.x) + k * kThreads;
-    if (v < n) q[k] = src[v];
+  if (threadIdx.x == 0) {
+    float w;
+    if (row_alive<kPolicy>(a, row, w)) {
+      const uint64_t t0 = global_timer_ns();
+      bool ok;
+      while (!(ok = ld_acquire(plan.state + row) == kReady) && global_timer_ns() - t0 < kWaitTimeoutNs) __nanosleep(100);
+      const float4* src = reinterpret_cast<const float4*>(plan.coef + row);
+      float4* dst = reinterpret_cast<float4*>(&coef);
+      dst[0] = __ldcg(src);
+      dst[1] = __ldcg(src + 1);
+      if (!ok) coef.log2s = coef.at = NAN, coef.zero = 0;
+    } else {
+      coef.zero = 1;
+    }
   }
-#pragma unroll
-  for (int k = 0; k < kGradVecs; ++k) {
-    const int v = int(threadIdx.x) + k * kThreads;
-    if (v < n) grad_vector<DT, ENT>(g, q[k], out, j0 + int64_t(v) * E);
-  }
-  const int64_t tail = sp.head + sp.nv * E + threadIdx.x;
-  if (chunk == 0 && threadIdx.x < sp.head)
-    grad_element<DT, ENT>(g, D::load(x + threadIdx.x), out, threadIdx.x);
-  if (chunk == chunks - 1 && tail < a.vocab) grad_element<DT, ENT>(g, D::load(x + tail), out, tail);
+  __syncthreads();
+  write_chunk<DT, ENT>(coef, static_cast<const T*>(a.logits) + row * a.row_stride,
+                       static_cast<T*>(a.grad_logits) + row * a.grad_stride, a.vocab, chunk, plan.chunks);
 }
 
 // ---------------------------------------------------------------------------
@@ -1126,63 +964,59 @@ int forward(const LossArgs& a, int dtype, cudaStream_t stream) {
   }
 }
 
-// Blocks per row of policy_kernel: the fewest whose rings hold two rows and two
-// chunks more; 0 when even kMaxCluster blocks do not.
-int pipe_blocks(int64_t vectors) {
-  for (int blocks = 1; blocks <= kMaxCluster; blocks *= 2) {
-    const int64_t block = (vectors + blocks - 1) / blocks, warp = (block + kRowWarps - 1) / kRowWarps;
-    const int64_t chunks = (warp + kChunkVecs - 1) / kChunkVecs;
-    if (2 * chunks + 2 <= kMaxSlots) return blocks;
-  }
-  return 0;
+// The shape of policy_kernel's work and its workspace: the counters, then the
+// parts and the rows' coefficients.
+struct PolicyShape {
+  int parts, chunks;
+  int64_t lead;
+  size_t counters, part, coef, bytes;
+};
+PolicyShape policy_shape(int64_t rows, int64_t vocab, int elem) {
+  PolicyShape s;
+  const int64_t vectors = vocab * elem / 16, row_bytes = vocab * elem;
+  s.parts = int(std::max<int64_t>(1, (row_bytes + kPartBytes - 1) / kPartBytes));
+  s.chunks = int(std::max<int64_t>(1, (vectors + kThreads * kGradVecs - 1) / (kThreads * kGradVecs)));
+  s.lead = std::max<int64_t>(1, kLeadBytes / row_bytes);
+  const auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+  s.counters = up((2 + size_t(rows)) * 4);
+  s.part = s.counters;
+  s.coef = s.part + up(size_t(rows) * s.parts * sizeof(float2));
+  s.bytes = s.coef + up(size_t(rows) * sizeof(GradRow));
+  return s;
 }
 
-// The clusters of policy_kernel that the current device holds at once.
-template <int DT, bool ENT>
-int pipe_clusters(int blocks, int* out) {
-  static std::mutex mu;
-  static int known[64][kMaxCluster + 1];
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return NS_ERR_CUDA;
-  std::lock_guard<std::mutex> lk(mu);
-  if (known[dev][blocks] == 0) {
-    if (cudaFuncSetAttribute(policy_kernel<DT, ENT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPipeSmem) != cudaSuccess)
-      return NS_ERR_CUDA;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(unsigned(blocks) * 64);
-    cfg.blockDim = dim3(kPipeThreads);
-    cfg.dynamicSmemBytes = kPipeSmem;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = unsigned(blocks);
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, policy_kernel<DT, ENT>, &cfg) != cudaSuccess || n < 1) return NS_ERR_CUDA;
-    known[dev][blocks] = n;
-  }
-  *out = known[dev][blocks];
-  return NS_OK;
+template <int DT>
+int launch_policy(const LossArgs& a, const PolicyPlan& plan, cudaStream_t stream) {
+  const int64_t blocks = a.rows * (plan.parts + plan.chunks);
+  if (blocks > 0x7FFFFFFF) return NS_ERR_INVALID_ARGUMENT;
+  if (a.entropy)
+    policy_kernel<DT, true><<<unsigned(blocks), kThreads, 0, stream>>>(a, plan);
+  else
+    policy_kernel<DT, false><<<unsigned(blocks), kThreads, 0, stream>>>(a, plan);
+  return cudaGetLastError() == cudaSuccess ? NS_OK : NS_ERR_CUDA;
 }
 
-template <int DT, bool ENT>
-int launch_policy(const LossArgs& a, int blocks, cudaStream_t stream) {
-  int clusters = 0;
-  if (const int rc = pipe_clusters<DT, ENT>(blocks, &clusters)) return rc;
-  const int64_t grid = std::min<int64_t>(a.rows, clusters) * blocks;
-  return launch_clusters(policy_kernel<DT, ENT>, grid, kPipeThreads, blocks, kPipeSmem, stream, a);
-}
-
-int policy_with_gradient(const LossArgs& a, int dtype, int blocks, cudaStream_t stream) {
-  const bool ent = a.entropy != nullptr;
+int policy_with_gradient(const LossArgs& a, int dtype, float* loss, void* workspace, size_t workspace_bytes,
+                         cudaStream_t stream) {
+  const PolicyShape s = policy_shape(a.rows, a.vocab, dtype == NS_DTYPE_F32 ? 4 : 2);
+  if (!workspace || workspace_bytes < s.bytes || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0)
+    return NS_ERR_WORKSPACE_TOO_SMALL;
+  unsigned char* ws = static_cast<unsigned char*>(workspace);
+  PolicyPlan plan;
+  plan.parts = s.parts;
+  plan.chunks = s.chunks;
+  plan.lead = s.lead;
+  plan.ticket = reinterpret_cast<uint32_t*>(ws);
+  plan.rows_done = plan.ticket + 1;
+  plan.state = plan.ticket + 2;
+  plan.part = reinterpret_cast<float2*>(ws + s.part);
+  plan.coef = reinterpret_cast<GradRow*>(ws + s.coef);
+  plan.loss = loss;
+  if (cudaMemsetAsync(ws, 0, s.counters, stream) != cudaSuccess) return NS_ERR_CUDA;
   switch (dtype) {
-    case NS_DTYPE_F32:
-      return ent ? launch_policy<NS_DTYPE_F32, true>(a, blocks, stream) : launch_policy<NS_DTYPE_F32, false>(a, blocks, stream);
-    case NS_DTYPE_BF16:
-      return ent ? launch_policy<NS_DTYPE_BF16, true>(a, blocks, stream) : launch_policy<NS_DTYPE_BF16, false>(a, blocks, stream);
-    default:
-      return ent ? launch_policy<NS_DTYPE_F16, true>(a, blocks, stream) : launch_policy<NS_DTYPE_F16, false>(a, blocks, stream);
+    case NS_DTYPE_F32: return launch_policy<NS_DTYPE_F32>(a, plan, stream);
+    case NS_DTYPE_BF16: return launch_policy<NS_DTYPE_BF16>(a, plan, stream);
+    default: return launch_policy<NS_DTYPE_F16>(a, plan, stream);
   }
 }
 
@@ -1271,12 +1105,20 @@ int ns_token_logprobs_grad(const void* logits, int dtype, int64_t rows, int64_t 
   return ns::gradient(a, dtype, reinterpret_cast<cudaStream_t>(stream));
 }
 
+int ns_policy_loss_workspace_bytes(int dtype, int64_t rows, int64_t vocab, size_t* out_bytes) {
+  if (!out_bytes) return NS_ERR_INVALID_ARGUMENT;
+  if (const int rc = ns::check_rows(dtype, rows, vocab, vocab, nullptr, 1.0f)) return rc;
+  *out_bytes = rows ? ns::policy_shape(rows, vocab, dtype == NS_DTYPE_F32 ? 4 : 2).bytes : 0;
+  return NS_OK;
+}
+
 int ns_policy_loss(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t row_stride,
                    const int64_t* targets, const float* temperature, float temperature_all,
                    const float* old_logprobs, const float* ref_logprobs, const float* advantages,
                    const float* weights, float clip_low, float clip_high, float kl_coef, float entropy_coef,
                    float* loss, float* row_loss, float* logprobs, float* entropy, float* kl, float* stats,
-                   float* row_grad, void* grad_logits, int64_t grad_stride, ns_stream_t stream) {
+                   float* row_grad, void* grad_logits, int64_t grad_stride, void* workspace, size_t workspace_bytes,
+                   ns_stream_t stream) {
   if (const int rc = ns::check_rows(dtype, rows, vocab, row_stride, temperature, temperature_all)) return rc;
   if (!(clip_low >= 0.0f && clip_low <= 1.0f) || !(clip_high >= 0.0f && clip_high < INFINITY) ||
       !std::isfinite(kl_coef) || !std::isfinite(entropy_coef))
@@ -1304,18 +1146,12 @@ int ns_policy_loss(const void* logits, int dtype, int64_t rows, int64_t vocab, i
   a.row_loss = row_loss;
   a.kl = kl;
   a.row_grad = row_grad;
-  a.grad_logprobs = row_grad;
-  a.grad_entropy = entropy_coef != 0.0f ? row_grad + rows : nullptr;
-  a.grad_logits = grad_logits;
-  a.grad_stride = grad_stride;
-  const int blocks = grad_logits ? ns::pipe_blocks(vocab / (dtype == NS_DTYPE_F32 ? 4 : 8)) : 0;
-  if (blocks) {
-    if (const int rc = ns::policy_with_gradient(a, dtype, blocks, s)) return rc;
-  } else {
-    if (const int rc = ns::forward<ns::kPolicy>(a, dtype, s)) return rc;
-    if (grad_logits)
-      if (const int rc = ns::gradient(a, dtype, s)) return rc;
+  if (grad_logits) {
+    a.grad_logits = grad_logits;
+    a.grad_stride = grad_stride;
+    return ns::policy_with_gradient(a, dtype, loss, workspace, workspace_bytes, s);
   }
+  if (const int rc = ns::forward<ns::kPolicy>(a, dtype, s)) return rc;
   ns::policy_sum_kernel<<<1, 1024, 0, s>>>(a, loss);
   return cudaGetLastError() == cudaSuccess ? NS_OK : NS_ERR_CUDA;
 }
