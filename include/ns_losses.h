@@ -30,9 +30,7 @@
  *     stride): the gradient then takes their place.  No other overlap.  The
  *     columns past vocab are left as they are.
  *   - Sums are fp32 per thread and joined in a fixed order: equal inputs give
- *     equal bits.  A workspace needs no particular contents on entry and
- *     leaves nothing the next call reads, but two calls that overlap on the
- *     device must not share one.
+ *     equal bits.  No call needs a workspace or leaves state for the next.
  *
  *   stats fp32 [rows][2], written by the forward calls and read by the
  *   gradient: an offset c (a logit of the row) and log2 of sum exp((x - c) / T).
@@ -82,18 +80,13 @@ int ns_token_logprobs_grad(const void* logits, int dtype, int64_t rows, int64_t 
  * when entropy_coef is 0; kl fp32 [rows] or NULL (it needs ref_logprobs);
  * stats as above; row_grad fp32 [2][rows]: dloss/dlogprob, then dloss/dentropy
  * (what ns_token_logprobs_grad takes).  grad_logits: dloss/dlogits, or NULL.
- * workspace: with grad_logits, ns_policy_loss_workspace_bytes bytes of device
- * scratch, 256-byte aligned (NS_ERR_WORKSPACE_TOO_SMALL otherwise); else NULL.
  */
-int ns_policy_loss_workspace_bytes(int dtype, int64_t rows, int64_t vocab, size_t* out_bytes);
-
 int ns_policy_loss(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t row_stride,
                    const int64_t* targets, const float* temperature, float temperature_all,
                    const float* old_logprobs, const float* ref_logprobs, const float* advantages,
                    const float* weights, float clip_low, float clip_high, float kl_coef, float entropy_coef,
                    float* loss, float* row_loss, float* logprobs, float* entropy, float* kl, float* stats,
-                   float* row_grad, void* grad_logits, int64_t grad_stride, void* workspace, size_t workspace_bytes,
-                   ns_stream_t stream);
+                   float* row_grad, void* grad_logits, int64_t grad_stride, ns_stream_t stream);
 
 /*
  * Preference loss on pairs of sequences whose tokens are packed row after row:

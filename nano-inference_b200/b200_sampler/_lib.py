@@ -108,13 +108,11 @@ PROTOTYPES = {
         *_ROWS, _c_vp, _c_vp,                        # stats, entropy
         _c_vp, _c_vp, _c_vp, _c_i64, _c_vp,          # grad_logprobs, grad_entropy, grad_logits, grad_stride, stream
     ]),
-    "ns_policy_loss_workspace_bytes": (_c_int, [_c_int, _c_i64, _c_i64, ctypes.POINTER(_c_sz)]),
     "ns_policy_loss": (_c_int, [
         *_ROWS, _c_vp, _c_vp, _c_vp, _c_vp,          # old_logprobs, ref_logprobs, advantages, weights
         _c_f32, _c_f32, _c_f32, _c_f32,              # clip_low, clip_high, kl_coef, entropy_coef
         _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp,    # loss, row_loss, logprobs, entropy, kl, stats
-        _c_vp, _c_vp, _c_i64,                        # row_grad, grad_logits, grad_stride
-        _c_vp, _c_sz, _c_vp,                         # workspace, workspace_bytes, stream
+        _c_vp, _c_vp, _c_i64, _c_vp,                 # row_grad, grad_logits, grad_stride, stream
     ]),
     "ns_preference_loss": (_c_int, [
         *_ROWS, _c_vp, _c_i64, _c_vp,                # seq_offsets, pairs, ref_logprobs

@@ -26,7 +26,6 @@ counterpart (its sampler returns ids alone, ``sampling/sampler.py:36-91``).
 """
 from __future__ import annotations
 
-import ctypes
 import math
 from typing import NamedTuple, Optional, Tuple, Union
 
@@ -220,17 +219,6 @@ def _policy(logits, targets, old_logprobs, advantages, ref_logprobs, weights, te
     return logits, targets, temperature, t_all, vectors, (clip_low, clip_high, kl_coef, entropy_coef)
 
 
-def _workspace(logits: torch.Tensor):
-    """Scratch of one ns_policy_loss call, from the caching allocator (whose
-    blocks are 512-byte aligned): a call, and a captured graph, has its own."""
-    need = ctypes.c_size_t()
-    rc = _lib.load().ns_policy_loss_workspace_bytes(_DTYPES[logits.dtype], logits.shape[0], logits.shape[1],
-                                                    ctypes.byref(need))
-    if rc != _lib.NS_OK:
-        raise ValueError(f"ns_policy_loss_workspace_bytes: {_lib.status_string(rc)}")
-    return torch.empty(max(need.value, 1), dtype=torch.uint8, device=logits.device), need.value
-
-
 def _policy_forward(logits, targets, temperature, t_all, vectors, coefs, grad):
     """(PolicyLoss, stats, row_grad [2, rows]); writes dloss/dlogits to ``grad`` when there is one."""
     n = logits.shape[0]
@@ -238,10 +226,9 @@ def _policy_forward(logits, targets, temperature, t_all, vectors, coefs, grad):
     entropy = _new(logits, n) if coefs[3] != 0.0 else None
     kl = _new(logits, n) if vectors[1] is not None else None
     stats, row_grad = _new(logits, n, 2), _new(logits, 2, n)
-    ws, ws_bytes = (None, 0) if grad is None else _workspace(logits)
     _call("ns_policy_loss", logits.device, *_head(logits, targets, temperature, t_all), *(_ptr(v) for v in vectors),
           *coefs, loss.data_ptr(), row_loss.data_ptr(), logprobs.data_ptr(), _ptr(entropy), _ptr(kl),
-          stats.data_ptr(), row_grad.data_ptr(), _ptr(grad), 0 if grad is None else _stride(grad), _ptr(ws), ws_bytes)
+          stats.data_ptr(), row_grad.data_ptr(), _ptr(grad), 0 if grad is None else _stride(grad))
     return PolicyLoss(loss, row_loss, logprobs, entropy, kl), stats, row_grad
 
 

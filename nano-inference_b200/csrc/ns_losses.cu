@@ -17,8 +17,8 @@
 //   dx_j = (a 1{j = target} - p_j (a + h (ln p_j + H))) / T.
 //
 // Bound: HBM.  A forward reads the logits once, a gradient reads them and
-// writes as many bytes; the policy loss reads a row for its gradient while L2
-// still holds it from its sums.
+// writes as many bytes; the policy loss keeps a row on chip between its sums
+// and its gradient, and reads it once.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -543,14 +543,14 @@ __device__ __forceinline__ void write_elements(const GradRow& g, const void* bas
 
 // Zeros in block `rank`'s share of a row.
 template <int DT>
-__device__ __forceinline__ void write_zeros(void* grad, int64_t vocab, int rank, int blocks) {
+__device__ __forceinline__ void write_zeros(void* grad, int64_t vocab, int rank, int blocks, int threads = kThreads) {
   using T = typename Elem<DT>::T;
   constexpr int E = Elem<DT>::E;
   T* out = static_cast<T*>(grad);
   const Span sp = row_span<E>(out, vocab);
   uint4* dst = reinterpret_cast<uint4*>(out + sp.head);
   const int v1 = int(sp.nv * (rank + 1) / blocks);
-  for (int v = int(sp.nv * rank / blocks) + threadIdx.x; v < v1; v += kThreads) dst[v] = make_uint4(0, 0, 0, 0);
+  for (int v = int(sp.nv * rank / blocks) + threadIdx.x; v < v1; v += threads) dst[v] = make_uint4(0, 0, 0, 0);
   const int64_t tail = sp.head + sp.nv * E + threadIdx.x;
   if (rank == 0 && threadIdx.x < sp.head) Elem<DT>::store(out + threadIdx.x, 0.0f);
   if (rank == blocks - 1 && tail < vocab) Elem<DT>::store(out + tail, 0.0f);
@@ -614,6 +614,18 @@ __device__ __forceinline__ double block_sum(double v, double* shared) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
   return v;
+}
+
+// The policy loss: the rows' losses by their weights, in 64 bits and in one order.
+__global__ void __launch_bounds__(1024) policy_sum_kernel(const LossArgs a, float* loss) {
+  __shared__ double shared[32];
+  double v = 0.0;
+  for (int64_t i = threadIdx.x; i < a.rows; i += 1024) {
+    const double w = a.weights ? double(a.weights[i]) : 1.0 / double(a.rows);
+    if (a.targets[i] >= 0 && w != 0.0) v += w * double(a.row_loss[i]);
+  }
+  v = block_sum(v, shared);
+  if (threadIdx.x == 0) *loss = float(v);
 }
 
 // The pairs: one warp sums a sequence's gains, then the pair's loss, and the
@@ -737,171 +749,391 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(const LossArgs a, int ch
 // ---------------------------------------------------------------------------
 // Policy loss and gradient from one reading of the logits
 // ---------------------------------------------------------------------------
-// A row's gradient needs the row's sums first, so its logits are read twice;
-// the second reading comes soon enough after the first to find them in L2.
-// Blocks take items by a ticket: the sums of row t, in `parts`, then the
-// gradient of row t - lead, in `chunks`.  The block that adds a row's last part
-// joins them in the parts' order and releases the row; a gradient block waits
-// for that.  An item waits only for items of lower tickets, which running
-// blocks hold and which do not wait themselves, so every wait ends; it is
-// bounded all the same.  The lead keeps a gradient from waiting for sums still
-// under way, and with it kLeadBytes of logits between their two readings.
-constexpr int64_t kLeadBytes = 32 << 20;
-constexpr int64_t kPartBytes = 80 << 10;
-constexpr uint32_t kReady = 0x80000000u;
+// A row's gradient needs the row's sums first, so a block keeps the row (or a
+// cluster's block its share of it) on chip between the two.  Persistent
+// clusters; cluster i takes rows i, i + clusters, ...  A producer warp copies
+// rows in chunks into a ring in shared memory.  The row warps add a row up as
+// its chunks land: the first chunks they keep in registers and hand back at
+// once, the others stay in the ring.  They join their sums (over the cluster
+// through the peers' shared memory) and write the gradient, the ring's chunks
+// first, handing each back as it is done, so the reads of the next row run
+// under the writes of this one.  The logits cross L2 and DRAM once.  The rows
+// that hold no token come last.
+//
+// What bounds it: 2 exponentials a logit are 70 % of the time that bf16's 4
+// bytes a logit need, and a row's sums cannot end before its last chunk lands.
+// Loading the registers straight from memory instead was slower (10 us a row of
+// 123 KB): beside 215 KB of shared memory L1 has room for few loads.
+constexpr int kRowWarps = 15;
+constexpr int kRowThreads = kRowWarps * 32;
+constexpr int kHeldThreads = kRowThreads + 32;      // and the producer warp
+constexpr int kLaneVecs = 2;                        // of a chunk
+constexpr int kChunkVecs = kRowThreads * kLaneVecs;
+constexpr int kChunkBytes = kChunkVecs * 16;
 
-struct PolicyPlan {
-  int parts, chunks;
-  int64_t lead;
-  // in the caller's workspace; the counters are zeroed before the launch
-  uint32_t *ticket, *rows_done, *state;     // state [rows]: parts added, then kReady
-  float2* part;                             // [rows][parts] (S, U)
-  GradRow* coef;                            // [rows]
-  float* loss;
+// Two shapes: one block of an SM with registers, or two with smaller rings.
+template <bool LARGE>
+struct HeldShape {
+  static constexpr int kHold = LARGE ? 8 : 0;       // chunks in registers
+  static constexpr int kSlots = LARGE ? 14 : 7;
+  static constexpr int kBlocks = LARGE ? 1 : 2;
+  static constexpr int kMostVecs = (kHold + kSlots - 1) * kChunkVecs;
+  static constexpr uint32_t kSmem = uint32_t(kSlots) * kChunkBytes;
 };
 
-__device__ __forceinline__ uint32_t ld_acquire(const uint32_t* p) {
-  uint32_t v;
-  asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
-  return v;
-}
-__device__ __forceinline__ void st_release(uint32_t* p, uint32_t v) {
-  asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
-}
+struct RowInfo {
+  int64_t target;
+  float x_target, t;      // t: the temperature
+  PolicyIn in;
+};
+struct HeldShared {
+  uint64_t full[16], empty[16];    // of the ring's chunks
+  uint64_t bar[2];                 // sums of the cluster's blocks, by turn
+  uint64_t far_bar;                // the same for a row that is added up again
+  float2 part[2][kMaxCluster];     // (S, U) of each block
+  float4 far_part[kMaxCluster];    // (m, S, U)
+  float2 warp_part[kRowWarps];
+  Part far_warp[kRowWarps];
+  RowInfo info[16];                // of the row whose first chunk lies in the slot
+  GradRow coef;
+  int far;
+};
 
-// The policy loss: the rows' losses by their weights, in 64 bits and in one order.
-__device__ __forceinline__ void sum_rows(const LossArgs& a, float* loss, double* shared) {
-  double v = 0.0;
-  for (int64_t i = threadIdx.x; i < a.rows; i += blockDim.x) {
-    const double w = a.weights ? double(a.weights[i]) : 1.0 / double(a.rows);
-    if (a.targets[i] >= 0 && w != 0.0) v += w * double(__ldcg(a.row_loss + i));
+__device__ __forceinline__ uint32_t peer_addr(const void* p, int rank) {
+  uint32_t d;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(d) : "r"(smem_addr(p)), "r"(rank));
+  return d;
+}
+// Stores 8 bytes in a peer block's shared memory and counts them on its barrier.
+__device__ __forceinline__ void send(uint32_t dst, float a, float b, uint32_t bar) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(dst), "f"(a),
+               "f"(b), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+// The barrier of the row warps.
+__device__ __forceinline__ void row_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(kRowThreads) : "memory"); }
+
+// The rows of a cluster that hold a token, or those that do not, in order.
+struct RowWalk {
+  int64_t rows, window = -1;
+  uint32_t mask = 0;
+  // the first such row from k on, or `rows`
+  __device__ __forceinline__ int64_t next(const LossArgs& a, int64_t first_row, int64_t clusters, int64_t k, bool alive) {
+    const int lane = threadIdx.x & 31;
+    while (k < rows) {
+      if ((k >> 5) != window) {
+        window = k >> 5;
+        const int64_t i = (window << 5) + lane;
+        float w;
+        mask = __ballot_sync(~0u, i < rows && row_alive<kPolicy>(a, first_row + i * clusters, w) == alive);
+      }
+      const uint32_t left = mask >> (k & 31);
+      if (left) return k + __ffs(left) - 1;
+      k = (window + 1) << 5;
+    }
+    return rows;
   }
-  v = block_sum(v, shared);
-  if (threadIdx.x == 0) *loss = float(v);
-}
-__global__ void __launch_bounds__(1024) policy_sum_kernel(const LossArgs a, float* loss) {
-  __shared__ double shared[32];
-  sum_rows(a, loss, shared);
+};
+
+// A block's vectors [v0, v0 + n) of a row that starts at `base`; `shift` is log2 of the cluster's blocks.
+struct Share {
+  int head, v0, n;
+};
+template <int E>
+__device__ __forceinline__ Share row_share(const void* base, int vocab, int rank, int shift) {
+  Share s;
+  s.head = min(vocab, int(((16 - (uint32_t(reinterpret_cast<uintptr_t>(base)) & 15)) & 15) / (16 / E)));
+  const int nv = (vocab - s.head) / E;          // at most 2^22, and rank + 1 at most 2^3
+  s.v0 = nv * rank >> shift;
+  s.n = (nv * (rank + 1) >> shift) - s.v0;
+  return s;
 }
 
-// Part `rank` of a row's sums, and the row when it is the last one.  True: every row is done.
-template <int DT, bool ENT>
-__device__ __forceinline__ bool policy_part(const LossArgs& a, const PolicyPlan& plan, int64_t row, int rank,
-                                            Part* shared, int* flag) {
+template <int DT, bool ENT, bool LARGE>
+__global__ void __launch_bounds__(kHeldThreads, HeldShape<LARGE>::kBlocks)
+    policy_kernel(const __grid_constant__ LossArgs a) {
   using D = Elem<DT>;
   using T = typename D::T;
-  float w;
-  if (!row_alive<kPolicy>(a, row, w)) {
-    if (rank != 0) return false;
-    if (threadIdx.x == 0) {
-      write_dead_row<kPolicy>(a, row);
-      __threadfence();
-      *flag = atomicAdd(plan.rows_done, 1u) == uint32_t(a.rows - 1);
-    }
-    __syncthreads();
-    return *flag != 0;
+  using H = HeldShape<LARGE>;
+  constexpr int E = D::E, kHold = H::kHold, kSlots = H::kSlots;
+  __shared__ HeldShared sh;
+  extern __shared__ __align__(128) uint4 ring[];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int blocks = int(cluster.num_blocks()), rank = int(cluster.block_rank());
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
+  const int shift = 31 - __clz(blocks);           // blocks is a power of two
+  const int64_t first_row = blockIdx.x >> shift, clusters = gridDim.x >> shift;
+  const int64_t rows = (a.rows - first_row + clusters - 1) / clusters;     // of this cluster
+  if (tid < kSlots) {
+    mbar_init(&sh.full[tid], 1);
+    mbar_init(&sh.empty[tid], kRowWarps);
   }
-  float scale;
-  double inv_t;
-  row_scale(a, row, scale, inv_t);
-  const T* x = static_cast<const T*>(a.logits) + row * a.row_stride;
-  const int64_t target = a.targets[row];
-  const float x_target = target < a.vocab ? D::load(x + target) : NAN;
-  Part p = part_sums<DT, ENT>(x, a.vocab, row_offset(x_target), scale, rank, plan.parts, shared);
-  if (plan.parts > 1) {
-    if (threadIdx.x == 0) {
-      __stcg(plan.part + row * plan.parts + rank, make_float2(p.s, p.u));
-      __threadfence();
-      *flag = atomicAdd(plan.state + row, 1u) == uint32_t(plan.parts - 1);
-      __threadfence();
-    }
-    __syncthreads();
-    if (!*flag) return false;
-    const int lane = threadIdx.x & 31;
-    p.s = p.u = 0.0f;
-    for (int i = lane; i < plan.parts; i += 32) {
-      const float2 v = __ldcg(plan.part + row * plan.parts + i);
-      p.s += v.x;
-      p.u += v.y;
-    }
-    p.s = warp_sum(p.s);
-    if (ENT) p.u = warp_sum(p.u);
+  if (tid == 0) {
+    mbar_init(&sh.bar[0], 1);
+    mbar_init(&sh.bar[1], 1);
+    mbar_init(&sh.far_bar, 1);
   }
-  if (sums_far(p.s)) p = running_part<DT, ENT>(x, a.vocab, scale, 0, 1, shared);
-  __syncthreads();                     // the flag has been read
-  if (threadIdx.x == 0) {
-    const RowResult r = finish<ENT>(p, x_target, scale);
-    const PolicyRow l = policy_row(a, policy_in(a, row, w), r.logprob, r.entropy);
-    plan.coef[row] = grad_row<ENT>(p.m, r.log2s, scale, inv_t, l.a, l.h, r.entropy, target, x_target);
-    a.row_loss[row] = l.loss;
-    __threadfence();
-    st_release(plan.state + row, kReady);
-    *flag = atomicAdd(plan.rows_done, 1u) == uint32_t(a.rows - 1);
-    __threadfence();
-    a.logprobs[row] = float(r.logprob);
-    if (ENT) a.entropy[row] = r.entropy;
-    a.stats[2 * row] = p.m;
-    a.stats[2 * row + 1] = r.log2s;
-    write_policy_row(a, row, l);
-  }
+  fence_mbar_init();
   __syncthreads();
-  return *flag != 0;
-}
+  if (blocks > 1) cluster.sync();       // the peers' barriers exist
+  const auto logits_row = [&](int64_t k) { return static_cast<const T*>(a.logits) + (first_row + k * clusters) * a.row_stride; };
+  const auto grad_out = [&](int64_t k) { return static_cast<T*>(a.grad_logits) + (first_row + k * clusters) * a.grad_stride; };
+  RowWalk walk;
+  walk.rows = rows;
 
-template <int DT, bool ENT>
-__global__ void __launch_bounds__(kThreads) policy_kernel(const LossArgs a, const PolicyPlan plan) {
-  using T = typename Elem<DT>::T;
-  __shared__ Part shared[kWarps];
-  __shared__ double sums[32];
-  __shared__ GradRow coef;
-  __shared__ uint32_t ticket;
-  __shared__ int flag;
-  if (threadIdx.x == 0) ticket = atomicAdd(plan.ticket, 1u);
-  __syncthreads();
-  // rows of sums before the first gradient, then both, then gradients alone
-  const int64_t lead = min(plan.lead, a.rows), alone = lead * plan.parts, both = plan.parts + plan.chunks;
-  int64_t row, i = ticket;
-  int part = -1, chunk = 0;
-  if (i < alone) {
-    row = i / plan.parts;
-    part = int(i - row * plan.parts);
+  if (warp == kRowWarps) {
+    // ------------------------------------------------------------ producer warp
+    const uint64_t policy = l2_policy_evict_first();
+    int slot = 0;
+    uint32_t phase = 1;                 // the first round finds the slots empty
+    bool bad = false;
+    int64_t window = -1;
+    RowInfo mine = {};                  // lane i: row `window` * 32 + i
+    for (int64_t k = walk.next(a, first_row, clusters, 0, true); k < rows && !bad;
+         k = walk.next(a, first_row, clusters, k + 1, true)) {
+      if ((k >> 5) != window) {
+        window = k >> 5;
+        const int64_t i = (window << 5) + lane;
+        if (i < rows) {
+          const int64_t row = first_row + i * clusters;
+          mine.target = a.targets[row];
+          mine.t = a.temperature ? a.temperature[row] : a.temperature_all;
+          mine.in = policy_in(a, row, a.weights ? a.weights[row] : 1.0f / float(a.rows));
+          mine.x_target = mine.target >= 0 && mine.target < a.vocab ? D::load(logits_row(i) + mine.target) : NAN;
+        }
+      }
+      const T* x = logits_row(k);
+      const Share s = row_share<E>(x, int(a.vocab), rank, shift);
+      const uint4* src = reinterpret_cast<const uint4*>(x + s.head) + s.v0;
+      int at = 0;
+      do {                              // a row has one chunk at least: it carries the row's numbers
+        if (!bad) bad = !mbar_wait_bounded(&sh.empty[slot], phase);
+        bad = __any_sync(~0u, bad);
+        if (bad) break;
+        if (at == 0 && lane == int(k & 31)) sh.info[slot] = mine;
+        __syncwarp();
+        if (lane == 0) {
+          const uint32_t bytes = uint32_t(min(kChunkVecs, s.n - at)) * 16;
+          mbar_arrive_expect_tx(&sh.full[slot], bytes);
+          if (bytes) bulk_g2s(ring + slot * kChunkVecs, src + at, bytes, &sh.full[slot], policy);
+        }
+        at += kChunkVecs;
+        if (++slot == kSlots) {
+          slot = 0;
+          phase ^= 1;
+        }
+      } while (at < s.n);
+    }
+    // the copies end before the block does
+    if (bad)
+      for (int i = 0; i < kSlots; ++i) mbar_wait_bounded(&sh.full[i], phase ^ 1);
   } else {
-    i -= alone;
-    const int64_t mixed = (a.rows - lead) * both;
-    if (i < mixed) {
-      const int64_t t = i / both;
-      const int at = int(i - t * both);
-      row = at < plan.parts ? lead + t : t;
-      part = at < plan.parts ? at : -1;
-      chunk = at - plan.parts;
-    } else {
-      i -= mixed;
-      row = a.rows - lead + i / plan.chunks;
-      chunk = int(i % plan.chunks);
+    // --------------------------------------------------------------- row warps
+    bool bad = false;
+    uint32_t joined = 0, far_phase = 0, phase = 0;
+    int slot = 0;
+    uint4 held[kHold ? kHold : 1][kLaneVecs];
+    // The element of this thread outside the row's vectors: the first block's
+    // threads 0.. hold those before, the last one's threads 16.. those after.
+    const auto edge_column = [&](const Share& s) {
+      const int nv = (int(a.vocab) - s.head) / E, tail = s.head + nv * E + tid - 16;
+      if (rank == 0 && tid < s.head) return tid;
+      return rank == blocks - 1 && tid >= 16 && tail < int(a.vocab) ? tail : -1;
+    };
+    const auto load_edge = [&](const T* x, const Share& s) {
+      const int col = edge_column(s);
+      return col >= 0 ? D::load(x + col) : -INFINITY;
+    };
+    int64_t k = walk.next(a, first_row, clusters, 0, true);
+    float edge = k < rows ? load_edge(logits_row(k), row_share<E>(logits_row(k), int(a.vocab), rank, shift)) : 0.0f;
+    while (k < rows) {
+      const int64_t row = first_row + k * clusters;
+      const T* x = logits_row(k);
+      const Share s = row_share<E>(x, int(a.vocab), rank, shift);
+      // ---- the row's sums, chunk after chunk as they land
+      const int first_slot = slot;
+      F2 sum[2] = {0, 0}, u[2] = {0, 0};
+      if (!bad) bad = !mbar_wait_bounded(&sh.full[slot], phase);
+      const RowInfo info = sh.info[first_slot];
+      const float c = row_offset(info.x_target);
+      float scale;
+      double inv_t;
+      row_scale(info.t, scale, inv_t);
+      const F2 minus_c = f2(-c, -c), scale2 = f2(scale, scale);
+      const auto take = [&](int at, uint4 (&q)[kLaneVecs]) {      // the chunk at vector `at` of the share
+        if (at > 0 && !bad) bad = !mbar_wait_bounded(&sh.full[slot], phase);
+        const uint4* src = ring + slot * kChunkVecs + tid;
+        if (at + kChunkVecs <= s.n) {
+#pragma unroll
+          for (int i = 0; i < kLaneVecs; ++i) q[i] = src[i * kRowThreads];
+#pragma unroll
+          for (int i = 0; i < kLaneVecs; ++i) add_vector<DT, ENT>(q[i], minus_c, scale2, sum[i & 1], u[i & 1]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < kLaneVecs; ++i)
+            if (at + i * kRowThreads + tid < s.n) {
+              q[i] = src[i * kRowThreads];
+              add_vector<DT, ENT>(q[i], minus_c, scale2, sum[i & 1], u[i & 1]);
+            }
+        }
+      };
+      const auto advance = [&]() {
+        if (++slot == kSlots) {
+          slot = 0;
+          phase ^= 1;
+        }
+      };
+      const auto hand_back = [&](int chunk) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.empty[chunk]);
+      };
+#pragma unroll
+      for (int j = 0; j < kHold; ++j)
+        if (j == 0 || j * kChunkVecs < s.n) {
+          take(j * kChunkVecs, held[j]);
+          hand_back(slot);
+          advance();
+        }
+      const int ring_slot = slot;
+      for (int at = kHold * kChunkVecs; at < s.n || at == 0; at += kChunkVecs) {
+        uint4 q[kLaneVecs];
+        take(at, q);
+        advance();
+      }
+      {
+        const float t = (edge - c) * scale, e = ex2_approx(t);
+        float lo, hi;
+        split(add2(sum[0], sum[1]), lo, hi);
+        const float total = warp_sum(lo + hi + e);
+        split(add2(u[0], u[1]), lo, hi);
+        const float mean = ENT ? warp_sum(lo + hi + e * fmaxf(t, -200.0f)) : 0.0f;
+        bad = __any_sync(~0u, bad);
+        if (lane == 0) sh.warp_part[warp] = make_float2(bad ? NAN : total, mean);
+      }
+      row_barrier();
+      // ---- joined, and turned into the row's numbers, by the first warp
+      if (warp == 0) {
+        Part p;
+        {
+          const float2 v = lane < kRowWarps ? sh.warp_part[lane] : make_float2(0.0f, 0.0f);
+          p = {c, warp_sum(v.x), ENT ? warp_sum(v.y) : 0.0f};
+        }
+        if (blocks > 1) {
+          // a peer may be one join ahead of this block, never two: two barriers take turns
+          const int turn = int(joined & 1);
+          if (lane == 0) mbar_arrive_expect_tx(&sh.bar[turn], uint32_t(blocks) * 8);
+          __syncwarp();
+          if (lane < blocks) send(peer_addr(&sh.part[turn][rank], lane), p.s, p.u, peer_addr(&sh.bar[turn], lane));
+          if (!bad) bad = __any_sync(~0u, !mbar_wait_bounded(&sh.bar[turn], (joined >> 1) & 1));
+          ++joined;
+          const float2 v = lane < blocks ? sh.part[turn][lane] : make_float2(0.0f, 0.0f);
+          p.s = warp_sum(v.x);
+          if (ENT) p.u = warp_sum(v.y);
+        }
+        if (bad) p.s = NAN;             // a wait ran out: the row has no result
+        if (sums_far(p.s)) {
+          // one warp of a block: a row whose target is all but impossible is rare
+          Part q = {-INFINITY, 0.0f, 0.0f};
+          const uint4* vec = reinterpret_cast<const uint4*>(x + s.head) + s.v0;
+          for (int v = lane; v < s.n; v += 32) {
+            float f[E];
+            D::unpack(vec[v], f);
+            add<ENT>(q, f, scale);
+          }
+          const Span sp = row_span<E>(x, a.vocab);
+          const int64_t tail = sp.head + sp.nv * E + lane;
+          const float f[2] = {rank == 0 && lane < sp.head ? D::load(x + lane) : -INFINITY,
+                              rank == blocks - 1 && tail < a.vocab ? D::load(x + tail) : -INFINITY};
+          add<ENT>(q, f, scale);
+          p = warp_join<ENT>(q, scale);
+          if (blocks > 1) {
+            if (lane == 0) mbar_arrive_expect_tx(&sh.far_bar, uint32_t(blocks) * 16);
+            __syncwarp();
+            if (lane < blocks) {
+              const uint32_t dst = peer_addr(&sh.far_part[rank], lane), bar = peer_addr(&sh.far_bar, lane);
+              send(dst, p.m, p.s, bar);
+              send(dst + 8, p.u, 0.0f, bar);
+            }
+            bad = __any_sync(~0u, !mbar_wait_bounded(&sh.far_bar, far_phase));
+            far_phase ^= 1;
+            const float4 v = lane < blocks ? sh.far_part[lane] : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+            p = warp_join<ENT>(Part{v.x, v.y, v.z}, scale);
+            if (bad) p.s = NAN;
+          }
+        }
+        if (lane == 0) {
+          const RowResult r = finish<ENT>(p, info.x_target, scale);
+          const PolicyRow l = policy_row(a, info.in, r.logprob, r.entropy);
+          sh.coef = grad_row<ENT>(p.m, r.log2s, scale, inv_t, l.a, l.h, r.entropy, info.target, info.x_target);
+          if (rank == 0) {
+            a.logprobs[row] = float(r.logprob);
+            if (ENT) a.entropy[row] = r.entropy;
+            a.stats[2 * row] = p.m;
+            a.stats[2 * row + 1] = r.log2s;
+            write_policy_row(a, row, l);
+          }
+        }
+      }
+      row_barrier();
+      // ---- its gradient; every chunk goes to the next row as it is done
+      const GradRow g = sh.coef;
+      const int64_t next = walk.next(a, first_row, clusters, k + 1, true);
+      T* out = grad_out(k);
+      if (const int col = edge_column(s); col >= 0) {
+        if (g.zero)
+          D::store(out + col, 0.0f);
+        else
+          grad_element<DT, ENT>(g, edge, out, col);
+      }
+      if (next < rows) edge = load_edge(logits_row(next), row_share<E>(logits_row(next), int(a.vocab), rank, shift));
+      T* mine = out + s.head + int64_t(s.v0) * E;
+      const auto write = [&](const auto& put) {
+        int chunk = ring_slot;
+        for (int at = kHold * kChunkVecs; at < s.n || at == 0; at += kChunkVecs) {
+          const uint4* q = ring + chunk * kChunkVecs + tid;
+#pragma unroll
+          for (int i = 0; i < kLaneVecs; ++i)
+            if (at + i * kRowThreads + tid < s.n) put(q[i * kRowThreads], at + i * kRowThreads + tid);
+          hand_back(chunk);
+          if (++chunk == kSlots) chunk = 0;
+        }
+#pragma unroll
+        for (int j = 0; j < kHold; ++j)
+#pragma unroll
+          for (int i = 0; i < kLaneVecs; ++i)
+            if (const int v = j * kChunkVecs + i * kRowThreads + tid; v < s.n) put(held[j][i], v);
+      };
+      uint4* dst = reinterpret_cast<uint4*>(mine);
+      const GradPairs pairs = grad_pairs(g);
+      if (((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(out)) & 15) != 0) {
+        // the rows start on different 16-byte phases: element by element
+        write([&](const uint4& q, int v) {
+          const uint4 r = g.zero ? make_uint4(0, 0, 0, 0) : grad_vector<DT, ENT>(pairs, q);
+          const T* e = reinterpret_cast<const T*>(&r);
+#pragma unroll
+          for (int i = 0; i < E; ++i) mine[v * E + i] = e[i];
+        });
+      } else if (g.zero) {
+        write([&](const uint4&, int v) { dst[v] = make_uint4(0, 0, 0, 0); });
+      } else {
+        write([&](const uint4& q, int v) { dst[v] = grad_vector<DT, ENT>(pairs, q); });
+      }
+      // the target's value over its vector, by the thread that wrote it
+      const unsigned target = unsigned(g.target - s.head) - unsigned(s.v0) * E;
+      if (!g.zero && target < unsigned(s.n) * E && int(target / E) % kRowThreads == tid) D::store(mine + target, g.at);
+      k = next;
+    }
+    // ---- the rows without a token
+    walk.window = -1;
+    for (k = walk.next(a, first_row, clusters, 0, false); k < rows; k = walk.next(a, first_row, clusters, k + 1, false)) {
+      if (rank == 0 && tid == 0) write_dead_row<kPolicy>(a, first_row + k * clusters);
+      write_zeros<DT>(grad_out(k), a.vocab, rank, blocks, kRowThreads);
     }
   }
-  if (part >= 0) {
-    if (policy_part<DT, ENT>(a, plan, row, part, shared, &flag)) sum_rows(a, plan.loss, sums);
-    return;
-  }
-  if (threadIdx.x == 0) {
-    float w;
-    if (row_alive<kPolicy>(a, row, w)) {
-      const uint64_t t0 = global_timer_ns();
-      bool ok;
-      while (!(ok = ld_acquire(plan.state + row) == kReady) && global_timer_ns() - t0 < kWaitTimeoutNs) __nanosleep(100);
-      const float4* src = reinterpret_cast<const float4*>(plan.coef + row);
-      float4* dst = reinterpret_cast<float4*>(&coef);
-      dst[0] = __ldcg(src);
-      dst[1] = __ldcg(src + 1);
-      if (!ok) coef.log2s = coef.at = NAN, coef.zero = 0;
-    } else {
-      coef.zero = 1;
-    }
-  }
-  __syncthreads();
-  write_chunk<DT, ENT>(coef, static_cast<const T*>(a.logits) + row * a.row_stride,
-                       static_cast<T*>(a.grad_logits) + row * a.grad_stride, a.vocab, chunk, plan.chunks);
+  if (blocks > 1) cluster.sync();        // no block leaves while a peer may still write to it
 }
 
 // ---------------------------------------------------------------------------
@@ -964,60 +1196,68 @@ int forward(const LossArgs& a, int dtype, cudaStream_t stream) {
   }
 }
 
-// The shape of policy_kernel's work and its workspace: the counters, then the
-// parts and the rows' coefficients.
-struct PolicyShape {
-  int parts, chunks;
-  int64_t lead;
-  size_t counters, part, coef, bytes;
-};
-PolicyShape policy_shape(int64_t rows, int64_t vocab, int elem) {
-  PolicyShape s;
-  const int64_t vectors = vocab * elem / 16, row_bytes = vocab * elem;
-  s.parts = int(std::max<int64_t>(1, (row_bytes + kPartBytes - 1) / kPartBytes));
-  s.chunks = int(std::max<int64_t>(1, (vectors + kThreads * kGradVecs - 1) / (kThreads * kGradVecs)));
-  s.lead = std::max<int64_t>(1, kLeadBytes / row_bytes);
-  const auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-  s.counters = up((2 + size_t(rows)) * 4);
-  s.part = s.counters;
-  s.coef = s.part + up(size_t(rows) * s.parts * sizeof(float2));
-  s.bytes = s.coef + up(size_t(rows) * sizeof(GradRow));
-  return s;
+// Blocks per row of policy_kernel: the fewest that hold a row on chip; 0 when kMaxCluster do not.
+template <bool LARGE>
+int held_blocks(int64_t vectors) {
+  for (int blocks = 1; blocks <= kMaxCluster; blocks *= 2)
+    if ((vectors + blocks - 1) / blocks <= HeldShape<LARGE>::kMostVecs) return blocks;
+  return 0;
+}
+
+template <int DT, bool ENT, bool LARGE>
+int launch_policy(const LossArgs& a, int blocks, cudaStream_t stream) {
+  using H = HeldShape<LARGE>;
+  static std::mutex mu;
+  static int known[64][kMaxCluster + 1];         // clusters that a device holds at once
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return NS_ERR_CUDA;
+  int clusters = 0;
+  {
+    std::lock_guard<std::mutex> lk(mu);
+    if (known[dev][blocks] == 0) {
+      if (cudaFuncSetAttribute(policy_kernel<DT, ENT, LARGE>, cudaFuncAttributeMaxDynamicSharedMemorySize, H::kSmem) !=
+          cudaSuccess)
+        return NS_ERR_CUDA;
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(unsigned(blocks) * 64);
+      cfg.blockDim = dim3(kHeldThreads);
+      cfg.dynamicSmemBytes = H::kSmem;
+      cudaLaunchAttribute at[1];
+      at[0].id = cudaLaunchAttributeClusterDimension;
+      at[0].val.clusterDim.x = unsigned(blocks);
+      at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+      cfg.attrs = at;
+      cfg.numAttrs = 1;
+      int n = 0;
+      if (cudaOccupancyMaxActiveClusters(&n, policy_kernel<DT, ENT, LARGE>, &cfg) != cudaSuccess || n < 1) return NS_ERR_CUDA;
+      known[dev][blocks] = n;
+    }
+    clusters = known[dev][blocks];
+  }
+  const int64_t grid = std::min<int64_t>(a.rows, clusters) * blocks;
+  return launch_clusters(policy_kernel<DT, ENT, LARGE>, grid, kHeldThreads, blocks, H::kSmem, stream, a);
 }
 
 template <int DT>
-int launch_policy(const LossArgs& a, const PolicyPlan& plan, cudaStream_t stream) {
-  const int64_t blocks = a.rows * (plan.parts + plan.chunks);
-  if (blocks > 0x7FFFFFFF) return NS_ERR_INVALID_ARGUMENT;
+int policy_typed(const LossArgs& a, int blocks, bool large, cudaStream_t stream) {
   if (a.entropy)
-    policy_kernel<DT, true><<<unsigned(blocks), kThreads, 0, stream>>>(a, plan);
-  else
-    policy_kernel<DT, false><<<unsigned(blocks), kThreads, 0, stream>>>(a, plan);
-  return cudaGetLastError() == cudaSuccess ? NS_OK : NS_ERR_CUDA;
+    return large ? launch_policy<DT, true, true>(a, blocks, stream) : launch_policy<DT, true, false>(a, blocks, stream);
+  return large ? launch_policy<DT, false, true>(a, blocks, stream) : launch_policy<DT, false, false>(a, blocks, stream);
 }
 
-int policy_with_gradient(const LossArgs& a, int dtype, float* loss, void* workspace, size_t workspace_bytes,
-                         cudaStream_t stream) {
-  const PolicyShape s = policy_shape(a.rows, a.vocab, dtype == NS_DTYPE_F32 ? 4 : 2);
-  if (!workspace || workspace_bytes < s.bytes || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0)
-    return NS_ERR_WORKSPACE_TOO_SMALL;
-  unsigned char* ws = static_cast<unsigned char*>(workspace);
-  PolicyPlan plan;
-  plan.parts = s.parts;
-  plan.chunks = s.chunks;
-  plan.lead = s.lead;
-  plan.ticket = reinterpret_cast<uint32_t*>(ws);
-  plan.rows_done = plan.ticket + 1;
-  plan.state = plan.ticket + 2;
-  plan.part = reinterpret_cast<float2*>(ws + s.part);
-  plan.coef = reinterpret_cast<GradRow*>(ws + s.coef);
-  plan.loss = loss;
-  if (cudaMemsetAsync(ws, 0, s.counters, stream) != cudaSuccess) return NS_ERR_CUDA;
+// The gradient with the loss, when a row can be held; false: it cannot.
+bool policy_held(const LossArgs& a, int dtype, cudaStream_t stream, int* rc) {
+  const int64_t vectors = a.vocab / (dtype == NS_DTYPE_F32 ? 4 : 8);
+  const char* env = getenv("NS_LARGE");
+  const bool large = env ? atoi(env) : vectors > HeldShape<false>::kMostVecs;
+  const int blocks = large ? held_blocks<true>(vectors) : held_blocks<false>(vectors);
+  if (blocks == 0 || (env && atoi(env) == 2)) return false;
   switch (dtype) {
-    case NS_DTYPE_F32: return launch_policy<NS_DTYPE_F32>(a, plan, stream);
-    case NS_DTYPE_BF16: return launch_policy<NS_DTYPE_BF16>(a, plan, stream);
-    default: return launch_policy<NS_DTYPE_F16>(a, plan, stream);
+    case NS_DTYPE_F32: *rc = policy_typed<NS_DTYPE_F32>(a, blocks, large, stream); break;
+    case NS_DTYPE_BF16: *rc = policy_typed<NS_DTYPE_BF16>(a, blocks, large, stream); break;
+    default: *rc = policy_typed<NS_DTYPE_F16>(a, blocks, large, stream);
   }
+  return true;
 }
 
 template <int DT>
@@ -1105,20 +1345,12 @@ int ns_token_logprobs_grad(const void* logits, int dtype, int64_t rows, int64_t 
   return ns::gradient(a, dtype, reinterpret_cast<cudaStream_t>(stream));
 }
 
-int ns_policy_loss_workspace_bytes(int dtype, int64_t rows, int64_t vocab, size_t* out_bytes) {
-  if (!out_bytes) return NS_ERR_INVALID_ARGUMENT;
-  if (const int rc = ns::check_rows(dtype, rows, vocab, vocab, nullptr, 1.0f)) return rc;
-  *out_bytes = rows ? ns::policy_shape(rows, vocab, dtype == NS_DTYPE_F32 ? 4 : 2).bytes : 0;
-  return NS_OK;
-}
-
 int ns_policy_loss(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t row_stride,
                    const int64_t* targets, const float* temperature, float temperature_all,
                    const float* old_logprobs, const float* ref_logprobs, const float* advantages,
                    const float* weights, float clip_low, float clip_high, float kl_coef, float entropy_coef,
                    float* loss, float* row_loss, float* logprobs, float* entropy, float* kl, float* stats,
-                   float* row_grad, void* grad_logits, int64_t grad_stride, void* workspace, size_t workspace_bytes,
-                   ns_stream_t stream) {
+                   float* row_grad, void* grad_logits, int64_t grad_stride, ns_stream_t stream) {
   if (const int rc = ns::check_rows(dtype, rows, vocab, row_stride, temperature, temperature_all)) return rc;
   if (!(clip_low >= 0.0f && clip_low <= 1.0f) || !(clip_high >= 0.0f && clip_high < INFINITY) ||
       !std::isfinite(kl_coef) || !std::isfinite(entropy_coef))
@@ -1146,12 +1378,16 @@ int ns_policy_loss(const void* logits, int dtype, int64_t rows, int64_t vocab, i
   a.row_loss = row_loss;
   a.kl = kl;
   a.row_grad = row_grad;
-  if (grad_logits) {
-    a.grad_logits = grad_logits;
-    a.grad_stride = grad_stride;
-    return ns::policy_with_gradient(a, dtype, loss, workspace, workspace_bytes, s);
+  a.grad_logprobs = row_grad;
+  a.grad_entropy = entropy_coef != 0.0f ? row_grad + rows : nullptr;
+  a.grad_logits = grad_logits;
+  a.grad_stride = grad_stride;
+  int rc = NS_OK;
+  if (!grad_logits || !ns::policy_held(a, dtype, s, &rc)) {
+    rc = ns::forward<ns::kPolicy>(a, dtype, s);
+    if (rc == NS_OK && grad_logits) rc = ns::gradient(a, dtype, s);
   }
-  if (const int rc = ns::forward<ns::kPolicy>(a, dtype, s)) return rc;
+  if (rc != NS_OK) return rc;
   ns::policy_sum_kernel<<<1, 1024, 0, s>>>(a, loss);
   return cudaGetLastError() == cudaSuccess ? NS_OK : NS_ERR_CUDA;
 }

@@ -1,7 +1,6 @@
 """Refusals of the operators on sampled tokens' logits (no GPU needed): the C
 entry points reject bad arguments before touching CUDA, and the Python calls
 name what is wrong.  The oracle's formulas are checked against differentiation."""
-import ctypes
 import math
 import os
 
@@ -19,7 +18,7 @@ ENTRIES = {
     "ns_token_logprobs_grad": dict(ROWS, stats=1, entropy=None, a=1, h=None, grad=2, grad_stride=10, stream=None),
     "ns_policy_loss": dict(ROWS, old=1, ref=None, adv=1, weights=None, low=0.2, high=0.2, kl_coef=0.0, entropy_coef=0.0,
                            loss=1, row_loss=1, logprobs=1, entropy=None, kl=None, stats=1, row_grad=1, grad=None,
-                           grad_stride=0, ws=None, ws_bytes=0, stream=None),
+                           grad_stride=0, stream=None),
     "ns_preference_loss": dict(ROWS, offsets=1, pairs=1, ref=None, beta=0.1, smoothing=0.0, average=0, loss=1,
                                pair_loss=1, rewards=1, logprobs=1, stats=1, row_grad=1, grad=None, grad_stride=0,
                                stream=None),
@@ -58,23 +57,6 @@ def test_c_entries_refuse_missing_results_and_bad_numbers():
                dict(logprobs=None), dict(stats=None), dict(row_grad=None), dict(grad=2, grad_stride=9),
                dict(grad=1, grad_stride=12)):
         assert _call("ns_preference_loss", **kw) == BAD, kw
-
-
-@needs_lib
-def test_policy_workspace_is_checked():
-    size = ctypes.c_size_t()
-    query = _lib.load().ns_policy_loss_workspace_bytes
-    assert query(0, 4, 10, ctypes.byref(size)) == _lib.NS_OK and size.value > 0
-    kw = dict(grad=2, grad_stride=10)
-    for ws, n in ((None, 1 << 20), (256, size.value - 1), (256 + 16, size.value)):
-        assert _call("ns_policy_loss", ws=ws, ws_bytes=n, **kw) == _lib.NS_ERR_WORKSPACE_TOO_SMALL
-    one = size.value
-    assert query(1, 4096, 151936, ctypes.byref(size)) == _lib.NS_OK and size.value > one
-    assert query(0, 0, 10, ctypes.byref(size)) == _lib.NS_OK and size.value == 0
-    assert query(5, 4, 10, ctypes.byref(size)) == TYPE
-    for bad in ((0, -1, 10), (0, 4, 0), (0, 4, (1 << 24) + 1), (0, (1 << 24) + 1, 10)):
-        assert query(*bad, ctypes.byref(size)) == BAD
-    assert query(0, 4, 10, None) == BAD
 
 
 @needs_lib
