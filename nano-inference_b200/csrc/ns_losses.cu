@@ -781,9 +781,12 @@ struct HeldShape {
   static constexpr uint32_t kSmem = uint32_t(kSlots) * kChunkBytes;
 };
 
+// What the producer says of a row, with its first chunk.
 struct RowInfo {
+  int64_t k;              // the cluster's row; -1 ends the rows
   int64_t target;
-  float x_target, t;      // t: the temperature
+  double inv_t;
+  float x_target, scale;
   PolicyIn in;
 };
 struct HeldShared {
@@ -881,39 +884,46 @@ __global__ void __launch_bounds__(kHeldThreads, HeldShape<LARGE>::kBlocks)
   if (blocks > 1) cluster.sync();       // the peers' barriers exist
   const auto logits_row = [&](int64_t k) { return static_cast<const T*>(a.logits) + (first_row + k * clusters) * a.row_stride; };
   const auto grad_out = [&](int64_t k) { return static_cast<T*>(a.grad_logits) + (first_row + k * clusters) * a.grad_stride; };
-  RowWalk walk;
-  walk.rows = rows;
 
   if (warp == kRowWarps) {
     // ------------------------------------------------------------ producer warp
     const uint64_t policy = l2_policy_evict_first();
+    RowWalk walk;
+    walk.rows = rows;
     int slot = 0;
     uint32_t phase = 1;                 // the first round finds the slots empty
     bool bad = false;
     int64_t window = -1;
     RowInfo mine = {};                  // lane i: row `window` * 32 + i
-    for (int64_t k = walk.next(a, first_row, clusters, 0, true); k < rows && !bad;
-         k = walk.next(a, first_row, clusters, k + 1, true)) {
-      if ((k >> 5) != window) {
-        window = k >> 5;
-        const int64_t i = (window << 5) + lane;
-        if (i < rows) {
-          const int64_t row = first_row + i * clusters;
-          mine.target = a.targets[row];
-          mine.t = a.temperature ? a.temperature[row] : a.temperature_all;
-          mine.in = policy_in(a, row, a.weights ? a.weights[row] : 1.0f / float(a.rows));
-          mine.x_target = mine.target >= 0 && mine.target < a.vocab ? D::load(logits_row(i) + mine.target) : NAN;
+    for (int64_t k = 0; k >= 0 && !bad;) {
+      k = walk.next(a, first_row, clusters, k, true);
+      const bool end = k >= rows;
+      Share s = {};
+      const uint4* src = nullptr;
+      if (!end) {
+        if ((k >> 5) != window) {
+          window = k >> 5;
+          mine.k = (window << 5) + lane;
+          if (mine.k < rows) {
+            const int64_t row = first_row + mine.k * clusters;
+            mine.target = a.targets[row];
+            row_scale(a, row, mine.scale, mine.inv_t);
+            mine.in = policy_in(a, row, a.weights ? a.weights[row] : 1.0f / float(a.rows));
+            mine.x_target = mine.target >= 0 && mine.target < a.vocab ? D::load(logits_row(mine.k) + mine.target) : NAN;
+          }
         }
+        const T* x = logits_row(k);
+        s = row_share<E>(x, int(a.vocab), rank, shift);
+        src = reinterpret_cast<const uint4*>(x + s.head) + s.v0;
       }
-      const T* x = logits_row(k);
-      const Share s = row_share<E>(x, int(a.vocab), rank, shift);
-      const uint4* src = reinterpret_cast<const uint4*>(x + s.head) + s.v0;
       int at = 0;
       do {                              // a row has one chunk at least: it carries the row's numbers
-        if (!bad) bad = !mbar_wait_bounded(&sh.empty[slot], phase);
-        bad = __any_sync(~0u, bad);
+        bad = __any_sync(~0u, !mbar_wait_bounded(&sh.empty[slot], phase));
         if (bad) break;
-        if (at == 0 && lane == int(k & 31)) sh.info[slot] = mine;
+        if (at == 0) {
+          if (end && lane == 0) sh.info[slot].k = -1;
+          if (!end && lane == int(k & 31)) sh.info[slot] = mine;
+        }
         __syncwarp();
         if (lane == 0) {
           const uint32_t bytes = uint32_t(min(kChunkVecs, s.n - at)) * 16;
@@ -926,6 +936,7 @@ __global__ void __launch_bounds__(kHeldThreads, HeldShape<LARGE>::kBlocks)
           phase ^= 1;
         }
       } while (at < s.n);
+      k = end ? -1 : k + 1;
     }
     // the copies end before the block does
     if (bad)
@@ -936,33 +947,33 @@ __global__ void __launch_bounds__(kHeldThreads, HeldShape<LARGE>::kBlocks)
     uint32_t joined = 0, far_phase = 0, phase = 0;
     int slot = 0;
     uint4 held[kHold ? kHold : 1][kLaneVecs];
-    // The element of this thread outside the row's vectors: the first block's
-    // threads 0.. hold those before, the last one's threads 16.. those after.
-    const auto edge_column = [&](const Share& s) {
-      const int nv = (int(a.vocab) - s.head) / E, tail = s.head + nv * E + tid - 16;
-      if (rank == 0 && tid < s.head) return tid;
-      return rank == blocks - 1 && tid >= 16 && tail < int(a.vocab) ? tail : -1;
-    };
-    const auto load_edge = [&](const T* x, const Share& s) {
-      const int col = edge_column(s);
-      return col >= 0 ? D::load(x + col) : -INFINITY;
-    };
-    int64_t k = walk.next(a, first_row, clusters, 0, true);
-    float edge = k < rows ? load_edge(logits_row(k), row_share<E>(logits_row(k), int(a.vocab), rank, shift)) : 0.0f;
-    while (k < rows) {
-      const int64_t row = first_row + k * clusters;
-      const T* x = logits_row(k);
-      const Share s = row_share<E>(x, int(a.vocab), rank, shift);
+    // Rows whose stride is whole vectors all start at the same phase: the share is looked up anew only for another.
+    Share s = {};
+    int edge_at = -1;
+    uint32_t start = ~0u;
+    int64_t done = 0;
+    while (true) {
       // ---- the row's sums, chunk after chunk as they land
       const int first_slot = slot;
       F2 sum[2] = {0, 0}, u[2] = {0, 0};
       if (!bad) bad = !mbar_wait_bounded(&sh.full[slot], phase);
-      const RowInfo info = sh.info[first_slot];
-      const float c = row_offset(info.x_target);
-      float scale;
-      double inv_t;
-      row_scale(info.t, scale, inv_t);
+      const int64_t k = bad ? -1 : sh.info[first_slot].k;
+      if (k < 0) break;
+      done = k + 1;
+      const T* x = logits_row(k);
+      if ((uint32_t(reinterpret_cast<uintptr_t>(x)) & 15) != start) {
+        start = uint32_t(reinterpret_cast<uintptr_t>(x)) & 15;
+        s = row_share<E>(x, int(a.vocab), rank, shift);
+        // the element of this thread outside the row's vectors: the first block's threads 0.. hold those before,
+        // the last one's threads 16.. those after
+        const int nv = (int(a.vocab) - s.head) / E, tail = s.head + nv * E + tid - 16;
+        edge_at = rank == 0 && tid < s.head ? tid : rank == blocks - 1 && tid >= 16 && tail < int(a.vocab) ? tail : -1;
+      }
+      const float edge = edge_at >= 0 ? D::load(x + edge_at) : -INFINITY;
+      const float c = row_offset(sh.info[first_slot].x_target), scale = sh.info[first_slot].scale;
       const F2 minus_c = f2(-c, -c), scale2 = f2(scale, scale);
+      RowInfo info;
+      if (warp == 0) info = sh.info[first_slot];
       const auto take = [&](int at, uint4 (&q)[kLaneVecs]) {      // the chunk at vector `at` of the share
         if (at > 0 && !bad) bad = !mbar_wait_bounded(&sh.full[slot], phase);
         const uint4* src = ring + slot * kChunkVecs + tid;
@@ -1016,6 +1027,7 @@ __global__ void __launch_bounds__(kHeldThreads, HeldShape<LARGE>::kBlocks)
       row_barrier();
       // ---- joined, and turned into the row's numbers, by the first warp
       if (warp == 0) {
+        const int64_t row = first_row + k * clusters;
         Part p;
         {
           const float2 v = lane < kRowWarps ? sh.warp_part[lane] : make_float2(0.0f, 0.0f);
@@ -1065,9 +1077,9 @@ __global__ void __launch_bounds__(kHeldThreads, HeldShape<LARGE>::kBlocks)
           }
         }
         if (lane == 0) {
-          const RowResult r = finish<ENT>(p, info.x_target, scale);
+          const RowResult r = finish<ENT>(p, info.x_target, info.scale);
           const PolicyRow l = policy_row(a, info.in, r.logprob, r.entropy);
-          sh.coef = grad_row<ENT>(p.m, r.log2s, scale, inv_t, l.a, l.h, r.entropy, info.target, info.x_target);
+          sh.coef = grad_row<ENT>(p.m, r.log2s, info.scale, info.inv_t, l.a, l.h, r.entropy, info.target, info.x_target);
           if (rank == 0) {
             a.logprobs[row] = float(r.logprob);
             if (ENT) a.entropy[row] = r.entropy;
@@ -1080,15 +1092,13 @@ __global__ void __launch_bounds__(kHeldThreads, HeldShape<LARGE>::kBlocks)
       row_barrier();
       // ---- its gradient; every chunk goes to the next row as it is done
       const GradRow g = sh.coef;
-      const int64_t next = walk.next(a, first_row, clusters, k + 1, true);
       T* out = grad_out(k);
-      if (const int col = edge_column(s); col >= 0) {
+      if (edge_at >= 0) {
         if (g.zero)
-          D::store(out + col, 0.0f);
+          D::store(out + edge_at, 0.0f);
         else
-          grad_element<DT, ENT>(g, edge, out, col);
+          grad_element<DT, ENT>(g, edge, out, edge_at);
       }
-      if (next < rows) edge = load_edge(logits_row(next), row_share<E>(logits_row(next), int(a.vocab), rank, shift));
       T* mine = out + s.head + int64_t(s.v0) * E;
       const auto write = [&](const auto& put) {
         int chunk = ring_slot;
@@ -1124,11 +1134,16 @@ __global__ void __launch_bounds__(kHeldThreads, HeldShape<LARGE>::kBlocks)
       // the target's value over its vector, by the thread that wrote it
       const unsigned target = unsigned(g.target - s.head) - unsigned(s.v0) * E;
       if (!g.zero && target < unsigned(s.n) * E && int(target / E) % kRowThreads == tid) D::store(mine + target, g.at);
-      k = next;
     }
     // ---- the rows without a token
-    walk.window = -1;
-    for (k = walk.next(a, first_row, clusters, 0, false); k < rows; k = walk.next(a, first_row, clusters, k + 1, false)) {
+    RowWalk walk;
+    walk.rows = rows;
+    if (bad) {                             // nor have those behind a wait that ran out
+      for (int64_t k = walk.next(a, first_row, clusters, done, true); k < rows; k = walk.next(a, first_row, clusters, k + 1, true))
+        if (tid == 0) a.logprobs[first_row + k * clusters] = a.row_loss[first_row + k * clusters] = NAN;
+      walk.window = -1;
+    }
+    for (int64_t k = walk.next(a, first_row, clusters, 0, false); k < rows; k = walk.next(a, first_row, clusters, k + 1, false)) {
       if (rank == 0 && tid == 0) write_dead_row<kPolicy>(a, first_row + k * clusters);
       write_zeros<DT>(grad_out(k), a.vocab, rank, blocks, kRowThreads);
     }
