@@ -25,5 +25,6 @@ def __getattr__(name):
         return vocab_parallel.VocabParallelSampler
     if name in _LOSSES:
         from . import losses
-        return getattr(losses, name)
+        globals()[name] = getattr(losses, name)     # found without this function from now on
+        return globals()[name]
     raise AttributeError(name)

@@ -80,17 +80,19 @@ def _rows(logits: torch.Tensor, targets: torch.Tensor, temperature: Temperature)
 def _check(name: str, t: torch.Tensor, n: int, device: torch.device) -> None:
     if t.device != device:
         raise ValueError(f"{name} must be on the logits' device")
-    if t.dim() != 1 or t.shape[0] != n:
+    if t.shape != (n,):
         raise ValueError(f"{name} must have one value per row")
 
 
 def _vector(name: str, t: Optional[torch.Tensor], n: int, device: torch.device) -> Optional[torch.Tensor]:
     if t is None:
         return None
-    if not t.is_floating_point():
-        raise TypeError(f"{name} must be floating point")
+    if t.dtype != torch.float32:
+        if not t.is_floating_point():
+            raise TypeError(f"{name} must be floating point")
+        t = t.detach().float()
     _check(name, t, n, device)
-    return t.detach().to(torch.float32).contiguous()
+    return t.contiguous()
 
 
 def _ptr(t: Optional[torch.Tensor]):
@@ -103,14 +105,17 @@ def _stride(t: torch.Tensor) -> int:
 
 
 def _call(name: str, device: torch.device, *args) -> None:
+    """One C call on the current stream of `device`, which is current meanwhile."""
     if device.type != "cuda":
         raise ValueError("the logits must be on a CUDA device (there is no CPU fallback)")
     fn = getattr(_lib.load(), name)
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        # the stream's handle alone: torch.cuda.current_stream makes an object of it, 4 us
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc != _lib.NS_OK:
         raise RuntimeError(f"{name} failed: {_lib.status_string(rc)}")
 
@@ -122,6 +127,11 @@ def _head(logits, targets, temperature, temperature_all):
 
 def _new(logits: torch.Tensor, *shape: int) -> torch.Tensor:
     return torch.empty(shape, dtype=torch.float32, device=logits.device)
+
+
+def _parts(logits: torch.Tensor, *sizes: int):
+    """fp32 vectors of these sizes from one allocation."""
+    return torch.empty(sum(sizes), dtype=torch.float32, device=logits.device).split(sizes)
 
 
 def _grad_out(logits: torch.Tensor, given: torch.Tensor, out: Optional[torch.Tensor]) -> torch.Tensor:
@@ -165,7 +175,19 @@ def _logprobs_forward(logits, targets, temperature, temperature_all, entropy, st
     return logprobs, ent, st
 
 
-class _TokenLogprobs(torch.autograd.Function):
+class _Once(torch.autograd.Function):
+    """A function whose ``gradient`` is not differentiable again.  Its wrapper,
+    which says so, costs 10 us and is needed only when a graph of the backward
+    pass is asked for."""
+
+    @classmethod
+    def backward(cls, ctx, *grads):
+        if torch.is_grad_enabled():
+            return once_differentiable(cls.gradient)(ctx, *grads)
+        return cls.gradient(ctx, *grads)
+
+
+class _TokenLogprobs(_Once):
     @staticmethod
     def forward(ctx, logits, targets, temperature, temperature_all, entropy):
         ctx.set_materialize_grads(False)
@@ -175,8 +197,7 @@ class _TokenLogprobs(torch.autograd.Function):
         return (logprobs, ent) if entropy else logprobs
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, a, h=None):
+    def gradient(ctx, a, h=None):
         logits, targets, temperature, stats, ent = ctx.saved_tensors
         a = None if a is None else a.contiguous()
         h = None if h is None else h.contiguous()
@@ -222,17 +243,18 @@ def _policy(logits, targets, old_logprobs, advantages, ref_logprobs, weights, te
 def _policy_forward(logits, targets, temperature, t_all, vectors, coefs, grad):
     """(PolicyLoss, stats, row_grad [2, rows]); writes dloss/dlogits to ``grad`` when there is one."""
     n = logits.shape[0]
-    loss, row_loss, logprobs = _new(logits), _new(logits, n), _new(logits, n)
-    entropy = _new(logits, n) if coefs[3] != 0.0 else None
-    kl = _new(logits, n) if vectors[1] is not None else None
-    stats, row_grad = _new(logits, n, 2), _new(logits, 2, n)
+    has_entropy, has_kl = coefs[3] != 0.0, vectors[1] is not None
+    loss, row_loss, logprobs, stats, row_grad, *rest = _parts(logits, 1, n, n, 2 * n, 2 * n, *[n] * (has_entropy + has_kl))
+    loss, row_grad = loss.view(()), row_grad.view(2, n)
+    entropy = rest[0] if has_entropy else None
+    kl = rest[-1] if has_kl else None
     _call("ns_policy_loss", logits.device, *_head(logits, targets, temperature, t_all), *(_ptr(v) for v in vectors),
           *coefs, loss.data_ptr(), row_loss.data_ptr(), logprobs.data_ptr(), _ptr(entropy), _ptr(kl),
           stats.data_ptr(), row_grad.data_ptr(), _ptr(grad), 0 if grad is None else _stride(grad))
     return PolicyLoss(loss, row_loss, logprobs, entropy, kl), stats, row_grad
 
 
-class _PolicyLoss(torch.autograd.Function):
+class _PolicyLoss(_Once):
     @staticmethod
     def forward(ctx, logits, targets, temperature, t_all, vectors, coefs):
         got, stats, row_grad = _policy_forward(logits, targets, temperature, t_all, vectors, coefs, None)
@@ -242,8 +264,7 @@ class _PolicyLoss(torch.autograd.Function):
         return tuple(got)
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, g, *_):
+    def gradient(ctx, g, *_):
         logits, targets, temperature, stats, entropy, row_grad = ctx.saved_tensors
         row_grad = row_grad * g
         out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
@@ -305,15 +326,15 @@ def _preference(logits, targets, seq_offsets, ref_logprobs, beta, label_smoothin
 
 def _preference_forward(logits, targets, temperature, t_all, offsets, ref, coefs, grad):
     n, pairs = logits.shape[0], offsets.shape[0] // 2
-    loss, pair_loss, rewards = _new(logits), _new(logits, pairs), _new(logits, pairs, 2)
-    logprobs, stats, row_grad = _new(logits, n), _new(logits, n, 2), _new(logits, n)
+    loss, pair_loss, rewards, logprobs, stats, row_grad = _parts(logits, 1, pairs, 2 * pairs, n, 2 * n, n)
+    loss, rewards = loss.view(()), rewards.view(pairs, 2)
     _call("ns_preference_loss", logits.device, *_head(logits, targets, temperature, t_all), offsets.data_ptr(), pairs,
           _ptr(ref), *coefs, loss.data_ptr(), pair_loss.data_ptr(), rewards.data_ptr(), logprobs.data_ptr(),
           stats.data_ptr(), row_grad.data_ptr(), _ptr(grad), 0 if grad is None else _stride(grad))
     return PreferenceLoss(loss, pair_loss, rewards, logprobs), stats, row_grad
 
 
-class _PreferenceLoss(torch.autograd.Function):
+class _PreferenceLoss(_Once):
     @staticmethod
     def forward(ctx, logits, targets, temperature, t_all, offsets, ref, coefs):
         got, stats, row_grad = _preference_forward(logits, targets, temperature, t_all, offsets, ref, coefs, None)
@@ -323,8 +344,7 @@ class _PreferenceLoss(torch.autograd.Function):
         return tuple(got)
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, g, *_):
+    def gradient(ctx, g, *_):
         logits, targets, temperature, stats, row_grad = ctx.saved_tensors
         out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         _gradient(logits, targets, temperature, ctx.t_all, stats, None, row_grad * g, None, out)
