@@ -244,8 +244,9 @@ def _policy_forward(logits, targets, temperature, t_all, vectors, coefs, grad):
     """(PolicyLoss, stats, row_grad [2, rows]); writes dloss/dlogits to ``grad`` when there is one."""
     n = logits.shape[0]
     has_entropy, has_kl = coefs[3] != 0.0, vectors[1] is not None
-    loss, row_loss, logprobs, stats, row_grad, *rest = _parts(logits, 1, n, n, 2 * n, 2 * n, *[n] * (has_entropy + has_kl))
-    loss, row_grad = loss.view(()), row_grad.view(2, n)
+    loss = _new(logits)              # by itself: a part of several may not be changed in place
+    row_loss, logprobs, stats, row_grad, *rest = _parts(logits, n, n, 2 * n, 2 * n, *[n] * (has_entropy + has_kl))
+    row_grad = row_grad.view(2, n)
     entropy = rest[0] if has_entropy else None
     kl = rest[-1] if has_kl else None
     _call("ns_policy_loss", logits.device, *_head(logits, targets, temperature, t_all), *(_ptr(v) for v in vectors),
@@ -326,8 +327,9 @@ def _preference(logits, targets, seq_offsets, ref_logprobs, beta, label_smoothin
 
 def _preference_forward(logits, targets, temperature, t_all, offsets, ref, coefs, grad):
     n, pairs = logits.shape[0], offsets.shape[0] // 2
-    loss, pair_loss, rewards, logprobs, stats, row_grad = _parts(logits, 1, pairs, 2 * pairs, n, 2 * n, n)
-    loss, rewards = loss.view(()), rewards.view(pairs, 2)
+    loss = _new(logits)
+    pair_loss, rewards, logprobs, stats, row_grad = _parts(logits, pairs, 2 * pairs, n, 2 * n, n)
+    rewards = rewards.view(pairs, 2)
     _call("ns_preference_loss", logits.device, *_head(logits, targets, temperature, t_all), offsets.data_ptr(), pairs,
           _ptr(ref), *coefs, loss.data_ptr(), pair_loss.data_ptr(), rewards.data_ptr(), logprobs.data_ptr(),
           stats.data_ptr(), row_grad.data_ptr(), _ptr(grad), 0 if grad is None else _stride(grad))

@@ -141,6 +141,37 @@ __device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
   return d;
 }
 
+// t = (x - c) s for pairs of logits.  fp32: difference, then product.  16-bit
+// logits: one multiply-add x s - fl(c s); the rounding of c s moves every t of
+// the row alike and is taken into account exactly, and while |c s| is below
+// kNearOffset the gradient's offset c s + log2 S rounds to 2^-15 of a value,
+// far below 16 bits' own step.  Rows beyond that go the way of `sums_far`.
+constexpr float kNearOffset = 1024.0f;
+template <int DT>
+struct ScaledPairs {
+  F2 a, b;
+  static __device__ __forceinline__ ScaledPairs of(float c, float scale) {
+    if constexpr (DT == NS_DTYPE_F32) return {f2(-c, -c), f2(scale, scale)};
+    const float off = -__fmul_rn(c, scale);
+    return {f2(scale, scale), f2(off, off)};
+  }
+  __device__ __forceinline__ F2 operator()(F2 x) const {
+    if constexpr (DT == NS_DTYPE_F32) return mul2(add2(x, a), b);
+    return fma2(x, a, b);
+  }
+};
+// The same for one value.
+template <int DT>
+__device__ __forceinline__ float scaled_one(float x, float c, float scale) {
+  return DT == NS_DTYPE_F32 ? (x - c) * scale : fmaf(x, scale, -__fmul_rn(c, scale));
+}
+// The offset c of a row's sums: the target's logit, 0 where that will not do.
+template <int DT>
+__device__ __forceinline__ float row_offset(float x_target, float scale) {
+  const bool ok = DT == NS_DTYPE_F32 ? isfinite(x_target) : fabsf(x_target * scale) < kNearOffset;
+  return ok ? x_target : 0.0f;
+}
+
 struct LossArgs {
   const void* logits;
   int64_t rows, vocab, row_stride;
@@ -176,6 +207,7 @@ __device__ __forceinline__ void row_scale(const LossArgs& a, int64_t row, float&
 }
 
 // Running (m, S, U) of a part of a row.  m = -inf: nothing but -inf so far.
+// Sums around the target's logit have it, or 0, as m.
 struct Part {
   float m, s, u;
 };
@@ -276,15 +308,14 @@ __device__ __noinline__ Part running_part(const void* base, int64_t vocab, float
 // Adds a vector's 2^t, and 2^t t, to the sums.  t is held above -200, where
 // 2^t is 0, so that 0 * -inf does not arise; a NaN t has made 2^t NaN.
 template <int DT, bool ENT>
-__device__ __forceinline__ void add_vector(const uint4& q, F2 minus_c, F2 scale, F2& s, F2& u) {
+__device__ __forceinline__ void add_vector(const uint4& q, const ScaledPairs<DT>& scaled, F2& s, F2& u) {
   using D = Elem<DT>;
   float x[D::E];
   D::unpack(q, x);
 #pragma unroll
   for (int i = 0; i < D::E; i += 2) {
     float a, b;
-    const F2 t = mul2(add2(f2(x[i], x[i + 1]), minus_c), scale);
-    split(t, a, b);
+    split(scaled(f2(x[i], x[i + 1])), a, b);
     const F2 e = f2(ex2_approx(a), ex2_approx(b));
     s = add2(s, e);
     if (ENT) u = fma2(e, f2(fmaxf(a, -200.0f), fmaxf(b, -200.0f)), u);
@@ -329,7 +360,7 @@ __device__ __forceinline__ Part part_sums(const void* base, int64_t vocab, float
   const int64_t tail = sp.head + sp.nv * E + threadIdx.x;
   const float edge[2] = {rank == 0 && threadIdx.x < sp.head ? D::load(row + threadIdx.x) : -INFINITY,
                          rank == parts - 1 && tail < vocab ? D::load(row + tail) : -INFINITY};
-  const F2 minus_c = f2(-c, -c), scale2 = f2(scale, scale);
+  const auto scaled = ScaledPairs<DT>::of(c, scale);
   F2 s[2] = {0, 0}, u[2] = {0, 0};
   for (int v = threadIdx.x; v < n; v += kBatch * kThreads) {
     uint4 next[kBatch];
@@ -340,7 +371,7 @@ __device__ __forceinline__ Part part_sums(const void* base, int64_t vocab, float
     }
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
-      add_vector<DT, ENT>(q[k], minus_c, scale2, s[k & 1], u[k & 1]);
+      add_vector<DT, ENT>(q[k], scaled, s[k & 1], u[k & 1]);
       q[k] = next[k];
     }
   }
@@ -355,7 +386,7 @@ __device__ __forceinline__ Part part_sums(const void* base, int64_t vocab, float
   }
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    const float t = (edge[k] - c) * scale, e = ex2_approx(t);
+    const float t = scaled_one<DT>(edge[k], c, scale), e = ex2_approx(t);
     p.s += e;
     if (ENT) p.u = fmaf(e, fmaxf(t, -200.0f), p.u);
   }
@@ -374,7 +405,7 @@ __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.w
 // The row's sums around c over the whole cluster, the same in every thread of it.
 template <int DT, bool ENT>
 __device__ __forceinline__ Part row_sums(const void* base, int64_t vocab, float c, float scale, RowShared& sh,
-                                         cg::cluster_group& cluster) {
+                                         cg::cluster_group& cluster, bool& near) {
   const int blocks = int(cluster.num_blocks()), rank = int(cluster.block_rank()), lane = threadIdx.x & 31;
   if (blocks > 1) cluster_arrive();
   Part p = part_sums<DT, ENT>(base, vocab, c, scale, rank, blocks, sh.warp);
@@ -385,7 +416,8 @@ __device__ __forceinline__ Part row_sums(const void* base, int64_t vocab, float 
     p.s = warp_sum(lane < blocks ? sh.block[lane].s : 0.0f);
     if (ENT) p.u = warp_sum(lane < blocks ? sh.block[lane].u : 0.0f);
   }
-  if (!sums_far(p.s)) return p;      // the same for the whole cluster
+  near = !sums_far(p.s);             // the same for the whole cluster
+  if (near) return p;
   p = running_part<DT, ENT>(base, vocab, scale, rank, blocks, sh.warp);
   if (blocks > 1) {
     cluster.sync();                    // every block has read the first sums
@@ -399,26 +431,28 @@ __device__ __forceinline__ Part row_sums(const void* base, int64_t vocab, float 
 
 // What a row's sums and target give, in 64 bits, so that differences from a
 // reference's log-probability keep their digits.  The target's t uses the same
-// rounded scale as the sums.  The logarithm is split as exponent * ln2 +
-// ln(mantissa), whose second part lies in [0, ln2) and is exact to 2^-25.
+// rounded scale, and `near` the same rounded offset, as the sums.  The
+// logarithm is split as exponent * ln2 + ln(mantissa), whose second part lies
+// in [0, ln2) and is exact to 2^-25.
 struct RowResult {
   double logprob;
-  float entropy, log2s;
+  float entropy, log2s;      // log2 S around m s, not rounded
 };
-template <bool ENT>
-__device__ __forceinline__ RowResult finish(const Part& p, float x_target, float scale) {
+template <int DT, bool ENT>
+__device__ __forceinline__ RowResult finish(const Part& p, float x_target, float scale, bool near) {
   int ex;
   const float mant = 2.0f * frexpf(p.s, &ex);
   const double ln_s = p.s < INFINITY && p.s > 0.0f ? double(ex - 1) * kLn2 + double(logf(mant)) : double(NAN);
+  // how far the sums' offset lies from m s
+  const double moved = DT != NS_DTYPE_F32 && near ? double(__fmul_rn(p.m, scale)) - double(p.m) * double(scale) : 0.0;
   RowResult r;
-  r.logprob = (double(x_target) - double(p.m)) * double(scale) * kLn2 - ln_s;
-  r.log2s = float(ln_s * (1.0 / kLn2));
+  r.logprob = ((double(x_target) - double(p.m)) * double(scale) - moved) * kLn2 - ln_s;
+  if (r.logprob > 0.0) r.logprob = 0.0;          // a rounding of S
+  r.log2s = float(ln_s * (1.0 / kLn2) + moved);
   r.entropy = ENT ? float(ln_s) - float(kLn2) * (p.u / p.s) : 0.0f;
   if (isnan(r.logprob)) r.log2s = r.entropy = NAN;
   return r;
 }
-
-__device__ __forceinline__ float row_offset(float x_target) { return isfinite(x_target) ? x_target : 0.0f; }
 
 struct PolicyIn {
   float old, adv, ref, w;
@@ -479,46 +513,58 @@ __device__ __forceinline__ bool row_alive(const LossArgs& a, int64_t row, float&
 struct alignas(16) GradRow {
   float c, log2s, scale, ca, cb;
   float at;                  // the value at the target
-  int zero;
+  short zero, wide;          // wide: |c s| is too large for one multiply-add
   int target;                // past the vocabulary: none
 };
-template <bool ENT>
+template <int DT, bool ENT>
 __device__ __forceinline__ float grad_value(const GradRow& g, float x) {
-  const float t = fmaf(x - g.c, g.scale, -g.log2s);
+  const float t = DT == NS_DTYPE_F32 || g.wide ? fmaf(x - g.c, g.scale, -g.log2s)
+                                               : fmaf(x, g.scale, -fmaf(g.c, g.scale, g.log2s));
   return ex2_approx(t) * (ENT ? fmaf(g.cb, fmaxf(t, -200.0f), g.ca) : g.ca);
 }
 // a and h: dloss/dlogprob and dloss/dentropy of the row
-template <bool ENT>
+template <int DT, bool ENT>
 __device__ __forceinline__ GradRow grad_row(float c, float log2s, float scale, double inv_t, float a, float h,
                                             float entropy, int64_t target, float x_target) {
   GradRow g;
   g.c = c == -INFINITY ? 0.0f : c;      // no distribution: log2 S is NaN
   g.log2s = log2s;
   g.scale = scale;
+  g.wide = !(fabsf(g.c * scale) < kNearOffset);
   g.ca = -float((double(a) + (ENT ? double(h) * double(entropy) : 0.0)) * inv_t);
   g.cb = ENT ? -float(double(h) * kLn2 * inv_t) : 0.0f;
-  g.at = grad_value<ENT>(g, x_target) + float(double(a) * inv_t);
+  g.at = grad_value<DT, ENT>(g, x_target) + float(double(a) * inv_t);
   g.zero = a == 0.0f && h == 0.0f;
   g.target = int(target < (int64_t(1) << 24) ? target : int64_t(1) << 24);
   return g;
 }
-// The same for a vector; the constants of the row are in pairs.
+// The same for a vector; the constants of the row are in pairs.  16-bit rows
+// that are not wide take one multiply-add to log2 p.
+template <int DT>
 struct GradPairs {
-  F2 minus_c, scale, minus_l, ca, cb;
+  F2 a, b, l, ca, cb;
+  __device__ __forceinline__ explicit GradPairs(const GradRow& g) : ca(f2(g.ca, g.ca)), cb(f2(g.cb, g.cb)) {
+    if constexpr (DT == NS_DTYPE_F32) {
+      a = f2(-g.c, -g.c), b = f2(g.scale, g.scale), l = f2(-g.log2s, -g.log2s);
+    } else {
+      const float off = -fmaf(g.c, g.scale, g.log2s);
+      a = f2(g.scale, g.scale), b = f2(off, off), l = 0;
+    }
+  }
+  __device__ __forceinline__ F2 operator()(F2 x) const {
+    if constexpr (DT == NS_DTYPE_F32) return fma2(add2(x, a), b, l);
+    return fma2(x, a, b);
+  }
 };
-__device__ __forceinline__ GradPairs grad_pairs(const GradRow& g) {
-  return {f2(-g.c, -g.c), f2(g.scale, g.scale), f2(-g.log2s, -g.log2s), f2(g.ca, g.ca), f2(g.cb, g.cb)};
-}
 template <int DT, bool ENT>
-__device__ __forceinline__ uint4 grad_vector(const GradPairs& g, const uint4& q) {
+__device__ __forceinline__ uint4 grad_vector(const GradPairs<DT>& g, const uint4& q) {
   using D = Elem<DT>;
   float x[D::E];
   D::unpack(q, x);
 #pragma unroll
   for (int i = 0; i < D::E; i += 2) {
     float a, b;
-    const F2 t = fma2(add2(f2(x[i], x[i + 1]), g.minus_c), g.scale, g.minus_l);
-    split(t, a, b);
+    split(g(f2(x[i], x[i + 1])), a, b);
     const F2 p = f2(ex2_approx(a), ex2_approx(b));
     const F2 w = ENT ? fma2(g.cb, f2(fmaxf(a, -200.0f), fmaxf(b, -200.0f)), g.ca) : g.ca;
     split(mul2(p, w), x[i], x[i + 1]);
@@ -527,10 +573,11 @@ __device__ __forceinline__ uint4 grad_vector(const GradPairs& g, const uint4& q)
 }
 template <int DT, bool ENT>
 __device__ __forceinline__ void grad_element(const GradRow& g, float x, typename Elem<DT>::T* out, int64_t j) {
-  Elem<DT>::store(out + j, j == g.target ? g.at : grad_value<ENT>(g, x));
+  Elem<DT>::store(out + j, j == g.target ? g.at : grad_value<DT, ENT>(g, x));
 }
 
-// Block `rank`'s share of a row's gradient where the rows start on different 16-byte phases: element by element.
+// Block `rank`'s share of a row's gradient element by element: the rows start on
+// different 16-byte phases, or the row is wide.
 template <int DT, bool ENT>
 __device__ __forceinline__ void write_elements(const GradRow& g, const void* base, void* grad, int64_t vocab, int rank,
                                                int blocks) {
@@ -590,9 +637,10 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const LossArgs a) {
   const T* x = static_cast<const T*>(a.logits) + row * a.row_stride;
   const int64_t target = a.targets[row];
   const float x_target = target < a.vocab ? D::load(x + target) : NAN;
-  const Part p = row_sums<DT, ENT>(x, a.vocab, row_offset(x_target), scale, sh, cluster);
+  bool near;
+  const Part p = row_sums<DT, ENT>(x, a.vocab, row_offset<DT>(x_target, scale), scale, sh, cluster, near);
   if (threadIdx.x != 0 || rank != 0) return;
-  const RowResult r = finish<ENT>(p, x_target, scale);
+  const RowResult r = finish<DT, ENT>(p, x_target, scale, near);
   a.logprobs[row] = float(r.logprob);
   if (ENT) a.entropy[row] = r.entropy;
   if (a.stats) {
@@ -695,7 +743,8 @@ __device__ __forceinline__ void write_chunk(const GradRow& g, const void* base, 
     write_zeros<DT>(out, vocab, chunk, chunks);
     return;
   }
-  if (((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(out)) & 15) != 0) {
+  const bool same = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+  if (!same || (DT != NS_DTYPE_F32 && g.wide)) {
     write_elements<DT, ENT>(g, x, out, vocab, chunk, chunks);
     return;
   }
@@ -704,7 +753,7 @@ __device__ __forceinline__ void write_chunk(const GradRow& g, const void* base, 
   const int j0 = int(sp.head) + v0 * E;
   const uint4* src = reinterpret_cast<const uint4*>(x + j0) + threadIdx.x;
   uint4* dst = reinterpret_cast<uint4*>(out + j0) + threadIdx.x;
-  const GradPairs pairs = grad_pairs(g);
+  const GradPairs<DT> pairs(g);
   uint4 q[kGradVecs];
 #pragma unroll
   for (int k = 0; k < kGradVecs; ++k)
@@ -740,7 +789,7 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(const LossArgs a, int ch
     double inv_t;
     row_scale(a, row, scale, inv_t);
     // every thread reads the target's logit before it writes; in place, the one that uses it is its writer
-    g = grad_row<ENT>(a.stats[2 * row], a.stats[2 * row + 1], scale, inv_t, ga, gh, ENT ? a.entropy[row] : 0.0f, target,
+    g = grad_row<DT, ENT>(a.stats[2 * row], a.stats[2 * row + 1], scale, inv_t, ga, gh, ENT ? a.entropy[row] : 0.0f, target,
                       target < a.vocab ? D::load(x + target) : NAN);
   }
   write_chunk<DT, ENT>(g, x, out, a.vocab, chunk, chunks);
@@ -767,15 +816,15 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(const LossArgs a, int ch
 constexpr int kRowWarps = 15;
 constexpr int kRowThreads = kRowWarps * 32;
 constexpr int kHeldThreads = kRowThreads + 32;      // and the producer warp
-constexpr int kLaneVecs = 2;                        // of a chunk
-constexpr int kChunkVecs = kRowThreads * kLaneVecs;
-constexpr int kChunkBytes = kChunkVecs * 16;
 
 // Two shapes: one block of an SM with registers, or two with smaller rings.
 template <bool LARGE>
 struct HeldShape {
-  static constexpr int kHold = LARGE ? 8 : 0;       // chunks in registers
-  static constexpr int kSlots = LARGE ? 14 : 7;
+  static constexpr int kLaneVecs = LARGE ? 4 : 2;   // of a chunk
+  static constexpr int kChunkVecs = kRowThreads * kLaneVecs;
+  static constexpr int kChunkBytes = kChunkVecs * 16;
+  static constexpr int kHold = LARGE ? 4 : 0;       // chunks in registers
+  static constexpr int kSlots = 7;
   static constexpr int kBlocks = LARGE ? 1 : 2;
   static constexpr int kMostVecs = (kHold + kSlots - 1) * kChunkVecs;
   static constexpr uint32_t kSmem = uint32_t(kSlots) * kChunkBytes;
@@ -861,7 +910,7 @@ __global__ void __launch_bounds__(kHeldThreads, HeldShape<LARGE>::kBlocks)
   using D = Elem<DT>;
   using T = typename D::T;
   using H = HeldShape<LARGE>;
-  constexpr int E = D::E, kHold = H::kHold, kSlots = H::kSlots;
+  constexpr int E = D::E, kHold = H::kHold, kSlots = H::kSlots, kLaneVecs = H::kLaneVecs, kChunkVecs = H::kChunkVecs;
   __shared__ HeldShared sh;
   extern __shared__ __align__(128) uint4 ring[];
   cg::cluster_group cluster = cg::this_cluster();
@@ -970,8 +1019,8 @@ __global__ void __launch_bounds__(kHeldThreads, HeldShape<LARGE>::kBlocks)
         edge_at = rank == 0 && tid < s.head ? tid : rank == blocks - 1 && tid >= 16 && tail < int(a.vocab) ? tail : -1;
       }
       const float edge = edge_at >= 0 ? D::load(x + edge_at) : -INFINITY;
-      const float c = row_offset(sh.info[first_slot].x_target), scale = sh.info[first_slot].scale;
-      const F2 minus_c = f2(-c, -c), scale2 = f2(scale, scale);
+      const float scale = sh.info[first_slot].scale, c = row_offset<DT>(sh.info[first_slot].x_target, scale);
+      const auto scaled = ScaledPairs<DT>::of(c, scale);
       RowInfo info;
       if (warp == 0) info = sh.info[first_slot];
       const auto take = [&](int at, uint4 (&q)[kLaneVecs]) {      // the chunk at vector `at` of the share
@@ -981,13 +1030,13 @@ __global__ void __launch_bounds__(kHeldThreads, HeldShape<LARGE>::kBlocks)
 #pragma unroll
           for (int i = 0; i < kLaneVecs; ++i) q[i] = src[i * kRowThreads];
 #pragma unroll
-          for (int i = 0; i < kLaneVecs; ++i) add_vector<DT, ENT>(q[i], minus_c, scale2, sum[i & 1], u[i & 1]);
+          for (int i = 0; i < kLaneVecs; ++i) add_vector<DT, ENT>(q[i], scaled, sum[i & 1], u[i & 1]);
         } else {
 #pragma unroll
           for (int i = 0; i < kLaneVecs; ++i)
             if (at + i * kRowThreads + tid < s.n) {
               q[i] = src[i * kRowThreads];
-              add_vector<DT, ENT>(q[i], minus_c, scale2, sum[i & 1], u[i & 1]);
+              add_vector<DT, ENT>(q[i], scaled, sum[i & 1], u[i & 1]);
             }
         }
       };
@@ -1015,7 +1064,7 @@ __global__ void __launch_bounds__(kHeldThreads, HeldShape<LARGE>::kBlocks)
         advance();
       }
       {
-        const float t = (edge - c) * scale, e = ex2_approx(t);
+        const float t = scaled_one<DT>(edge, c, scale), e = ex2_approx(t);
         float lo, hi;
         split(add2(sum[0], sum[1]), lo, hi);
         const float total = warp_sum(lo + hi + e);
@@ -1046,7 +1095,8 @@ __global__ void __launch_bounds__(kHeldThreads, HeldShape<LARGE>::kBlocks)
           if (ENT) p.u = warp_sum(v.y);
         }
         if (bad) p.s = NAN;             // a wait ran out: the row has no result
-        if (sums_far(p.s)) {
+        const bool near = !sums_far(p.s);
+        if (!near) {
           // one warp of a block: a row whose target is all but impossible is rare
           Part q = {-INFINITY, 0.0f, 0.0f};
           const uint4* vec = reinterpret_cast<const uint4*>(x + s.head) + s.v0;
@@ -1077,9 +1127,9 @@ __global__ void __launch_bounds__(kHeldThreads, HeldShape<LARGE>::kBlocks)
           }
         }
         if (lane == 0) {
-          const RowResult r = finish<ENT>(p, info.x_target, info.scale);
+          const RowResult r = finish<DT, ENT>(p, info.x_target, info.scale, near);
           const PolicyRow l = policy_row(a, info.in, r.logprob, r.entropy);
-          sh.coef = grad_row<ENT>(p.m, r.log2s, info.scale, info.inv_t, l.a, l.h, r.entropy, info.target, info.x_target);
+          sh.coef = grad_row<DT, ENT>(p.m, r.log2s, info.scale, info.inv_t, l.a, l.h, r.entropy, info.target, info.x_target);
           if (rank == 0) {
             a.logprobs[row] = float(r.logprob);
             if (ENT) a.entropy[row] = r.entropy;
@@ -1117,14 +1167,15 @@ __global__ void __launch_bounds__(kHeldThreads, HeldShape<LARGE>::kBlocks)
             if (const int v = j * kChunkVecs + i * kRowThreads + tid; v < s.n) put(held[j][i], v);
       };
       uint4* dst = reinterpret_cast<uint4*>(mine);
-      const GradPairs pairs = grad_pairs(g);
-      if (((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(out)) & 15) != 0) {
-        // the rows start on different 16-byte phases: element by element
+      const GradPairs<DT> pairs(g);
+      const bool same = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+      if (!same || (DT != NS_DTYPE_F32 && g.wide)) {
+        // the rows start on different 16-byte phases, or the row is wide: element by element
         write([&](const uint4& q, int v) {
-          const uint4 r = g.zero ? make_uint4(0, 0, 0, 0) : grad_vector<DT, ENT>(pairs, q);
-          const T* e = reinterpret_cast<const T*>(&r);
+          float f[E];
+          D::unpack(q, f);
 #pragma unroll
-          for (int i = 0; i < E; ++i) mine[v * E + i] = e[i];
+          for (int i = 0; i < E; ++i) D::store(mine + v * E + i, g.zero ? 0.0f : grad_value<DT, ENT>(g, f[i]));
         });
       } else if (g.zero) {
         write([&](const uint4&, int v) { dst[v] = make_uint4(0, 0, 0, 0); });
