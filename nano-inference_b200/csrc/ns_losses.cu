@@ -40,7 +40,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
-constexpr int kBatch = 4;          // 16-byte loads a thread has in flight
+constexpr int kBatch = 2;          // 16-byte loads a thread has in flight
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr double kLn2 = 0.6931471805599453;
 
@@ -578,26 +578,26 @@ __device__ __forceinline__ void grad_element(const GradRow& g, float x, typename
 
 // Block `rank`'s share of a row's gradient element by element: the rows start on
 // different 16-byte phases, or the row is wide.
-template <int DT, bool ENT>
+template <int DT, bool ENT, int THREADS>
 __device__ __forceinline__ void write_elements(const GradRow& g, const void* base, void* grad, int64_t vocab, int rank,
                                                int blocks) {
   using T = typename Elem<DT>::T;
   const T* row = static_cast<const T*>(base);
   const int64_t end = vocab * (rank + 1) / blocks;
-  for (int64_t j = vocab * rank / blocks + threadIdx.x; j < end; j += kThreads)
+  for (int64_t j = vocab * rank / blocks + threadIdx.x; j < end; j += THREADS)
     grad_element<DT, ENT>(g, Elem<DT>::load(row + j), static_cast<T*>(grad), j);
 }
 
 // Zeros in block `rank`'s share of a row.
-template <int DT>
-__device__ __forceinline__ void write_zeros(void* grad, int64_t vocab, int rank, int blocks, int threads = kThreads) {
+template <int DT, int THREADS>
+__device__ __forceinline__ void write_zeros(void* grad, int64_t vocab, int rank, int blocks) {
   using T = typename Elem<DT>::T;
   constexpr int E = Elem<DT>::E;
   T* out = static_cast<T*>(grad);
   const Span sp = row_span<E>(out, vocab);
   uint4* dst = reinterpret_cast<uint4*>(out + sp.head);
   const int v1 = int(sp.nv * (rank + 1) / blocks);
-  for (int v = int(sp.nv * rank / blocks) + threadIdx.x; v < v1; v += threads) dst[v] = make_uint4(0, 0, 0, 0);
+  for (int v = int(sp.nv * rank / blocks) + threadIdx.x; v < v1; v += THREADS) dst[v] = make_uint4(0, 0, 0, 0);
   const int64_t tail = sp.head + sp.nv * E + threadIdx.x;
   if (rank == 0 && threadIdx.x < sp.head) Elem<DT>::store(out + threadIdx.x, 0.0f);
   if (rank == blocks - 1 && tail < vocab) Elem<DT>::store(out + tail, 0.0f);
@@ -676,58 +676,77 @@ __global__ void __launch_bounds__(1024) policy_sum_kernel(const LossArgs a, floa
   if (threadIdx.x == 0) *loss = float(v);
 }
 
-// The pairs: one warp sums a sequence's gains, then the pair's loss, and the
-// rows' coefficients over the gains.
+// The pairs: warps sum the sequences' gains (several a sequence while they are
+// few), one thread a pair turns two sums into the pair's loss, and the warps
+// write the rows' coefficients over the gains.
 __global__ void __launch_bounds__(1024) pair_kernel(const LossArgs a, float beta, float smoothing, int average,
                                                     float* loss, float* pair_loss, float* rewards) {
-  __shared__ double shared[32];
+  __shared__ double sums[32], shared[32];
+  __shared__ int counts[32];
+  __shared__ float coef[32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int each = 1;                           // warps of a sequence
+  while (each < 16 && 2 * a.pairs * each * 2 <= 32) each *= 2;
+  const int at_once = 32 / each, step = 32 * each;
   double total = 0.0;
-  for (int64_t p = warp; p < a.pairs; p += 32) {
-    int64_t lo[2], hi[2];
-    double reward[2], share[2];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      lo[k] = max(a.seq_offsets[2 * p + k], int64_t(0));
-      hi[k] = min(a.seq_offsets[2 * p + k + 1], a.rows);
-      double sum = 0.0;
-      int64_t count = 0;
-      for (int64_t i = lo[k] + lane; i < hi[k]; i += 32) {
-        sum += double(a.row_grad[i]);
-        count += a.targets[i] >= 0;
-      }
-#pragma unroll
-      for (int o = 16; o; o >>= 1) {
-        sum += __shfl_xor_sync(~0u, sum, o);
-        count += __shfl_xor_sync(~0u, count, o);
-      }
-      share[k] = average ? 1.0 / double(max(count, int64_t(1))) : 1.0;
-      reward[k] = double(beta) * sum * share[k];
+  for (int64_t first = 0; first < 2 * a.pairs; first += at_once) {
+    const int64_t seq = first + warp / each;
+    int64_t lo = 0, hi = 0;
+    if (seq < 2 * a.pairs) {
+      lo = max(a.seq_offsets[seq], int64_t(0)) + warp % each * 32 + lane;
+      hi = min(a.seq_offsets[seq + 1], a.rows);
     }
-    const double h = reward[0] - reward[1];
-    // ln sigmoid(h) = min(h, 0) - ln(1 + exp(-|h|)), and the same with -h
-    const float tail = log1pf(expf(-fabsf(float(h))));
-    const double win = fmin(h, 0.0) - double(tail), lose = fmin(-h, 0.0) - double(tail);
-    const double e = double(smoothing);
-    const double l = isnan(h) ? h : -(1.0 - e) * win - e * lose;
-    const double up = 1.0 / (1.0 + double(expf(float(-h)))), down = 1.0 / (1.0 + double(expf(float(h))));
-    const double slope = (e * up - (1.0 - e) * down) * double(beta) / double(a.pairs);
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const float c = float((k ? -slope : slope) * share[k]);
-      for (int64_t i = lo[k] + lane; i < hi[k]; i += 32) a.row_grad[i] = a.targets[i] >= 0 ? c : 0.0f;
+    double sum = 0.0;
+    int count = 0;
+#pragma unroll 4
+    for (int64_t i = lo; i < hi; i += step) {
+      sum += double(a.row_grad[i]);
+      count += a.targets[i] >= 0;
     }
-    if (lane == 0) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      sum += __shfl_xor_sync(~0u, sum, o);
+      count += __shfl_xor_sync(~0u, count, o);
+    }
+    if (lane == 0) sums[warp] = sum, counts[warp] = count;
+    __syncthreads();
+    const int64_t p = first / 2 + threadIdx.x;
+    if (threadIdx.x < at_once / 2 && p < a.pairs) {
+      double reward[2], share[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int w = (2 * int(threadIdx.x) + k) * each;
+        double s = 0.0;
+        int n = 0;
+        for (int i = 0; i < each; ++i) s += sums[w + i], n += counts[w + i];
+        share[k] = average ? 1.0 / double(max(n, 1)) : 1.0;
+        reward[k] = double(beta) * s * share[k];
+      }
+      const double h = reward[0] - reward[1];
+      // ln sigmoid(h) = min(h, 0) - ln(1 + exp(-|h|)), and the same with -h
+      const float tail = log1pf(expf(-fabsf(float(h))));
+      const double win = fmin(h, 0.0) - double(tail), lose = fmin(-h, 0.0) - double(tail);
+      const double e = double(smoothing);
+      // without smoothing an infinite margin must not meet 0 * inf
+      const double l = isnan(h) ? h : -(1.0 - e) * win - (e != 0.0 ? e * lose : 0.0);
+      const double up = 1.0 / (1.0 + double(expf(float(-h)))), down = 1.0 / (1.0 + double(expf(float(h))));
+      const double slope = (e * up - (1.0 - e) * down) * double(beta) / double(a.pairs);
+      coef[2 * threadIdx.x] = float(slope * share[0]);
+      coef[2 * threadIdx.x + 1] = float(-slope * share[1]);
       pair_loss[p] = float(l);
       rewards[2 * p] = float(reward[0]);
       rewards[2 * p + 1] = float(reward[1]);
       total += l;
     }
+    __syncthreads();
+    const float c = coef[warp / each];
+    for (int64_t i = lo; i < hi; i += step) a.row_grad[i] = a.targets[i] >= 0 ? c : 0.0f;
   }
   total = block_sum(total, shared);
   if (threadIdx.x == 0) *loss = a.pairs ? float(total / double(a.pairs)) : 0.0f;
 }
 
+constexpr int kGradThreads = 128;
 constexpr int kGradVecs = 8;    // vectors of a thread
 
 // Chunk `chunk` of `chunks` of a row's gradient.
@@ -740,12 +759,12 @@ __device__ __forceinline__ void write_chunk(const GradRow& g, const void* base, 
   const T* x = static_cast<const T*>(base);
   T* out = static_cast<T*>(grad);
   if (g.zero) {
-    write_zeros<DT>(out, vocab, chunk, chunks);
+    write_zeros<DT, kGradThreads>(out, vocab, chunk, chunks);
     return;
   }
   const bool same = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
   if (!same || (DT != NS_DTYPE_F32 && g.wide)) {
-    write_elements<DT, ENT>(g, x, out, vocab, chunk, chunks);
+    write_elements<DT, ENT, kGradThreads>(g, x, out, vocab, chunk, chunks);
     return;
   }
   const Span sp = row_span<E>(x, vocab);
@@ -757,25 +776,26 @@ __device__ __forceinline__ void write_chunk(const GradRow& g, const void* base, 
   uint4 q[kGradVecs];
 #pragma unroll
   for (int k = 0; k < kGradVecs; ++k)
-    if (int(threadIdx.x) + k * kThreads < n) q[k] = src[k * kThreads];
+    if (int(threadIdx.x) + k * kGradThreads < n) q[k] = src[k * kGradThreads];
 #pragma unroll
   for (int k = 0; k < kGradVecs; ++k)
-    if (int(threadIdx.x) + k * kThreads < n) dst[k * kThreads] = grad_vector<DT, ENT>(pairs, q[k]);
+    if (int(threadIdx.x) + k * kGradThreads < n) dst[k * kGradThreads] = grad_vector<DT, ENT>(pairs, q[k]);
   // the target's value over its vector, by the thread that wrote it
   const unsigned at = unsigned(g.target - j0);
-  if (at < unsigned(n) * E && int(at / E) % kThreads == int(threadIdx.x)) D::store(out + g.target, g.at);
+  if (at < unsigned(n) * E && int(at / E) % kGradThreads == int(threadIdx.x)) D::store(out + g.target, g.at);
   const int64_t tail = sp.head + sp.nv * E + threadIdx.x;
   if (chunk == 0 && threadIdx.x < sp.head)
     grad_element<DT, ENT>(g, D::load(x + threadIdx.x), out, threadIdx.x);
   if (chunk == chunks - 1 && tail < vocab) grad_element<DT, ENT>(g, D::load(x + tail), out, tail);
 }
 
-// The gradient alone: one block per (row, chunk of kThreads x kGradVecs vectors).
+// The gradient alone: one block per (row, chunk of kGradThreads x kGradVecs vectors),
+// from the last row on, whose logits L2 still holds from the sums.
 template <int DT, bool ENT>
-__global__ void __launch_bounds__(kThreads) grad_kernel(const LossArgs a, int chunks) {
+__global__ void __launch_bounds__(kGradThreads) grad_kernel(const LossArgs a, int chunks) {
   using D = Elem<DT>;
   using T = typename D::T;
-  const int64_t row = blockIdx.x / chunks;
+  const int64_t row = a.rows - 1 - blockIdx.x / chunks;
   const int chunk = int(blockIdx.x % chunks);
   const T* x = static_cast<const T*>(a.logits) + row * a.row_stride;
   T* out = static_cast<T*>(a.grad_logits) + row * a.grad_stride;
@@ -800,14 +820,13 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(const LossArgs a, int ch
 // ---------------------------------------------------------------------------
 // A row's gradient needs the row's sums first, so a block keeps the row (or a
 // cluster's block its share of it) on chip between the two.  Persistent
-// clusters; cluster i takes rows i, i + clusters, ...  A producer warp copies
-// rows in chunks into a ring in shared memory.  The row warps add a row up as
-// its chunks land: the first chunks they keep in registers and hand back at
+// clusters, to which the rows are dealt out.  A producer warp copies rows in
+// chunks into a ring in shared memory.  The row warps add a row up as its
+// chunks land: the first chunks they keep in registers and hand back at
 // once, the others stay in the ring.  They join their sums (over the cluster
 // through the peers' shared memory) and write the gradient, the ring's chunks
 // first, handing each back as it is done, so the reads of the next row run
-// under the writes of this one.  The logits cross L2 and DRAM once.  The rows
-// that hold no token come last.
+// under the writes of this one.  The logits cross L2 and DRAM once.
 //
 // What bounds it: 2 exponentials a logit are 70 % of the time that bf16's 4
 // bytes a logit need, and a row's sums cannot end before its last chunk lands.
@@ -832,7 +851,8 @@ struct HeldShape {
 
 // What the producer says of a row, with its first chunk.
 struct RowInfo {
-  int64_t k;              // the cluster's row; -1 ends the rows
+  int64_t row;            // -1 ends the rows
+  int alive;              // 0: it holds no token, and there is no more to say
   int64_t target;
   double inv_t;
   float x_target, scale;
@@ -868,25 +888,51 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
 // The barrier of the row warps.
 __device__ __forceinline__ void row_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(kRowThreads) : "memory"); }
 
-// The rows of a cluster that hold a token, or those that do not, in order.
+// A cluster's rows in order.  The rows that hold a token are dealt out in turn,
+// and so are those that do not, so every cluster has its share of both however
+// the padding lies.  One warp looks through the rows, 32 at a time; the numbers
+// that say which are which come 128 rows at a time and as many ahead.
 struct RowWalk {
-  int64_t rows, window = -1;
-  uint32_t mask = 0;
-  // the first such row from k on, or `rows`
-  __device__ __forceinline__ int64_t next(const LossArgs& a, int64_t first_row, int64_t clusters, int64_t k, bool alive) {
-    const int lane = threadIdx.x & 31;
-    while (k < rows) {
-      if ((k >> 5) != window) {
-        window = k >> 5;
-        const int64_t i = (window << 5) + lane;
-        float w;
-        mask = __ballot_sync(~0u, i < rows && row_alive<kPolicy>(a, first_row + i * clusters, w) == alive);
-      }
-      const uint32_t left = mask >> (k & 31);
-      if (left) return k + __ffs(left) - 1;
-      k = (window + 1) << 5;
+  static constexpr int kAhead = 4;
+  int64_t base = 0;                 // of the 32 rows looked at next
+  unsigned alive = 0, dead = 0;     // those before them, modulo the clusters
+  uint32_t mine = 0, mine_alive = 0;
+  uint32_t held = 0;                // bit i: this lane's row of the block's i-th 32 holds a token
+  bool next_held[kAhead];
+  __device__ __forceinline__ void look(const LossArgs& a, int64_t block) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int64_t row = block + 32 * i + (threadIdx.x & 31), at = min(row, a.rows - 1);
+      const float w = a.weights ? a.weights[at] : 1.0f;
+      next_held[i] = (a.targets[at] >= 0) & (w != 0.0f) & (row < a.rows);
     }
-    return rows;
+  }
+  // The masks of the next 32 rows that are this cluster's.
+  __device__ __forceinline__ void step(const LossArgs& a, unsigned cluster, unsigned clusters) {
+    const int i = int(base >> 5) & (kAhead - 1);
+    if (i == 0) {
+      if (base == 0) look(a, 0);
+      held = 0;
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) held |= uint32_t(next_held[j]) << j;
+      look(a, base + 32 * kAhead);
+    }
+    const bool here = base + (threadIdx.x & 31) < a.rows, hold = (held >> i) & 1;
+    const uint32_t lower = lanemask_lt(), holds = __ballot_sync(~0u, hold), rest = __ballot_sync(~0u, here && !hold);
+    const unsigned turn = hold ? alive + __popc(holds & lower) : dead + __popc(rest & lower);
+    alive += __popc(holds), dead += __popc(rest);
+    bool is_mine;
+    if (clusters >= 32) {           // one round at most goes by in 32 rows
+      is_mine = turn == cluster || turn == cluster + clusters;
+      if (alive >= clusters) alive -= clusters;
+      if (dead >= clusters) dead -= clusters;
+    } else {
+      is_mine = turn % clusters == cluster;
+      alive %= clusters, dead %= clusters;
+    }
+    mine = __ballot_sync(~0u, here && is_mine);
+    mine_alive = holds;
+    base += 32;
   }
 };
 
@@ -917,8 +963,6 @@ __global__ void __launch_bounds__(kHeldThreads, HeldShape<LARGE>::kBlocks)
   const int blocks = int(cluster.num_blocks()), rank = int(cluster.block_rank());
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
   const int shift = 31 - __clz(blocks);           // blocks is a power of two
-  const int64_t first_row = blockIdx.x >> shift, clusters = gridDim.x >> shift;
-  const int64_t rows = (a.rows - first_row + clusters - 1) / clusters;     // of this cluster
   if (tid < kSlots) {
     mbar_init(&sh.full[tid], 1);
     mbar_init(&sh.empty[tid], kRowWarps);
@@ -931,37 +975,38 @@ __global__ void __launch_bounds__(kHeldThreads, HeldShape<LARGE>::kBlocks)
   fence_mbar_init();
   __syncthreads();
   if (blocks > 1) cluster.sync();       // the peers' barriers exist
-  const auto logits_row = [&](int64_t k) { return static_cast<const T*>(a.logits) + (first_row + k * clusters) * a.row_stride; };
-  const auto grad_out = [&](int64_t k) { return static_cast<T*>(a.grad_logits) + (first_row + k * clusters) * a.grad_stride; };
+  const auto logits_row = [&](int64_t row) { return static_cast<const T*>(a.logits) + row * a.row_stride; };
 
   if (warp == kRowWarps) {
     // ------------------------------------------------------------ producer warp
     const uint64_t policy = l2_policy_evict_first();
     RowWalk walk;
-    walk.rows = rows;
     int slot = 0;
     uint32_t phase = 1;                 // the first round finds the slots empty
     bool bad = false;
-    int64_t window = -1;
-    RowInfo mine = {};                  // lane i: row `window` * 32 + i
-    for (int64_t k = 0; k >= 0 && !bad;) {
-      k = walk.next(a, first_row, clusters, k, true);
-      const bool end = k >= rows;
-      Share s = {};
-      const uint4* src = nullptr;
-      if (!end) {
-        if ((k >> 5) != window) {
-          window = k >> 5;
-          mine.k = (window << 5) + lane;
-          if (mine.k < rows) {
-            const int64_t row = first_row + mine.k * clusters;
-            mine.target = a.targets[row];
-            row_scale(a, row, mine.scale, mine.inv_t);
-            mine.in = policy_in(a, row, a.weights ? a.weights[row] : 1.0f / float(a.rows));
-            mine.x_target = mine.target >= 0 && mine.target < a.vocab ? D::load(logits_row(mine.k) + mine.target) : NAN;
+    RowInfo mine = {};                  // lane i: of the i-th of 32 rows
+    for (bool end = false; !end && !bad;) {
+      while (walk.mine == 0 && walk.base < a.rows) {
+        walk.step(a, blockIdx.x >> shift, gridDim.x >> shift);
+        if ((walk.mine >> lane) & 1) {
+          mine.row = walk.base - 32 + lane;
+          mine.alive = (walk.mine_alive >> lane) & 1;
+          if (mine.alive) {
+            mine.target = a.targets[mine.row];
+            row_scale(a, mine.row, mine.scale, mine.inv_t);
+            mine.in = policy_in(a, mine.row, a.weights ? a.weights[mine.row] : 1.0f / float(a.rows));
+            mine.x_target = mine.target < a.vocab ? D::load(logits_row(mine.row) + mine.target) : NAN;
           }
         }
-        const T* x = logits_row(k);
+      }
+      end = walk.mine == 0;
+      const int of = end ? 0 : __ffs(walk.mine) - 1;
+      walk.mine &= walk.mine - 1;
+      const int64_t row = __shfl_sync(~0u, mine.row, of);
+      Share s = {};
+      const uint4* src = nullptr;
+      if (!end && __shfl_sync(~0u, mine.alive, of)) {
+        const T* x = logits_row(row);
         s = row_share<E>(x, int(a.vocab), rank, shift);
         src = reinterpret_cast<const uint4*>(x + s.head) + s.v0;
       }
@@ -969,9 +1014,9 @@ __global__ void __launch_bounds__(kHeldThreads, HeldShape<LARGE>::kBlocks)
       do {                              // a row has one chunk at least: it carries the row's numbers
         bad = __any_sync(~0u, !mbar_wait_bounded(&sh.empty[slot], phase));
         if (bad) break;
-        if (at == 0) {
-          if (end && lane == 0) sh.info[slot].k = -1;
-          if (!end && lane == int(k & 31)) sh.info[slot] = mine;
+        if (at == 0 && lane == of) {
+          sh.info[slot] = mine;
+          if (end) sh.info[slot].row = -1;
         }
         __syncwarp();
         if (lane == 0) {
@@ -985,7 +1030,6 @@ __global__ void __launch_bounds__(kHeldThreads, HeldShape<LARGE>::kBlocks)
           phase ^= 1;
         }
       } while (at < s.n);
-      k = end ? -1 : k + 1;
     }
     // the copies end before the block does
     if (bad)
@@ -1000,16 +1044,26 @@ __global__ void __launch_bounds__(kHeldThreads, HeldShape<LARGE>::kBlocks)
     Share s = {};
     int edge_at = -1;
     uint32_t start = ~0u;
-    int64_t done = 0;
     while (true) {
       // ---- the row's sums, chunk after chunk as they land
       const int first_slot = slot;
       F2 sum[2] = {0, 0}, u[2] = {0, 0};
       if (!bad) bad = !mbar_wait_bounded(&sh.full[slot], phase);
-      const int64_t k = bad ? -1 : sh.info[first_slot].k;
-      if (k < 0) break;
-      done = k + 1;
-      const T* x = logits_row(k);
+      const int64_t row = bad ? -1 : sh.info[first_slot].row;
+      if (row < 0) break;
+      const T* x = logits_row(row);
+      T* out = static_cast<T*>(a.grad_logits) + row * a.grad_stride;
+      if (!sh.info[first_slot].alive) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.empty[slot]);
+        if (++slot == kSlots) {
+          slot = 0;
+          phase ^= 1;
+        }
+        if (rank == 0 && tid == 0) write_dead_row<kPolicy>(a, row);
+        write_zeros<DT, kRowThreads>(out, a.vocab, rank, blocks);
+        continue;
+      }
       if ((uint32_t(reinterpret_cast<uintptr_t>(x)) & 15) != start) {
         start = uint32_t(reinterpret_cast<uintptr_t>(x)) & 15;
         s = row_share<E>(x, int(a.vocab), rank, shift);
@@ -1076,7 +1130,6 @@ __global__ void __launch_bounds__(kHeldThreads, HeldShape<LARGE>::kBlocks)
       row_barrier();
       // ---- joined, and turned into the row's numbers, by the first warp
       if (warp == 0) {
-        const int64_t row = first_row + k * clusters;
         Part p;
         {
           const float2 v = lane < kRowWarps ? sh.warp_part[lane] : make_float2(0.0f, 0.0f);
@@ -1142,7 +1195,6 @@ __global__ void __launch_bounds__(kHeldThreads, HeldShape<LARGE>::kBlocks)
       row_barrier();
       // ---- its gradient; every chunk goes to the next row as it is done
       const GradRow g = sh.coef;
-      T* out = grad_out(k);
       if (edge_at >= 0) {
         if (g.zero)
           D::store(out + edge_at, 0.0f);
@@ -1186,18 +1238,9 @@ __global__ void __launch_bounds__(kHeldThreads, HeldShape<LARGE>::kBlocks)
       const unsigned target = unsigned(g.target - s.head) - unsigned(s.v0) * E;
       if (!g.zero && target < unsigned(s.n) * E && int(target / E) % kRowThreads == tid) D::store(mine + target, g.at);
     }
-    // ---- the rows without a token
-    RowWalk walk;
-    walk.rows = rows;
-    if (bad) {                             // nor have those behind a wait that ran out
-      for (int64_t k = walk.next(a, first_row, clusters, done, true); k < rows; k = walk.next(a, first_row, clusters, k + 1, true))
-        if (tid == 0) a.logprobs[first_row + k * clusters] = a.row_loss[first_row + k * clusters] = NAN;
-      walk.window = -1;
-    }
-    for (int64_t k = walk.next(a, first_row, clusters, 0, false); k < rows; k = walk.next(a, first_row, clusters, k + 1, false)) {
-      if (rank == 0 && tid == 0) write_dead_row<kPolicy>(a, first_row + k * clusters);
-      write_zeros<DT>(grad_out(k), a.vocab, rank, blocks, kRowThreads);
-    }
+    // a wait ran out: rows are left over, and with them there is no loss
+    if (__any_sync(~0u, bad))
+      for (int64_t i = tid; i < a.rows; i += kRowThreads) a.row_loss[i] = a.logprobs[i] = NAN;
   }
   if (blocks > 1) cluster.sync();        // no block leaves while a peer may still write to it
 }
@@ -1328,14 +1371,14 @@ bool policy_held(const LossArgs& a, int dtype, cudaStream_t stream, int* rc) {
 
 template <int DT>
 int launch_grad(const LossArgs& a, cudaStream_t stream) {
-  const int64_t per = int64_t(kThreads) * kGradVecs * Elem<DT>::E;    // shares differ by one vector at most
+  const int64_t per = int64_t(kGradThreads) * kGradVecs * Elem<DT>::E;    // shares differ by one vector at most
   const int chunks = int((a.vocab + per - 1) / per);
   const int64_t blocks = a.rows * chunks;
   if (blocks > 0x7FFFFFFF) return NS_ERR_INVALID_ARGUMENT;
   if (a.grad_entropy)
-    grad_kernel<DT, true><<<unsigned(blocks), kThreads, 0, stream>>>(a, chunks);
+    grad_kernel<DT, true><<<unsigned(blocks), kGradThreads, 0, stream>>>(a, chunks);
   else
-    grad_kernel<DT, false><<<unsigned(blocks), kThreads, 0, stream>>>(a, chunks);
+    grad_kernel<DT, false><<<unsigned(blocks), kGradThreads, 0, stream>>>(a, chunks);
   return cudaGetLastError() == cudaSuccess ? NS_OK : NS_ERR_CUDA;
 }
 
