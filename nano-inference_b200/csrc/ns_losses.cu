@@ -269,11 +269,10 @@ __device__ __forceinline__ Span row_span(const void* row, int64_t vocab) {
   return {head, (vocab - head) / E};
 }
 
-// Block `rank` of `blocks` adds its share of the row with a running maximum:
-// the part of a thread whose columns rise is rescaled.
-template <int DT, bool ENT>
-__device__ __noinline__ Part running_part(const void* base, int64_t vocab, float scale, int rank, int blocks,
-                                          Part* shared) {
+// One thread's part of share `rank` of `blocks` of a row with a running
+// maximum: the part of a thread whose columns rise is rescaled.
+template <int DT, bool ENT, int THREADS>
+__device__ __forceinline__ Part thread_running(const void* base, int64_t vocab, float scale, int rank, int blocks, int tid) {
   using D = Elem<DT>;
   using T = typename D::T;
   constexpr int E = D::E;
@@ -282,21 +281,25 @@ __device__ __noinline__ Part running_part(const void* base, int64_t vocab, float
   const int64_t v0 = sp.nv * rank / blocks, v1 = sp.nv * (rank + 1) / blocks;
   const uint4* vec = reinterpret_cast<const uint4*>(row + sp.head);
   Part p = {-INFINITY, 0.0f, 0.0f};
-  for (int64_t v = v0 + threadIdx.x; v < v1; v += kThreads) {
+  for (int64_t v = v0 + tid; v < v1; v += THREADS) {
     float x[E];
     D::unpack(vec[v], x);
     add<ENT>(p, x, scale);
   }
-  if (rank == 0 && threadIdx.x < sp.head) {
-    const float x[1] = {D::load(row + threadIdx.x)};
-    add<ENT>(p, x, scale);
-  }
-  const int64_t tail = sp.head + sp.nv * E + threadIdx.x;
-  if (rank == blocks - 1 && tail < vocab) {
-    const float x[1] = {D::load(row + tail)};
-    add<ENT>(p, x, scale);
-  }
-  p = warp_join<ENT>(p, scale);
+  const int64_t tail = sp.head + sp.nv * E + tid;
+  const float x[2] = {rank == 0 && tid < sp.head ? D::load(row + tid) : -INFINITY,
+                      rank == blocks - 1 && tail < vocab ? D::load(row + tail) : -INFINITY};
+  add<ENT>(p, x, scale);
+  return p;
+}
+template <int DT, bool ENT>
+__device__ __noinline__ Part warp_running(const void* base, int64_t vocab, float scale, int rank, int blocks) {
+  return warp_join<ENT>(thread_running<DT, ENT, 32>(base, vocab, scale, rank, blocks, threadIdx.x & 31), scale);
+}
+template <int DT, bool ENT>
+__device__ __noinline__ Part block_running(const void* base, int64_t vocab, float scale, int rank, int blocks,
+                                           Part* shared) {
+  Part p = warp_join<ENT>(thread_running<DT, ENT, kThreads>(base, vocab, scale, rank, blocks, threadIdx.x), scale);
   __syncthreads();
   if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = p;
   __syncthreads();
@@ -337,14 +340,13 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// The sums around c over part `rank` of `parts` of a row, in every thread.
-template <int DT, bool ENT>
-__device__ __forceinline__ Part part_sums(const void* base, int64_t vocab, float c, float scale, int rank, int parts,
-                                          Part* shared) {
+// One thread's sums around c over part `rank` of `parts` of a row that THREADS threads add up.
+template <int DT, bool ENT, int THREADS>
+__device__ __forceinline__ Part thread_sums(const void* base, int64_t vocab, float c, float scale, int rank, int parts,
+                                            int tid) {
   using D = Elem<DT>;
   using T = typename D::T;
   constexpr int E = D::E;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const T* row = static_cast<const T*>(base);
   const Span sp = row_span<E>(row, vocab);
   const int v0 = int(sp.nv * rank / parts), n = int(sp.nv * (rank + 1) / parts) - v0;
@@ -353,20 +355,20 @@ __device__ __forceinline__ Part part_sums(const void* base, int64_t vocab, float
   uint4 q[kBatch];
 #pragma unroll
   for (int k = 0; k < kBatch; ++k) {
-    const int v = int(threadIdx.x) + k * kThreads;
+    const int v = tid + k * THREADS;
     q[k] = v < n ? vec[v] : none;
   }
   // the elements before the first 16-byte boundary and after the last whole vector
-  const int64_t tail = sp.head + sp.nv * E + threadIdx.x;
-  const float edge[2] = {rank == 0 && threadIdx.x < sp.head ? D::load(row + threadIdx.x) : -INFINITY,
+  const int64_t tail = sp.head + sp.nv * E + tid;
+  const float edge[2] = {rank == 0 && tid < sp.head ? D::load(row + tid) : -INFINITY,
                          rank == parts - 1 && tail < vocab ? D::load(row + tail) : -INFINITY};
   const auto scaled = ScaledPairs<DT>::of(c, scale);
   F2 s[2] = {0, 0}, u[2] = {0, 0};
-  for (int v = threadIdx.x; v < n; v += kBatch * kThreads) {
+  for (int v = tid; v < n; v += kBatch * THREADS) {
     uint4 next[kBatch];
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
-      const int at = v + (kBatch + k) * kThreads;
+      const int at = v + (kBatch + k) * THREADS;
       next[k] = at < n ? vec[at] : none;
     }
 #pragma unroll
@@ -377,19 +379,26 @@ __device__ __forceinline__ Part part_sums(const void* base, int64_t vocab, float
   }
   Part p;
   p.m = c;
-  {
-    float a, b;
-    split(add2(s[0], s[1]), a, b);
-    p.s = a + b;
-    split(add2(u[0], u[1]), a, b);
-    p.u = a + b;
-  }
+  float lo, hi;
+  split(add2(s[0], s[1]), lo, hi);
+  p.s = lo + hi;
+  split(add2(u[0], u[1]), lo, hi);
+  p.u = lo + hi;
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const float t = scaled_one<DT>(edge[k], c, scale), e = ex2_approx(t);
     p.s += e;
     if (ENT) p.u = fmaf(e, fmaxf(t, -200.0f), p.u);
   }
+  return p;
+}
+
+// The sums around c over part `rank` of `parts` of a row, in every thread.
+template <int DT, bool ENT>
+__device__ __forceinline__ Part part_sums(const void* base, int64_t vocab, float c, float scale, int rank, int parts,
+                                          Part* shared) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  Part p = thread_sums<DT, ENT, kThreads>(base, vocab, c, scale, rank, parts, threadIdx.x);
   p.s = warp_sum(p.s);
   if (ENT) p.u = warp_sum(p.u);
   if (lane == 0) shared[warp] = p;
@@ -418,7 +427,7 @@ __device__ __forceinline__ Part row_sums(const void* base, int64_t vocab, float 
   }
   near = !sums_far(p.s);             // the same for the whole cluster
   if (near) return p;
-  p = running_part<DT, ENT>(base, vocab, scale, rank, blocks, sh.warp);
+  p = block_running<DT, ENT>(base, vocab, scale, rank, blocks, sh.warp);
   if (blocks > 1) {
     cluster.sync();                    // every block has read the first sums
     if (int(threadIdx.x) < blocks) *cluster.map_shared_rank(&sh.block[rank], threadIdx.x) = p;
@@ -617,6 +626,22 @@ __device__ __forceinline__ void write_dead_row(const LossArgs& a, int64_t row) {
   if (OP == kPreference) a.row_grad[row] = 0.0f;
 }
 
+// What a forward call leaves of a row (one thread).
+template <int DT, bool ENT, int OP>
+__device__ __forceinline__ void write_row(const LossArgs& a, int64_t row, const Part& p, float x_target, float scale,
+                                          float w, bool near) {
+  const RowResult r = finish<DT, ENT>(p, x_target, scale, near);
+  a.logprobs[row] = float(r.logprob);
+  if (ENT) a.entropy[row] = r.entropy;
+  if (a.stats) {
+    a.stats[2 * row] = p.m;
+    a.stats[2 * row + 1] = r.log2s;
+  }
+  if (OP == kPolicy) write_policy_row(a, row, policy_row(a, policy_in(a, row, w), r.logprob, r.entropy));
+  if (OP == kPreference)   // the row's gain; the pair kernel turns it into the coefficient
+    a.row_grad[row] = float(r.logprob - (a.ref_logprobs ? double(a.ref_logprobs[row]) : 0.0));
+}
+
 // One cluster of blocks per row.
 template <int DT, bool ENT, int OP>
 __global__ void __launch_bounds__(kThreads) forward_kernel(const LossArgs a) {
@@ -639,17 +664,36 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const LossArgs a) {
   const float x_target = target < a.vocab ? D::load(x + target) : NAN;
   bool near;
   const Part p = row_sums<DT, ENT>(x, a.vocab, row_offset<DT>(x_target, scale), scale, sh, cluster, near);
-  if (threadIdx.x != 0 || rank != 0) return;
-  const RowResult r = finish<DT, ENT>(p, x_target, scale, near);
-  a.logprobs[row] = float(r.logprob);
-  if (ENT) a.entropy[row] = r.entropy;
-  if (a.stats) {
-    a.stats[2 * row] = p.m;
-    a.stats[2 * row + 1] = r.log2s;
+  if (threadIdx.x == 0 && rank == 0) write_row<DT, ENT, OP>(a, row, p, x_target, scale, w, near);
+}
+
+// One warp per row, for rows so short that a block's barriers would be most of
+// the work.  8192 x 2000 bf16: 33 us by blocks.
+template <int DT, bool ENT, int OP>
+__global__ void __launch_bounds__(kThreads) forward_rows_kernel(const LossArgs a) {
+  using D = Elem<DT>;
+  using T = typename D::T;
+  const int64_t row = int64_t(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (row >= a.rows) return;
+  float w;
+  if (!row_alive<OP>(a, row, w)) {
+    if (lane == 0) write_dead_row<OP>(a, row);
+    return;
   }
-  if (OP == kPolicy) write_policy_row(a, row, policy_row(a, policy_in(a, row, w), r.logprob, r.entropy));
-  if (OP == kPreference)   // the row's gain; the pair kernel turns it into the coefficient
-    a.row_grad[row] = float(r.logprob - (a.ref_logprobs ? double(a.ref_logprobs[row]) : 0.0));
+  float scale;
+  double inv_t;
+  row_scale(a, row, scale, inv_t);
+  const T* x = static_cast<const T*>(a.logits) + row * a.row_stride;
+  const int64_t target = a.targets[row];
+  const float x_target = target < a.vocab ? D::load(x + target) : NAN;
+  const float c = row_offset<DT>(x_target, scale);
+  Part p = thread_sums<DT, ENT, 32>(x, a.vocab, c, scale, 0, 1, lane);
+  p.s = warp_sum(p.s);
+  if (ENT) p.u = warp_sum(p.u);
+  const bool near = !sums_far(p.s);
+  if (!near) p = warp_running<DT, ENT>(x, a.vocab, scale, 0, 1);
+  if (lane == 0) write_row<DT, ENT, OP>(a, row, p, x_target, scale, w, near);
 }
 
 __device__ __forceinline__ double block_sum(double v, double* shared) {
@@ -865,10 +909,8 @@ struct HeldShared {
   float2 part[2][kMaxCluster];     // (S, U) of each block
   float4 far_part[kMaxCluster];    // (m, S, U)
   float2 warp_part[kRowWarps];
-  Part far_warp[kRowWarps];
   RowInfo info[16];                // of the row whose first chunk lies in the slot
   GradRow coef;
-  int far;
 };
 
 __device__ __forceinline__ uint32_t peer_addr(const void* p, int rank) {
@@ -1151,19 +1193,7 @@ __global__ void __launch_bounds__(kHeldThreads, HeldShape<LARGE>::kBlocks)
         const bool near = !sums_far(p.s);
         if (!near) {
           // one warp of a block: a row whose target is all but impossible is rare
-          Part q = {-INFINITY, 0.0f, 0.0f};
-          const uint4* vec = reinterpret_cast<const uint4*>(x + s.head) + s.v0;
-          for (int v = lane; v < s.n; v += 32) {
-            float f[E];
-            D::unpack(vec[v], f);
-            add<ENT>(q, f, scale);
-          }
-          const Span sp = row_span<E>(x, a.vocab);
-          const int64_t tail = sp.head + sp.nv * E + lane;
-          const float f[2] = {rank == 0 && lane < sp.head ? D::load(x + lane) : -INFINITY,
-                              rank == blocks - 1 && tail < a.vocab ? D::load(x + tail) : -INFINITY};
-          add<ENT>(q, f, scale);
-          p = warp_join<ENT>(q, scale);
+          p = warp_running<DT, ENT>(x, a.vocab, scale, rank, blocks);
           if (blocks > 1) {
             if (lane == 0) mbar_arrive_expect_tx(&sh.far_bar, uint32_t(blocks) * 16);
             __syncwarp();
@@ -1282,6 +1312,12 @@ int launch_forward(const LossArgs& a, cudaStream_t stream) {
   int sms = 0;
   if (const int rc = sm_count(&sms)) return rc;
   const int64_t vectors = a.vocab / Elem<DT>::E;
+  // a warp per row while rows are short and many: 4096 x 8000 bf16 15 us against 21, 1024 x 4000 6 against 8;
+  // at 2048 x 16000 and for 300 rows the two are even
+  if (vectors <= 1024 && a.rows >= 2 * sms) {
+    forward_rows_kernel<DT, ENT, OP><<<unsigned((a.rows + kWarps - 1) / kWarps), kThreads, 0, stream>>>(a);
+    return cudaGetLastError() == cudaSuccess ? NS_OK : NS_ERR_CUDA;
+  }
   // blocks per row: enough to give every SM two, each thread at least one vector
   int blocks = 1;
   while (blocks < kMaxCluster && a.rows * blocks < 2 * sms && vectors >= int64_t(2) * blocks * kThreads) blocks *= 2;
