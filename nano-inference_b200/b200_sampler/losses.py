@@ -7,7 +7,8 @@
 ``policy_loss_and_grad`` and ``preference_loss_and_grad`` return the loss
 together with dloss/dlogits, without a graph: the gradient may take the logits'
 place (``out=logits``), and the policy loss computes both from one reading of
-the logits.
+the logits.  They are also the calls to capture in a CUDA graph: they allocate,
+launch and return, where a captured ``backward()`` has torch's own rules.
 
 One row of ``logits`` [rows, vocab] (fp32, bf16 or fp16, any row stride) holds
 one token, and ``targets`` (int64 [rows]) its id: what ``B200Sampler`` draws,
@@ -87,7 +88,7 @@ def _check(name: str, t: torch.Tensor, n: int, device: torch.device) -> None:
 def _vector(name: str, t: Optional[torch.Tensor], n: int, device: torch.device) -> Optional[torch.Tensor]:
     if t is None:
         return None
-    if t.dtype != torch.float32:
+    if t.dtype is not torch.float32:
         if not t.is_floating_point():
             raise TypeError(f"{name} must be floating point")
         t = t.detach().float()
@@ -232,11 +233,10 @@ def _policy(logits, targets, old_logprobs, advantages, ref_logprobs, weights, te
         raise ValueError("kl_coef and entropy_coef must be finite")
     if kl_coef != 0.0 and ref_logprobs is None:
         raise ValueError("a KL term needs ref_logprobs")
-    vectors = [_vector(name, t, n, device) for name, t in
-               (("old_logprobs", old_logprobs), ("ref_logprobs", ref_logprobs), ("advantages", advantages),
-                ("weights", weights))]
-    if vectors[0] is None or vectors[2] is None:
+    if old_logprobs is None or advantages is None:
         raise ValueError("old_logprobs and advantages are needed")
+    vectors = (_vector("old_logprobs", old_logprobs, n, device), _vector("ref_logprobs", ref_logprobs, n, device),
+               _vector("advantages", advantages, n, device), _vector("weights", weights, n, device))
     return logits, targets, temperature, t_all, vectors, (clip_low, clip_high, kl_coef, entropy_coef)
 
 
@@ -249,7 +249,7 @@ def _policy_forward(logits, targets, temperature, t_all, vectors, coefs, grad):
     row_grad = row_grad.view(2, n)
     entropy = rest[0] if has_entropy else None
     kl = rest[-1] if has_kl else None
-    _call("ns_policy_loss", logits.device, *_head(logits, targets, temperature, t_all), *(_ptr(v) for v in vectors),
+    _call("ns_policy_loss", logits.device, *_head(logits, targets, temperature, t_all), *map(_ptr, vectors),
           *coefs, loss.data_ptr(), row_loss.data_ptr(), logprobs.data_ptr(), _ptr(entropy), _ptr(kl),
           stats.data_ptr(), row_grad.data_ptr(), _ptr(grad), 0 if grad is None else _stride(grad))
     return PolicyLoss(loss, row_loss, logprobs, entropy, kl), stats, row_grad

@@ -8,8 +8,7 @@
 // the entropy is ln2 (log2 S - U / S).  Any offset near the row's largest logit
 // would do in fp32; the target's is known before the row is read and is the
 // same for every thread and block of the row, so no maximum is kept and no sum
-// is ever rescaled: the exponential's error (2^-22, and -5e-8 on average,
-// measured over 4 M arguments) enters once.  The difference is taken before the
+// is ever rescaled: the exponential's error enters once.  The difference is taken before the
 // scale, so a row whose logits are all the type's lowest value still gets its
 // uniform distribution.  A row whose S leaves [2^-60, 2^100] (a target less
 // likely than 2^-100, or barred) is added up again with a running maximum.  The
@@ -43,6 +42,9 @@ constexpr int kMaxCluster = 8;
 constexpr int kBatch = 2;          // 16-byte loads a thread has in flight
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr double kLn2 = 0.6931471805599453;
+// Mean relative error of ex2.approx.ftz.f32, measured over 4 M arguments in [-30, 0]: -5.07e-8, between -3.4e-8 and
+// -6.1e-8 in every sixteenth of an octave (largest 1.4e-7).
+constexpr double kEx2Mean = 5.07e-8;
 
 enum Op { kLogprob = 0, kPolicy = 1, kPreference = 2 };
 
@@ -454,11 +456,14 @@ __device__ __forceinline__ RowResult finish(const Part& p, float x_target, float
   const double ln_s = p.s < INFINITY && p.s > 0.0f ? double(ex - 1) * kLn2 + double(logf(mant)) : double(NAN);
   // how far the sums' offset lies from m s
   const double moved = DT != NS_DTYPE_F32 && near ? double(__fmul_rn(p.m, scale)) - double(p.m) * double(scale) : 0.0;
+  // the exponentials are kEx2Mean low on average, but for the target's own, 2^0 = 1, which is p of S.  A
+  // sequence's reward adds such errors up, a gradient's p divides them out
+  const double ln_all = ln_s + (near ? kEx2Mean * (1.0 - double(1.0f / p.s)) : 0.0);
   RowResult r;
-  r.logprob = ((double(x_target) - double(p.m)) * double(scale) - moved) * kLn2 - ln_s;
+  r.logprob = ((double(x_target) - double(p.m)) * double(scale) - moved) * kLn2 - ln_all;
   if (r.logprob > 0.0) r.logprob = 0.0;          // a rounding of S
   r.log2s = float(ln_s * (1.0 / kLn2) + moved);
-  r.entropy = ENT ? float(ln_s) - float(kLn2) * (p.u / p.s) : 0.0f;
+  r.entropy = ENT ? float(ln_all) - float(kLn2) * (p.u / p.s) : 0.0f;
   if (isnan(r.logprob)) r.log2s = r.entropy = NAN;
   return r;
 }
@@ -876,19 +881,20 @@ __global__ void __launch_bounds__(kGradThreads) grad_kernel(const LossArgs a, in
 // bytes a logit need, and a row's sums cannot end before its last chunk lands.
 // Loading the registers straight from memory instead was slower (10 us a row of
 // 123 KB): beside 215 KB of shared memory L1 has room for few loads.
-constexpr int kRowWarps = 15;
-constexpr int kRowThreads = kRowWarps * 32;
-constexpr int kHeldThreads = kRowThreads + 32;      // and the producer warp
-
-// Two shapes: one block of an SM with registers, or two with smaller rings.
-template <bool LARGE>
+// The shapes of a block: 15 row warps with registers, alone on an SM; 15 with
+// a smaller ring, two to an SM; 7, three to an SM.
+enum Shape { kLarge = 0, kMedium = 1, kSmall = 2 };
+template <int SHAPE>
 struct HeldShape {
-  static constexpr int kLaneVecs = LARGE ? 4 : 2;   // of a chunk
+  static constexpr int kRowWarps = SHAPE == kSmall ? 7 : 15;
+  static constexpr int kRowThreads = kRowWarps * 32;
+  static constexpr int kThreads = kRowThreads + 32;          // and the producer warp
+  static constexpr int kLaneVecs = SHAPE == kLarge ? 4 : 2;  // of a chunk
   static constexpr int kChunkVecs = kRowThreads * kLaneVecs;
   static constexpr int kChunkBytes = kChunkVecs * 16;
-  static constexpr int kHold = LARGE ? 4 : 0;       // chunks in registers
-  static constexpr int kSlots = 7;
-  static constexpr int kBlocks = LARGE ? 1 : 2;
+  static constexpr int kHold = SHAPE == kLarge ? 4 : 0;      // chunks in registers
+  static constexpr int kSlots = SHAPE == kSmall ? 10 : 7;
+  static constexpr int kBlocks = SHAPE == kLarge ? 1 : SHAPE == kMedium ? 2 : 3;
   static constexpr int kMostVecs = (kHold + kSlots - 1) * kChunkVecs;
   static constexpr uint32_t kSmem = uint32_t(kSlots) * kChunkBytes;
 };
@@ -908,7 +914,7 @@ struct HeldShared {
   uint64_t far_bar;                // the same for a row that is added up again
   float2 part[2][kMaxCluster];     // (S, U) of each block
   float4 far_part[kMaxCluster];    // (m, S, U)
-  float2 warp_part[kRowWarps];
+  float2 warp_part[16];
   RowInfo info[16];                // of the row whose first chunk lies in the slot
   GradRow coef;
 };
@@ -928,7 +934,10 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 // The barrier of the row warps.
-__device__ __forceinline__ void row_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(kRowThreads) : "memory"); }
+template <int THREADS>
+__device__ __forceinline__ void row_barrier() {
+  asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
+}
 
 // A cluster's rows in order.  The rows that hold a token are dealt out in turn,
 // and so are those that do not, so every cluster has its share of both however
@@ -992,12 +1001,13 @@ __device__ __forceinline__ Share row_share(const void* base, int vocab, int rank
   return s;
 }
 
-template <int DT, bool ENT, bool LARGE>
-__global__ void __launch_bounds__(kHeldThreads, HeldShape<LARGE>::kBlocks)
+template <int DT, bool ENT, int SHAPE>
+__global__ void __launch_bounds__(HeldShape<SHAPE>::kThreads, HeldShape<SHAPE>::kBlocks)
     policy_kernel(const __grid_constant__ LossArgs a) {
   using D = Elem<DT>;
   using T = typename D::T;
-  using H = HeldShape<LARGE>;
+  using H = HeldShape<SHAPE>;
+  constexpr int kRowWarps = H::kRowWarps, kRowThreads = H::kRowThreads;
   constexpr int E = D::E, kHold = H::kHold, kSlots = H::kSlots, kLaneVecs = H::kLaneVecs, kChunkVecs = H::kChunkVecs;
   __shared__ HeldShared sh;
   extern __shared__ __align__(128) uint4 ring[];
@@ -1169,7 +1179,7 @@ __global__ void __launch_bounds__(kHeldThreads, HeldShape<LARGE>::kBlocks)
         bad = __any_sync(~0u, bad);
         if (lane == 0) sh.warp_part[warp] = make_float2(bad ? NAN : total, mean);
       }
-      row_barrier();
+      row_barrier<kRowThreads>();
       // ---- joined, and turned into the row's numbers, by the first warp
       if (warp == 0) {
         Part p;
@@ -1222,7 +1232,7 @@ __global__ void __launch_bounds__(kHeldThreads, HeldShape<LARGE>::kBlocks)
           }
         }
       }
-      row_barrier();
+      row_barrier<kRowThreads>();
       // ---- its gradient; every chunk goes to the next row as it is done
       const GradRow g = sh.coef;
       if (edge_at >= 0) {
@@ -1342,16 +1352,16 @@ int forward(const LossArgs& a, int dtype, cudaStream_t stream) {
 }
 
 // Blocks per row of policy_kernel: the fewest that hold a row on chip; 0 when kMaxCluster do not.
-template <bool LARGE>
+template <int SHAPE>
 int held_blocks(int64_t vectors) {
   for (int blocks = 1; blocks <= kMaxCluster; blocks *= 2)
-    if ((vectors + blocks - 1) / blocks <= HeldShape<LARGE>::kMostVecs) return blocks;
+    if ((vectors + blocks - 1) / blocks <= HeldShape<SHAPE>::kMostVecs) return blocks;
   return 0;
 }
 
-template <int DT, bool ENT, bool LARGE>
+template <int DT, bool ENT, int SHAPE>
 int launch_policy(const LossArgs& a, int blocks, cudaStream_t stream) {
-  using H = HeldShape<LARGE>;
+  using H = HeldShape<SHAPE>;
   static std::mutex mu;
   static int known[64][kMaxCluster + 1];         // clusters that a device holds at once
   int dev = 0;
@@ -1360,12 +1370,12 @@ int launch_policy(const LossArgs& a, int blocks, cudaStream_t stream) {
   {
     std::lock_guard<std::mutex> lk(mu);
     if (known[dev][blocks] == 0) {
-      if (cudaFuncSetAttribute(policy_kernel<DT, ENT, LARGE>, cudaFuncAttributeMaxDynamicSharedMemorySize, H::kSmem) !=
+      if (cudaFuncSetAttribute(policy_kernel<DT, ENT, SHAPE>, cudaFuncAttributeMaxDynamicSharedMemorySize, H::kSmem) !=
           cudaSuccess)
         return NS_ERR_CUDA;
       cudaLaunchConfig_t cfg = {};
       cfg.gridDim = dim3(unsigned(blocks) * 64);
-      cfg.blockDim = dim3(kHeldThreads);
+      cfg.blockDim = dim3(H::kThreads);
       cfg.dynamicSmemBytes = H::kSmem;
       cudaLaunchAttribute at[1];
       at[0].id = cudaLaunchAttributeClusterDimension;
@@ -1374,35 +1384,55 @@ int launch_policy(const LossArgs& a, int blocks, cudaStream_t stream) {
       cfg.attrs = at;
       cfg.numAttrs = 1;
       int n = 0;
-      if (cudaOccupancyMaxActiveClusters(&n, policy_kernel<DT, ENT, LARGE>, &cfg) != cudaSuccess || n < 1) return NS_ERR_CUDA;
+      if (cudaOccupancyMaxActiveClusters(&n, policy_kernel<DT, ENT, SHAPE>, &cfg) != cudaSuccess || n < 1) return NS_ERR_CUDA;
       known[dev][blocks] = n;
     }
     clusters = known[dev][blocks];
   }
   const int64_t grid = std::min<int64_t>(a.rows, clusters) * blocks;
-  return launch_clusters(policy_kernel<DT, ENT, LARGE>, grid, kHeldThreads, blocks, H::kSmem, stream, a);
+  return launch_clusters(policy_kernel<DT, ENT, SHAPE>, grid, H::kThreads, blocks, H::kSmem, stream, a);
 }
 
+template <int DT, int SHAPE>
+int launch_shape(const LossArgs& a, int blocks, cudaStream_t stream) {
+  return a.entropy ? launch_policy<DT, true, SHAPE>(a, blocks, stream) : launch_policy<DT, false, SHAPE>(a, blocks, stream);
+}
+
+// The gradient with the loss in one launch; `held` is false where a launch for
+// the sums and one for the gradient do better (rows too short) or must (rows
+// past the chip).  Measured on a B200, us by shape (large / medium / small /
+// two launches):
+//   2048 x 16000 bf16    53 / 46 / 36 / 39      4096 x 8000 bf16   81 / 72 / 54 / 37
+//   2048 x 32000 bf16    69 / 62 / 53 / 69       777 x 64007 fp16  52 / 48 / 45 / 54
+//   1000 x 100000 bf16   79 / 98 / -  / -       2048 x 151936 bf16 214 / 264 / 290 / 285
+//    333 x 151936 bf16   55 / 49 / -  / 62       600 x 151936 fp32 134 / 123 / - / 170
+// Short rows spend their time in joins, which more blocks of an SM hide.
+// 16-bit rows are bound by their exponentials and want whole SMs without a
+// cluster's join; fp32 rows and few rows want their columns spread.  Below
+// 16 MB of logits two launches over all SMs win (16 x 32000 bf16 9.4 against
+// 11.0, 200 x 32000 12.9 against 13.6; 64 x 151936 15.5 against 13.8).
 template <int DT>
-int policy_typed(const LossArgs& a, int blocks, bool large, cudaStream_t stream) {
-  if (a.entropy)
-    return large ? launch_policy<DT, true, true>(a, blocks, stream) : launch_policy<DT, true, false>(a, blocks, stream);
-  return large ? launch_policy<DT, false, true>(a, blocks, stream) : launch_policy<DT, false, false>(a, blocks, stream);
+int policy_held(const LossArgs& a, cudaStream_t stream, bool* held) {
+  int sms = 0;
+  if (const int rc = sm_count(&sms)) return rc;
+  const int64_t vectors = a.vocab / Elem<DT>::E;
+  const int small = held_blocks<kSmall>(vectors), medium = held_blocks<kMedium>(vectors), large = held_blocks<kLarge>(vectors);
+  *held = true;
+  if (vectors >= 1800 && a.rows * vectors >= (int64_t(16) << 20) / 16) {
+    if (small == 1 || (small == 2 && DT != NS_DTYPE_F32)) return launch_shape<DT, kSmall>(a, small, stream);
+    if (medium && (DT == NS_DTYPE_F32 || 2 * a.rows < 5 * sms)) return launch_shape<DT, kMedium>(a, medium, stream);
+    if (large) return launch_shape<DT, kLarge>(a, large, stream);
+  }
+  *held = false;
+  return NS_OK;
 }
 
-// The gradient with the loss, when a row can be held; false: it cannot.
-bool policy_held(const LossArgs& a, int dtype, cudaStream_t stream, int* rc) {
-  const int64_t vectors = a.vocab / (dtype == NS_DTYPE_F32 ? 4 : 8);
-  const char* env = getenv("NS_LARGE");
-  const bool large = env ? atoi(env) : vectors > HeldShape<false>::kMostVecs;
-  const int blocks = large ? held_blocks<true>(vectors) : held_blocks<false>(vectors);
-  if (blocks == 0 || (env && atoi(env) == 2)) return false;
+int policy_held(const LossArgs& a, int dtype, cudaStream_t stream, bool* held) {
   switch (dtype) {
-    case NS_DTYPE_F32: *rc = policy_typed<NS_DTYPE_F32>(a, blocks, large, stream); break;
-    case NS_DTYPE_BF16: *rc = policy_typed<NS_DTYPE_BF16>(a, blocks, large, stream); break;
-    default: *rc = policy_typed<NS_DTYPE_F16>(a, blocks, large, stream);
+    case NS_DTYPE_F32: return policy_held<NS_DTYPE_F32>(a, stream, held);
+    case NS_DTYPE_BF16: return policy_held<NS_DTYPE_BF16>(a, stream, held);
+    default: return policy_held<NS_DTYPE_F16>(a, stream, held);
   }
-  return true;
 }
 
 template <int DT>
@@ -1527,12 +1557,14 @@ int ns_policy_loss(const void* logits, int dtype, int64_t rows, int64_t vocab, i
   a.grad_entropy = entropy_coef != 0.0f ? row_grad + rows : nullptr;
   a.grad_logits = grad_logits;
   a.grad_stride = grad_stride;
-  int rc = NS_OK;
-  if (!grad_logits || !ns::policy_held(a, dtype, s, &rc)) {
-    rc = ns::forward<ns::kPolicy>(a, dtype, s);
-    if (rc == NS_OK && grad_logits) rc = ns::gradient(a, dtype, s);
+  bool held = false;
+  if (grad_logits)
+    if (const int rc = ns::policy_held(a, dtype, s, &held)) return rc;
+  if (!held) {
+    if (const int rc = ns::forward<ns::kPolicy>(a, dtype, s)) return rc;
+    if (grad_logits)
+      if (const int rc = ns::gradient(a, dtype, s)) return rc;
   }
-  if (rc != NS_OK) return rc;
   ns::policy_sum_kernel<<<1, 1024, 0, s>>>(a, loss);
   return cudaGetLastError() == cudaSuccess ? NS_OK : NS_ERR_CUDA;
 }

@@ -303,6 +303,43 @@ def test_policy_masks_infinities_and_nan(dtype, vocab):
                   weights, 0.05)
 
 
+@pytest.mark.parametrize("rows,vocab,dtype", [
+    (500, 100003, torch.bfloat16),      # one block per row, registers and ring
+    (420, 170000, torch.float16),       # two of them per row
+    (30, 400000, torch.bfloat16),       # few rows: eight smaller blocks
+    (400, 400000, torch.bfloat16),
+    (6, 600000, torch.float32),         # past the smaller blocks
+    (5, 700000, torch.float32),         # past what a cluster holds
+    (3, 1300000, torch.bfloat16),
+    (40, 14400, torch.bfloat16), (40, 14392, torch.float16),       # around the shortest rows held
+    (40, 32256, torch.bfloat16), (40, 32264, torch.bfloat16), (40, 64520, torch.bfloat16), (40, 64535, torch.float16),
+    (40, 16128, torch.float32), (40, 16132, torch.float32), (40, 23041, torch.float32), (40, 46090, torch.float32),
+    (40, 92163, torch.float32), (3000, 14403, torch.bfloat16), (2000, 8200, torch.float16)])
+@pytest.mark.parametrize("entropy", [0.0, 0.01])
+def test_policy_by_size(rows, vocab, dtype, entropy):
+    """Sizes on both sides of each way a row is held on chip.  Most rows hold no
+    token, as in a padded batch; those that do are checked."""
+    g = torch.Generator().manual_seed(rows + vocab)
+    x = (torch.randn(rows, vocab, device="cuda", generator=torch.Generator("cuda").manual_seed(1)) * 3).to(dtype)
+    alive = torch.randperm(rows, generator=g)[:min(rows, 12)].sort().values.cuda()
+    targets = torch.full((rows,), -3, device="cuda")
+    targets[alive] = torch.randint(0, vocab, (len(alive),), generator=g).cuda()
+    part = x[alive].contiguous()
+    old, ref, adv, _ = _policy_inputs(rows, part, targets[alive], 1.0)
+    every = [torch.full((rows,), NAN, device="cuda") for _ in range(3)]
+    for v, w in zip(every, (old, ref, adv)):
+        v[alive] = w
+    want = O.policy(part, targets[alive], old, adv, ref, None, 1.0, 0.2, 0.2, 0.05, entropy)
+    weights = torch.full((rows,), 1.0 / len(alive), device="cuda")
+    got, grad = policy_loss_and_grad(x, targets, every[0], every[2], ref_logprobs=every[1], weights=weights,
+                                     kl_coef=0.05, entropy_coef=entropy)
+    rest = torch.ones(rows, dtype=torch.bool, device="cuda")
+    rest[alive] = False
+    assert not grad[rest].any() and not got.row_loss[rest].any() and not got.kl[rest].any()
+    picked = type(got)(got.loss, *(None if t is None else t[alive] for t in got[1:]))
+    _check_policy(picked, grad[alive], want, part, targets[alive], old, ref, adv, torch.full_like(old, 1.0 / len(alive)), 0.05)
+
+
 def test_policy_all_rows_padded():
     x = torch.full((5, 333), NAN, device="cuda", dtype=torch.bfloat16)
     t = torch.full((5,), -1, device="cuda")
