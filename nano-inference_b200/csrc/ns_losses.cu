@@ -310,20 +310,36 @@ __device__ __noinline__ Part block_running(const void* base, int64_t vocab, floa
   return warp_join<ENT>(p, scale);
 }
 
-// Adds a vector's 2^t, and 2^t t, to the sums.  t is held above -200, where
-// 2^t is 0, so that 0 * -inf does not arise; a NaN t has made 2^t NaN.
+// Adds a vector's 2^t, and 2^t t, to the sums; of the 2^t the vector's own sum
+// first, so that small values are not lost one by one beside a large sum (they
+// made log-probabilities 8e-8 high on average at V = 151936).  t is held
+// above -200, where 2^t is 0, so that 0 * -inf does not arise; a NaN t has made
+// 2^t NaN.
 template <int DT, bool ENT>
 __device__ __forceinline__ void add_vector(const uint4& q, const ScaledPairs<DT>& scaled, F2& s, F2& u) {
   using D = Elem<DT>;
+  constexpr int P = D::E / 2;
   float x[D::E];
+  F2 e[P];
   D::unpack(q, x);
 #pragma unroll
-  for (int i = 0; i < D::E; i += 2) {
+  for (int i = 0; i < P; ++i) {
     float a, b;
-    split(scaled(f2(x[i], x[i + 1])), a, b);
-    const F2 e = f2(ex2_approx(a), ex2_approx(b));
-    s = add2(s, e);
-    if (ENT) u = fma2(e, f2(fmaxf(a, -200.0f), fmaxf(b, -200.0f)), u);
+    split(scaled(f2(x[2 * i], x[2 * i + 1])), a, b);
+    e[i] = f2(ex2_approx(a), ex2_approx(b));
+    if (ENT) u = fma2(e[i], f2(fmaxf(a, -200.0f), fmaxf(b, -200.0f)), u);
+  }
+  if constexpr (ENT && DT == NS_DTYPE_F32) {      // the products leave no registers for it
+    s = add2(add2(s, e[0]), e[1]);
+  } else if constexpr (ENT) {                     // and here for two at a time
+#pragma unroll
+    for (int i = 0; i < P; i += 2) s = add2(s, add2(e[i], e[i + 1]));
+  } else {
+#pragma unroll
+    for (int n = P / 2; n; n /= 2)
+#pragma unroll
+      for (int i = 0; i < n; ++i) e[i] = add2(e[i], e[i + n]);
+    s = add2(s, e[0]);
   }
 }
 

@@ -521,10 +521,11 @@ def test_two_captured_graphs_replayed_at_once(name):
                 assert torch.equal(u, v)
 
 
-def test_offsets_past_32_bits():
-    """Rows whose elements lie past 2^32 (row stride and rows large): the last
-    rows give what they give alone."""
-    rows, vocab, stride = 9, 1003, 600_000_000
+@pytest.mark.parametrize("vocab", [1003, 1000003])       # two launches, and rows held on chip
+def test_offsets_past_32_bits(vocab):
+    """Rows whose elements lie past 2^32 (9 rows 600 M elements apart), the
+    gradient in place."""
+    rows, stride = 9, 600_000_000
     if torch.cuda.mem_get_info()[0] < 24 << 30:
         pytest.skip("needs 20 GB of device memory")
     buf = torch.empty((rows - 1) * stride + vocab, dtype=torch.bfloat16, device="cuda")
@@ -532,9 +533,10 @@ def test_offsets_past_32_bits():
     x.copy_(_logits(3, rows, vocab, torch.bfloat16))
     targets = _targets(3, rows, vocab)
     old, ref, adv, _ = _policy_inputs(3, x, targets, 1.0)
-    want, want_grad = policy_loss_and_grad(x.contiguous(), targets, old, adv)
-    got, grad = policy_loss_and_grad(x, targets, old, adv, out=x)
-    assert torch.equal(got.logprobs, want.logprobs) and torch.equal(grad, want_grad)
+    want = O.policy(x, targets, old, adv, ref, None, 1.0, 0.2, 0.2, 0.05, 0.01)
+    got, grad = policy_loss_and_grad(x, targets, old, adv, ref_logprobs=ref, kl_coef=0.05, entropy_coef=0.01, out=x)
+    assert grad.data_ptr() == x.data_ptr()
+    _check_policy(got, grad, want, x, targets, old, ref, adv, None, 0.05)
 
 
 def test_backward_twice_and_upstream_gradients():
