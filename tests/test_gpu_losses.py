@@ -55,7 +55,7 @@ def _temperature(kind, rows):
     return kind
 
 
-def _check_logprobs(x, targets, temperature, entropy=True, grads=True, seed=0):
+def _check_logprobs(x, targets, temperature, entropy=True, grads=True, seed=0, extra=0.0):
     ln_p, lp, ent, alive, t = O.rows(x, targets, temperature)
     leaf = x.detach().requires_grad_()
     got = token_logprobs(leaf, targets, temperature=temperature, entropy=entropy)
@@ -78,6 +78,8 @@ def _check_logprobs(x, targets, temperature, entropy=True, grads=True, seed=0):
     aa = torch.where(alive, a.cpu().double(), torch.zeros_like(lp))
     bound = grad_bound(ln_p, lp, t, ent, targets.cpu(), want, aa, torch.zeros_like(lp),
                        torch.where(alive, hh.cpu().double(), torch.zeros_like(lp)), x.dtype)
+    size = aa.abs()[:, None] + hh.cpu().double().abs()[:, None] * (torch.nan_to_num(ln_p, neginf=0.0).abs() + ent[:, None])
+    bound = bound + extra * torch.exp(ln_p) * size / t[:, None]
     assert grad.dtype == x.dtype and grad.shape == x.shape
     close(grad, want, torch.nan_to_num(bound), "grad")
 
@@ -109,6 +111,21 @@ def test_row_counts_cross_the_blocks_per_row(rows):
 def test_temperatures(temperature):
     x = _logits(1, 7, 5003, torch.float32)
     _check_logprobs(x, _targets(1, 7, 5003), temperature)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shift", [-900.0, -600.0, 600.0, 900.0, 40000.0])
+@pytest.mark.parametrize("vocab", [1003, 32000])
+def test_logits_far_from_zero(dtype, shift, vocab):
+    """Distributions do not see a shift of all logits; the kernels' offsets do.
+    16-bit values this far out are coarse, so the rows have few distinct ones."""
+    if dtype == torch.float16 and shift > 30000:
+        shift = 30000.0
+    x = (_logits(9, 6, vocab, torch.float32) + shift).to(dtype)
+    targets = x.float().topk(3, dim=1).indices[:, 1].contiguous()
+    # 16-bit gradients: the offset c s + log2 S, below 1024 + 60 in size, is rounded to 2^-14
+    _check_logprobs(x, targets, 1.0, extra=0.0 if dtype == torch.float32 else math.log(2) * 2.0 ** -13)
+    _check_logprobs(x, targets, 2.0, entropy=False, extra=0.0 if dtype == torch.float32 else math.log(2) * 2.0 ** -13)
 
 
 def _odd_rows(dtype, vocab):
