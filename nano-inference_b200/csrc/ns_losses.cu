@@ -348,6 +348,13 @@ __device__ __forceinline__ void add_vector(const uint4& q, const ScaledPairs<DT>
   }
 }
 
+// A call's kernels follow one another closely: each lets the next one start (its
+// blocks take places as they fall free), and that one waits until every block
+// before it has ended and what they wrote is there; 1 to 2 us a call.  A third
+// kernel waits for the second, which has itself waited for the first.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 struct RowShared {
   Part warp[kWarps];
   Part block[kMaxCluster];
@@ -671,6 +678,7 @@ __device__ __forceinline__ void write_row(const LossArgs& a, int64_t row, const 
 // One cluster of blocks per row.
 template <int DT, bool ENT, int OP>
 __global__ void __launch_bounds__(kThreads) forward_kernel(const LossArgs a) {
+  if (OP != kLogprob) let_next_start();
   using D = Elem<DT>;
   using T = typename D::T;
   __shared__ RowShared sh;
@@ -697,6 +705,7 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const LossArgs a) {
 // the work.  8192 x 2000 bf16: 33 us by blocks.
 template <int DT, bool ENT, int OP>
 __global__ void __launch_bounds__(kThreads) forward_rows_kernel(const LossArgs a) {
+  if (OP != kLogprob) let_next_start();
   using D = Elem<DT>;
   using T = typename D::T;
   const int64_t row = int64_t(blockIdx.x) * kWarps + (threadIdx.x >> 5);
@@ -737,6 +746,7 @@ __device__ __forceinline__ double block_sum(double v, double* shared) {
 // The policy loss: the rows' losses by their weights, in 64 bits and in one order.
 __global__ void __launch_bounds__(1024) policy_sum_kernel(const LossArgs a, float* loss) {
   __shared__ double shared[32];
+  wait_for_previous();
   double v = 0.0;
   for (int64_t i = threadIdx.x; i < a.rows; i += 1024) {
     const double w = a.weights ? double(a.weights[i]) : 1.0 / double(a.rows);
@@ -754,6 +764,8 @@ __global__ void __launch_bounds__(1024) pair_kernel(const LossArgs a, float beta
   __shared__ double sums[32], shared[32];
   __shared__ int counts[32];
   __shared__ float coef[32];
+  let_next_start();
+  wait_for_previous();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int each = 1;                           // warps of a sequence
   while (each < 16 && 2 * a.pairs * each * 2 <= 32) each *= 2;
@@ -863,6 +875,8 @@ __device__ __forceinline__ void write_chunk(const GradRow& g, const void* base, 
 // from the last row on, whose logits L2 still holds from the sums.
 template <int DT, bool ENT>
 __global__ void __launch_bounds__(kGradThreads) grad_kernel(const LossArgs a, int chunks) {
+  let_next_start();
+  wait_for_previous();
   using D = Elem<DT>;
   using T = typename D::T;
   const int64_t row = a.rows - 1 - blockIdx.x / chunks;
@@ -1038,6 +1052,7 @@ __device__ __forceinline__ Share row_share(const void* base, int vocab, int rank
 template <int DT, bool ENT, int SHAPE>
 __global__ void __launch_bounds__(HeldShape<SHAPE>::kThreads, HeldShape<SHAPE>::kBlocks)
     policy_kernel(const __grid_constant__ LossArgs a) {
+  let_next_start();
   using D = Elem<DT>;
   using T = typename D::T;
   using H = HeldShape<SHAPE>;
@@ -1341,20 +1356,29 @@ int sm_count(int* out) {
   return NS_OK;
 }
 
+// `blocks`: of a cluster; one of 1 is not the same as none (policy_kernel took 3 us
+// longer at 2048 x 32000 without).  `follows`: the kernel waits for the one before it by
+// wait_for_previous, and may be started before that one has ended.
 template <typename... Args>
-int launch_clusters(void (*kernel)(Args...), int64_t grid, int threads, int blocks, size_t smem, cudaStream_t stream,
-                    Args... args) {
+int launch(void (*kernel)(Args...), int64_t grid, int threads, int blocks, size_t smem, bool follows, cudaStream_t stream,
+           Args... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(grid));
   cfg.blockDim = dim3(unsigned(threads));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = unsigned(blocks);
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  if (follows) {
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 1;
+  } else {
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = unsigned(blocks);
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.numAttrs = 1;
+  }
   return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? NS_OK : NS_ERR_CUDA;
 }
 
@@ -1366,13 +1390,12 @@ int launch_forward(const LossArgs& a, cudaStream_t stream) {
   // a warp per row while rows are short and many: 4096 x 8000 bf16 15 us against 21, 1024 x 4000 6 against 8;
   // at 2048 x 16000 and for 300 rows the two are even
   if (vectors <= 1024 && a.rows >= 2 * sms) {
-    forward_rows_kernel<DT, ENT, OP><<<unsigned((a.rows + kWarps - 1) / kWarps), kThreads, 0, stream>>>(a);
-    return cudaGetLastError() == cudaSuccess ? NS_OK : NS_ERR_CUDA;
+    return launch(forward_rows_kernel<DT, ENT, OP>, (a.rows + kWarps - 1) / kWarps, kThreads, 1, 0, false, stream, a);
   }
   // blocks per row: enough to give every SM two, each thread at least one vector
   int blocks = 1;
   while (blocks < kMaxCluster && a.rows * blocks < 2 * sms && vectors >= int64_t(2) * blocks * kThreads) blocks *= 2;
-  return launch_clusters(forward_kernel<DT, ENT, OP>, a.rows * blocks, kThreads, blocks, 0, stream, a);
+  return launch(forward_kernel<DT, ENT, OP>, a.rows * blocks, kThreads, blocks, 0, false, stream, a);
 }
 
 template <int OP, int DT>
@@ -1431,7 +1454,7 @@ int launch_policy(const LossArgs& a, int blocks, cudaStream_t stream) {
     clusters = known[dev][blocks];
   }
   const int64_t grid = std::min<int64_t>(a.rows, clusters) * blocks;
-  return launch_clusters(policy_kernel<DT, ENT, SHAPE>, grid, H::kThreads, blocks, H::kSmem, stream, a);
+  return launch(policy_kernel<DT, ENT, SHAPE>, grid, H::kThreads, blocks, H::kSmem, false, stream, a);
 }
 
 template <int DT, int SHAPE>
@@ -1449,9 +1472,9 @@ int launch_shape(const LossArgs& a, int blocks, cudaStream_t stream) {
 //    333 x 151936 bf16   55 / 49 / -  / 62       600 x 151936 fp32 134 / 123 / - / 170
 // Short rows spend their time in joins, which more blocks of an SM hide.
 // 16-bit rows are bound by their exponentials and want whole SMs without a
-// cluster's join; fp32 rows and few rows want their columns spread.  Below
-// 16 MB of logits two launches over all SMs win (16 x 32000 bf16 9.4 against
-// 11.0, 200 x 32000 12.9 against 13.6; 64 x 151936 15.5 against 13.8).
+// cluster's join; fp32 rows and few rows want their columns spread.  A handful
+// of rows is even: 16 x 32000 bf16 takes 11.0 against 9.4 in a graph, 12.3
+// against 14.4 launch by launch.
 template <int DT>
 int policy_held(const LossArgs& a, cudaStream_t stream, bool* held) {
   int sms = 0;
@@ -1459,7 +1482,7 @@ int policy_held(const LossArgs& a, cudaStream_t stream, bool* held) {
   const int64_t vectors = a.vocab / Elem<DT>::E;
   const int small = held_blocks<kSmall>(vectors), medium = held_blocks<kMedium>(vectors), large = held_blocks<kLarge>(vectors);
   *held = true;
-  if (vectors >= 1800 && a.rows * vectors >= (int64_t(16) << 20) / 16) {
+  if (vectors >= 1800) {
     if (small == 1 || (small == 2 && DT != NS_DTYPE_F32)) return launch_shape<DT, kSmall>(a, small, stream);
     if (medium && (DT == NS_DTYPE_F32 || 2 * a.rows < 5 * sms)) return launch_shape<DT, kMedium>(a, medium, stream);
     if (large) return launch_shape<DT, kLarge>(a, large, stream);
@@ -1477,23 +1500,20 @@ int policy_held(const LossArgs& a, int dtype, cudaStream_t stream, bool* held) {
 }
 
 template <int DT>
-int launch_grad(const LossArgs& a, cudaStream_t stream) {
+int launch_grad(const LossArgs& a, bool follows, cudaStream_t stream) {
   const int64_t per = int64_t(kGradThreads) * kGradVecs * Elem<DT>::E;    // shares differ by one vector at most
   const int chunks = int((a.vocab + per - 1) / per);
   const int64_t blocks = a.rows * chunks;
   if (blocks > 0x7FFFFFFF) return NS_ERR_INVALID_ARGUMENT;
-  if (a.grad_entropy)
-    grad_kernel<DT, true><<<unsigned(blocks), kGradThreads, 0, stream>>>(a, chunks);
-  else
-    grad_kernel<DT, false><<<unsigned(blocks), kGradThreads, 0, stream>>>(a, chunks);
-  return cudaGetLastError() == cudaSuccess ? NS_OK : NS_ERR_CUDA;
+  return launch(a.grad_entropy ? grad_kernel<DT, true> : grad_kernel<DT, false>, blocks, kGradThreads, 1, 0, follows,
+                stream, a, chunks);
 }
 
-int gradient(const LossArgs& a, int dtype, cudaStream_t stream) {
+int gradient(const LossArgs& a, int dtype, bool follows, cudaStream_t stream) {
   switch (dtype) {
-    case NS_DTYPE_F32: return launch_grad<NS_DTYPE_F32>(a, stream);
-    case NS_DTYPE_BF16: return launch_grad<NS_DTYPE_BF16>(a, stream);
-    default: return launch_grad<NS_DTYPE_F16>(a, stream);
+    case NS_DTYPE_F32: return launch_grad<NS_DTYPE_F32>(a, follows, stream);
+    case NS_DTYPE_BF16: return launch_grad<NS_DTYPE_BF16>(a, follows, stream);
+    default: return launch_grad<NS_DTYPE_F16>(a, follows, stream);
   }
 }
 
@@ -1558,7 +1578,7 @@ int ns_token_logprobs_grad(const void* logits, int dtype, int64_t rows, int64_t 
   a.grad_entropy = grad_entropy;
   a.grad_logits = grad_logits;
   a.grad_stride = grad_stride;
-  return ns::gradient(a, dtype, reinterpret_cast<cudaStream_t>(stream));
+  return ns::gradient(a, dtype, false, reinterpret_cast<cudaStream_t>(stream));
 }
 
 int ns_policy_loss(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t row_stride,
@@ -1604,10 +1624,9 @@ int ns_policy_loss(const void* logits, int dtype, int64_t rows, int64_t vocab, i
   if (!held) {
     if (const int rc = ns::forward<ns::kPolicy>(a, dtype, s)) return rc;
     if (grad_logits)
-      if (const int rc = ns::gradient(a, dtype, s)) return rc;
+      if (const int rc = ns::gradient(a, dtype, true, s)) return rc;
   }
-  ns::policy_sum_kernel<<<1, 1024, 0, s>>>(a, loss);
-  return cudaGetLastError() == cudaSuccess ? NS_OK : NS_ERR_CUDA;
+  return ns::launch(ns::policy_sum_kernel, 1, 1024, 1, 0, true, s, a, loss);
 }
 
 int ns_preference_loss(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t row_stride,
@@ -1636,13 +1655,14 @@ int ns_preference_loss(const void* logits, int dtype, int64_t rows, int64_t voca
   a.pairs = pairs;
   if (rows > 0)
     if (const int rc = ns::forward<ns::kPreference>(a, dtype, s)) return rc;
-  ns::pair_kernel<<<1, 1024, 0, s>>>(a, beta, label_smoothing, average, loss, pair_loss, rewards);
-  if (cudaGetLastError() != cudaSuccess) return NS_ERR_CUDA;
+  if (const int rc = ns::launch(ns::pair_kernel, 1, 1024, 1, 0, rows > 0, s, a, beta, label_smoothing, average, loss,
+                                pair_loss, rewards))
+    return rc;
   if (!grad_logits || rows == 0) return NS_OK;
   a.grad_logprobs = row_grad;
   a.grad_logits = grad_logits;
   a.grad_stride = grad_stride;
-  return ns::gradient(a, dtype, s);
+  return ns::gradient(a, dtype, true, s);
 }
 
 }  // extern "C"
