@@ -1387,9 +1387,10 @@ int launch_forward(const LossArgs& a, cudaStream_t stream) {
   int sms = 0;
   if (const int rc = sm_count(&sms)) return rc;
   const int64_t vectors = a.vocab / Elem<DT>::E;
-  // a warp per row while rows are short and many: 4096 x 8000 bf16 15 us against 21, 1024 x 4000 6 against 8;
-  // at 2048 x 16000 and for 300 rows the two are even
-  if (vectors <= 1024 && a.rows >= 2 * sms) {
+  // a warp per row while rows are short and many: 4096 x 8000 bf16 15 us against 21, 1024 x 4000 6 against 8,
+  // 4096 x 16000 27 against 32, 2048 x 9000 9 against 12; even at 300 rows of 1000 vectors, at 1000 x 9000 and
+  // at 2048 x 16000 (there, with entropy, 17 against 15), and worse at 2048 x 32000, 33 against 28
+  if (vectors <= 1024 ? a.rows >= 2 * sms : vectors <= 2560 && 2 * a.rows >= 3 * vectors) {
     return launch(forward_rows_kernel<DT, ENT, OP>, (a.rows + kWarps - 1) / kWarps, kThreads, 1, 0, false, stream, a);
   }
   // blocks per row: enough to give every SM two, each thread at least one vector

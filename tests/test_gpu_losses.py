@@ -107,6 +107,15 @@ def test_row_counts_cross_the_blocks_per_row(rows):
     _check_logprobs(x, _targets(rows, rows, 20011, 0.1), _temperature("rows", rows))
 
 
+@pytest.mark.parametrize("rows,vocab,dtype", [
+    (295, 8193, torch.bfloat16), (296, 8193, torch.bfloat16),       # a warp per row from 296 rows on 148 SMs
+    (1544, 4121, torch.float32), (1545, 4121, torch.float32),       # from 1545 rows of 1030 vectors
+    (1600, 8209, torch.float16)])
+def test_row_counts_cross_a_warp_per_row(rows, vocab, dtype):
+    x = _logits(rows, rows, vocab, dtype)
+    _check_logprobs(x, _targets(rows, rows, vocab, 0.1), _temperature("rows", rows))
+
+
 @pytest.mark.parametrize("temperature", [0.0, 0.05, 0.7, 1.0, 3.0, 1e30])
 def test_temperatures(temperature):
     x = _logits(1, 7, 5003, torch.float32)
