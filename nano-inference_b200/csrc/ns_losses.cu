@@ -46,9 +46,12 @@ constexpr int kMaxCluster = 8;
 constexpr int kBatch = 2;          // 16-byte loads that a thread of a forward issues ahead of its sums; 4 and 8 were no faster
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr double kLn2 = 0.6931471805599453;
-// Mean relative error of ex2.approx.ftz.f32, measured over 4 M arguments in [-30, 0]: -5.07e-8, between -3.4e-8 and
-// -6.1e-8 in every sixteenth of an octave (largest 1.4e-7).
-constexpr double kEx2Mean = 5.07e-8;
+// Mean relative error of ex2.approx.ftz.f32, measured over 4 M arguments an interval: -5.0e-8 from -30 to -1, -2.2e-8
+// from -1 to 0, 0.6e-8 from 0 to 1, 3.3e-8 from 1 to 32.  The target of a draw has half of the row's mass above it on
+// average, so S is low by half the sum of the outer two; a row whose mass is all on one side is 4.2e-8 away from that.
+// Log-probabilities of drawn targets are then off by 0.2e-8 on average (600 rows of 151936), where the error of the
+// negative arguments alone gave -3.3e-8.
+constexpr double kEx2Mean = 0.85e-8;
 
 enum Op { kLogprob = 0, kPolicy = 1, kPreference = 2 };
 
@@ -484,7 +487,7 @@ __device__ __forceinline__ RowResult finish(const Part& p, float x_target, float
   const double ln_s = p.s < INFINITY && p.s > 0.0f ? double(ex - 1) * kLn2 + double(logf(mant)) : double(NAN);
   // how far the sums' offset lies from m s
   const double moved = DT != NS_DTYPE_F32 && near ? double(__fmul_rn(p.m, scale)) - double(p.m) * double(scale) : 0.0;
-  // the exponentials are kEx2Mean low on average, but for the target's own, 2^0 = 1, which is p of S.  A
+  // the exponentials are kEx2Mean low on average, all but for the target's own, 2^0 = 1, which is p of S.  A
   // sequence's reward adds such errors up, a gradient's p divides them out
   const double ln_all = ln_s + (near ? kEx2Mean * (1.0 - double(1.0f / p.s)) : 0.0);
   RowResult r;
