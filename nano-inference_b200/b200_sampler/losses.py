@@ -132,14 +132,18 @@ def _new(logits: torch.Tensor, *shape: int) -> torch.Tensor:
 
 def _parts(logits: torch.Tensor, *sizes: int):
     """fp32 vectors of these sizes from one allocation."""
-    return torch.empty(sum(sizes), dtype=torch.float32, device=logits.device).split(sizes)
+    return torch.empty(sum(sizes), dtype=torch.float32, device=logits.device).split_with_sizes(sizes)
+
+
+def _like(logits: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(logits, memory_format=torch.contiguous_format)
 
 
 def _grad_out(logits: torch.Tensor, given: torch.Tensor, out: Optional[torch.Tensor]) -> torch.Tensor:
     """The gradient's tensor: a new one, or the caller's after its checks.
     ``given`` is the caller's logits, ``logits`` what the kernels read."""
     if out is None:
-        return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        return _like(logits)
     if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
         raise ValueError("out must have the logits' shape, dtype and device")
     if out.stride(1) != 1 or (out.shape[0] > 1 and out.stride(0) < out.shape[1]):
@@ -159,7 +163,8 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a0 < b1 and b0 < a1
 
 
-def _gradient(logits, targets, temperature, temperature_all, stats, entropy, a, h, out):
+def _gradient(logits, targets, temperature, temperature_all, stats, entropy, a, h):
+    out = _like(logits)
     _call("ns_token_logprobs_grad", logits.device, *_head(logits, targets, temperature, temperature_all),
           stats.data_ptr(), _ptr(entropy), _ptr(a), _ptr(h), out.data_ptr(), _stride(out))
     return out
@@ -204,8 +209,7 @@ class _TokenLogprobs(_Once):
         h = None if h is None else h.contiguous()
         if a is None and h is None:
             return None, None, None, None, None
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        _gradient(logits, targets, temperature, ctx.temperature_all, stats, ent, a, h, out)
+        out = _gradient(logits, targets, temperature, ctx.temperature_all, stats, ent, a, h)
         return out, None, None, None, None
 
 
@@ -241,36 +245,37 @@ def _policy(logits, targets, old_logprobs, advantages, ref_logprobs, weights, te
 
 
 def _policy_forward(logits, targets, temperature, t_all, vectors, coefs, grad):
-    """(PolicyLoss, stats, row_grad [2, rows]); writes dloss/dlogits to ``grad`` when there is one."""
+    """(PolicyLoss, the backward pass's numbers: stats [rows, 2], coefficients [2, rows]); writes
+    dloss/dlogits to ``grad`` when there is one."""
     n = logits.shape[0]
     has_entropy, has_kl = coefs[3] != 0.0, vectors[1] is not None
     loss = _new(logits)              # by itself: a part of several may not be changed in place
-    row_loss, logprobs, stats, row_grad, *rest = _parts(logits, n, n, 2 * n, 2 * n, *[n] * (has_entropy + has_kl))
-    row_grad = row_grad.view(2, n)
+    row_loss, logprobs, back, *rest = _parts(logits, n, n, 4 * n, *[n] * (has_entropy + has_kl))
+    stats = back.data_ptr()
     entropy = rest[0] if has_entropy else None
     kl = rest[-1] if has_kl else None
     _call("ns_policy_loss", logits.device, *_head(logits, targets, temperature, t_all), *map(_ptr, vectors),
           *coefs, loss.data_ptr(), row_loss.data_ptr(), logprobs.data_ptr(), _ptr(entropy), _ptr(kl),
-          stats.data_ptr(), row_grad.data_ptr(), _ptr(grad), 0 if grad is None else _stride(grad))
-    return PolicyLoss(loss, row_loss, logprobs, entropy, kl), stats, row_grad
+          stats, stats + 8 * n, _ptr(grad), 0 if grad is None else _stride(grad))
+    return PolicyLoss(loss, row_loss, logprobs, entropy, kl), back
 
 
 class _PolicyLoss(_Once):
     @staticmethod
     def forward(ctx, logits, targets, temperature, t_all, vectors, coefs):
-        got, stats, row_grad = _policy_forward(logits, targets, temperature, t_all, vectors, coefs, None)
+        got, back = _policy_forward(logits, targets, temperature, t_all, vectors, coefs, None)
         ctx.t_all = t_all
-        ctx.save_for_backward(logits, targets, temperature, stats, got.entropy, row_grad)
+        ctx.save_for_backward(logits, targets, temperature, back, got.entropy)
         ctx.mark_non_differentiable(*(t for t in got[1:] if t is not None))
         return tuple(got)
 
     @staticmethod
     def gradient(ctx, g, *_):
-        logits, targets, temperature, stats, entropy, row_grad = ctx.saved_tensors
-        row_grad = row_grad * g
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        _gradient(logits, targets, temperature, ctx.t_all, stats, entropy, row_grad[0],
-                  None if entropy is None else row_grad[1], out)
+        logits, targets, temperature, back, entropy = ctx.saved_tensors
+        n = logits.shape[0]
+        coefs = back[2 * n:] * g
+        out = _gradient(logits, targets, temperature, ctx.t_all, back, entropy, coefs,
+                        None if entropy is None else coefs[n:])
         return out, None, None, None, None, None
 
 
@@ -328,28 +333,28 @@ def _preference(logits, targets, seq_offsets, ref_logprobs, beta, label_smoothin
 def _preference_forward(logits, targets, temperature, t_all, offsets, ref, coefs, grad):
     n, pairs = logits.shape[0], offsets.shape[0] // 2
     loss = _new(logits)
-    pair_loss, rewards, logprobs, stats, row_grad = _parts(logits, pairs, 2 * pairs, n, 2 * n, n)
+    pair_loss, rewards, logprobs, back = _parts(logits, pairs, 2 * pairs, n, 3 * n)
     rewards = rewards.view(pairs, 2)
+    stats = back.data_ptr()
     _call("ns_preference_loss", logits.device, *_head(logits, targets, temperature, t_all), offsets.data_ptr(), pairs,
           _ptr(ref), *coefs, loss.data_ptr(), pair_loss.data_ptr(), rewards.data_ptr(), logprobs.data_ptr(),
-          stats.data_ptr(), row_grad.data_ptr(), _ptr(grad), 0 if grad is None else _stride(grad))
-    return PreferenceLoss(loss, pair_loss, rewards, logprobs), stats, row_grad
+          stats, stats + 8 * n, _ptr(grad), 0 if grad is None else _stride(grad))
+    return PreferenceLoss(loss, pair_loss, rewards, logprobs), back
 
 
 class _PreferenceLoss(_Once):
     @staticmethod
     def forward(ctx, logits, targets, temperature, t_all, offsets, ref, coefs):
-        got, stats, row_grad = _preference_forward(logits, targets, temperature, t_all, offsets, ref, coefs, None)
+        got, back = _preference_forward(logits, targets, temperature, t_all, offsets, ref, coefs, None)
         ctx.t_all = t_all
-        ctx.save_for_backward(logits, targets, temperature, stats, row_grad)
+        ctx.save_for_backward(logits, targets, temperature, back)
         ctx.mark_non_differentiable(*got[1:])
         return tuple(got)
 
     @staticmethod
     def gradient(ctx, g, *_):
-        logits, targets, temperature, stats, row_grad = ctx.saved_tensors
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        _gradient(logits, targets, temperature, ctx.t_all, stats, None, row_grad * g, None, out)
+        logits, targets, temperature, back = ctx.saved_tensors
+        out = _gradient(logits, targets, temperature, ctx.t_all, back, None, back[2 * logits.shape[0]:] * g, None)
         return out, None, None, None, None, None, None
 
 
