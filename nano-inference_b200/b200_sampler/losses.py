@@ -245,15 +245,16 @@ def _policy(logits, targets, old_logprobs, advantages, ref_logprobs, weights, te
 
 
 def _policy_forward(logits, targets, temperature, t_all, vectors, coefs, grad):
-    """(PolicyLoss, the backward pass's numbers: stats [rows, 2], coefficients [2, rows]); writes
-    dloss/dlogits to ``grad`` when there is one."""
+    """(PolicyLoss, the backward pass's numbers: stats [rows, 2], coefficients [2, rows], entropies);
+    writes dloss/dlogits to ``grad`` when there is one."""
     n = logits.shape[0]
     has_entropy, has_kl = coefs[3] != 0.0, vectors[1] is not None
     loss = _new(logits)              # by itself: a part of several may not be changed in place
-    row_loss, logprobs, back, *rest = _parts(logits, n, n, 4 * n, *[n] * (has_entropy + has_kl))
+    row_loss, logprobs, *rest = _parts(logits, n, n, *[n] * has_kl)
+    kl = rest[0] if has_kl else None
+    back = _new(logits, (4 + has_entropy) * n)      # by itself: the caller may change the others before the backward pass
+    entropy = back[4 * n:] if has_entropy else None
     stats = back.data_ptr()
-    entropy = rest[0] if has_entropy else None
-    kl = rest[-1] if has_kl else None
     _call("ns_policy_loss", logits.device, *_head(logits, targets, temperature, t_all), *map(_ptr, vectors),
           *coefs, loss.data_ptr(), row_loss.data_ptr(), logprobs.data_ptr(), _ptr(entropy), _ptr(kl),
           stats, stats + 8 * n, _ptr(grad), 0 if grad is None else _stride(grad))
@@ -263,19 +264,22 @@ def _policy_forward(logits, targets, temperature, t_all, vectors, coefs, grad):
 class _PolicyLoss(_Once):
     @staticmethod
     def forward(ctx, logits, targets, temperature, t_all, vectors, coefs):
+        ctx.set_materialize_grads(False)
         got, back = _policy_forward(logits, targets, temperature, t_all, vectors, coefs, None)
-        ctx.t_all = t_all
-        ctx.save_for_backward(logits, targets, temperature, back, got.entropy)
+        ctx.t_all, ctx.has_entropy = t_all, got.entropy is not None
+        ctx.save_for_backward(logits, targets, temperature, back)
         ctx.mark_non_differentiable(*(t for t in got[1:] if t is not None))
         return tuple(got)
 
     @staticmethod
     def gradient(ctx, g, *_):
-        logits, targets, temperature, back, entropy = ctx.saved_tensors
+        if g is None:
+            return None, None, None, None, None, None
+        logits, targets, temperature, back = ctx.saved_tensors
         n = logits.shape[0]
-        coefs = back[2 * n:] * g
-        out = _gradient(logits, targets, temperature, ctx.t_all, back, entropy, coefs,
-                        None if entropy is None else coefs[n:])
+        coefs = back[2 * n:4 * n] * g
+        entropy, h = (back[4 * n:], coefs[n:]) if ctx.has_entropy else (None, None)
+        out = _gradient(logits, targets, temperature, ctx.t_all, back, entropy, coefs, h)
         return out, None, None, None, None, None
 
 
@@ -333,8 +337,9 @@ def _preference(logits, targets, seq_offsets, ref_logprobs, beta, label_smoothin
 def _preference_forward(logits, targets, temperature, t_all, offsets, ref, coefs, grad):
     n, pairs = logits.shape[0], offsets.shape[0] // 2
     loss = _new(logits)
-    pair_loss, rewards, logprobs, back = _parts(logits, pairs, 2 * pairs, n, 3 * n)
+    pair_loss, rewards, logprobs = _parts(logits, pairs, 2 * pairs, n)
     rewards = rewards.view(pairs, 2)
+    back = _new(logits, 3 * n)
     stats = back.data_ptr()
     _call("ns_preference_loss", logits.device, *_head(logits, targets, temperature, t_all), offsets.data_ptr(), pairs,
           _ptr(ref), *coefs, loss.data_ptr(), pair_loss.data_ptr(), rewards.data_ptr(), logprobs.data_ptr(),
@@ -345,6 +350,7 @@ def _preference_forward(logits, targets, temperature, t_all, offsets, ref, coefs
 class _PreferenceLoss(_Once):
     @staticmethod
     def forward(ctx, logits, targets, temperature, t_all, offsets, ref, coefs):
+        ctx.set_materialize_grads(False)
         got, back = _preference_forward(logits, targets, temperature, t_all, offsets, ref, coefs, None)
         ctx.t_all = t_all
         ctx.save_for_backward(logits, targets, temperature, back)
@@ -353,6 +359,8 @@ class _PreferenceLoss(_Once):
 
     @staticmethod
     def gradient(ctx, g, *_):
+        if g is None:
+            return None, None, None, None, None, None, None
         logits, targets, temperature, back = ctx.saved_tensors
         out = _gradient(logits, targets, temperature, ctx.t_all, back, None, back[2 * logits.shape[0]:] * g, None)
         return out, None, None, None, None, None, None

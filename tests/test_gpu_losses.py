@@ -595,6 +595,48 @@ def test_the_loss_may_be_changed_in_place():
         assert torch.equal(half.grad * 2, leaf.grad)
 
 
+def test_the_other_results_may_be_changed_before_the_backward_pass():
+    x, targets, old, ref, adv, _, offs = _case(torch.float32, vocab=100)
+    for f, names in ((lambda z: policy_loss(z, targets, old, adv, ref_logprobs=ref, kl_coef=0.1, entropy_coef=0.02),
+                      ("row_loss", "logprobs", "kl")),
+                     (lambda z: preference_loss(z, targets, offs), ("pair_loss", "rewards", "logprobs"))):
+        leaf, again = x.clone().requires_grad_(), x.clone().requires_grad_()
+        f(leaf).loss.backward()
+        got = f(again)
+        for name in names:
+            getattr(got, name).mul_(3.0)
+        got.loss.backward()
+        assert torch.equal(again.grad, leaf.grad)
+
+
+def test_first_calls_captured():
+    """The first call of a process is captured, and a replay gives what an eager call gives."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch
+from b200_sampler import policy_loss_and_grad, preference_loss_and_grad, token_logprobs
+g = torch.Generator("cuda").manual_seed(1)
+x = torch.randn(40, 32000, device="cuda", generator=g).bfloat16()
+t = torch.randint(0, 32000, (40,), device="cuda", generator=g)
+f = torch.randn(40, device="cuda", generator=g)
+offs = torch.tensor([0, 10, 30], device="cuda")
+def run():
+    (a, ga), (b, gb) = policy_loss_and_grad(x, t, f, f), preference_loss_and_grad(x, t, offs)
+    return [token_logprobs(x, t), a.loss, a.logprobs, ga, b.loss, b.rewards, gb]
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = run()
+graph.replay()
+for u, v in zip(got, run()):
+    assert torch.equal(u, v)
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
+                       env={**os.environ, "PYTHONPATH": os.pathsep.join(sys.path)})
+    assert r.returncode == 0, r.stderr
+
+
 def test_changed_logits_stop_the_backward_pass():
     x, targets, old, _, adv, _, _ = _case(torch.float32, vocab=100)
     leaf = x.clone().requires_grad_()
