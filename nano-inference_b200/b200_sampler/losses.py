@@ -31,7 +31,6 @@ import math
 from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -181,16 +180,30 @@ def _logprobs_forward(logits, targets, temperature, temperature_all, entropy, st
     return logprobs, ent, st
 
 
+class _Last(torch.autograd.Function):
+    """Its argument, whose derivative is refused."""
+
+    @staticmethod
+    def forward(ctx, grad):
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, _):
+        raise RuntimeError("token_logprobs, policy_loss and preference_loss are differentiable once: "
+                           "their gradients have no derivatives")
+
+
 class _Once(torch.autograd.Function):
-    """A function whose ``gradient`` is not differentiable again.  Its wrapper,
-    which says so, costs 10 us and is needed only when a graph of the backward
-    pass is asked for."""
+    """A function whose ``gradient`` is not differentiable again, and says so
+    when a graph of the backward pass is asked for."""
 
     @classmethod
     def backward(cls, ctx, *grads):
-        if torch.is_grad_enabled():
-            return once_differentiable(cls.gradient)(ctx, *grads)
-        return cls.gradient(ctx, *grads)
+        if not torch.is_grad_enabled():
+            return cls.gradient(ctx, *grads)
+        with torch.no_grad():
+            out, *rest = cls.gradient(ctx, *grads)
+        return (out if out is None else _Last.apply(out.requires_grad_()), *rest)
 
 
 class _TokenLogprobs(_Once):

@@ -609,6 +609,17 @@ def test_the_other_results_may_be_changed_before_the_backward_pass():
         assert torch.equal(again.grad, leaf.grad)
 
 
+def test_second_derivatives_are_refused():
+    """Also where a gradient is one term of what is differentiated: it is no constant."""
+    x, targets, old, _, adv, _, offs = _case(torch.float32, vocab=100)
+    for f in (lambda z: policy_loss(z, targets, old, adv).loss, lambda z: preference_loss(z, targets, offs).loss,
+              lambda z: token_logprobs(z, targets).sum(), lambda z: token_logprobs(z, targets).square().sum()):
+        leaf = x.clone().requires_grad_()
+        (grad,) = torch.autograd.grad(f(leaf), [leaf], create_graph=True)
+        with pytest.raises(RuntimeError, match="once"):
+            (grad.square().sum() + leaf.sum()).backward()
+
+
 def test_first_calls_captured():
     """The first call of a process is captured, and a replay gives what an eager call gives."""
     import os
