@@ -896,8 +896,8 @@ __global__ void __launch_bounds__(kGradThreads) grad_kernel(const LossArgs a, in
     double inv_t;
     row_scale(a, row, scale, inv_t);
     // every thread reads the target's logit before it writes; in place, the one that uses it is its writer
-    g = grad_row<DT, ENT>(a.stats[2 * row], a.stats[2 * row + 1], scale, inv_t, ga, gh, ENT ? a.entropy[row] : 0.0f, target,
-                      target < a.vocab ? D::load(x + target) : NAN);
+    g = grad_row<DT, ENT>(a.stats[2 * row], a.stats[2 * row + 1], scale, inv_t, ga, gh, ENT ? a.entropy[row] : 0.0f,
+                          target, target < a.vocab ? D::load(x + target) : NAN);
   }
   write_chunk<DT, ENT>(g, x, out, a.vocab, chunk, chunks);
 }
