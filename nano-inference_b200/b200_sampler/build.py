@@ -5,8 +5,8 @@
 nvcc cross-compiles for sm_100a only; no GPU is needed to build.  The library
 is a plain shared object with a C ABI (``include/ns_sampler.h``,
 ``include/ns_losses.h``); it links the CUDA runtime statically and uses no
-torch headers.  Every source has its own object under ``build/``, so a change
-to one compiles that one alone.
+torch headers.  Every source has its own object under ``build/``: a change
+to one compiles that one alone, a change to a header or to this file all of them.
 """
 from __future__ import annotations
 
@@ -77,14 +77,14 @@ def _headers():
     return glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(INCLUDE, "*.h"))
 
 
-def _included(src: str):
-    """The headers that a source names."""
-    text = open(src).read()
-    return [h for h in _headers() if os.path.basename(h) in text]
+def _common():
+    """What every object depends on beside its source: all headers, since one
+    may name another, and the flags, which stand in this file."""
+    return [*_headers(), __file__]
 
 
 def _deps():
-    return sources() + _headers()
+    return sources() + _common()
 
 
 def needs_build() -> bool:
@@ -107,7 +107,7 @@ def _run(cmd, verbose: bool = False) -> None:
 def _compile(src: str, force: bool, verbose: bool) -> str:
     obj = os.path.join(OBJ_DIR, os.path.basename(src) + ".o")
     if not force and os.path.exists(obj) and all(os.path.getmtime(obj) >= os.path.getmtime(p)
-                                                 for p in [src, *_included(src)]):
+                                                 for p in [src, *_common()]):
         return obj
     cmd = [nvcc_path(), *NVCC_FLAGS, "-I", INCLUDE, "-I", CSRC, "-c", "-o", obj + ".tmp", src]
     if verbose:
