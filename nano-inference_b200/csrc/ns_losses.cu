@@ -487,9 +487,10 @@ __device__ __forceinline__ RowResult finish(const Part& p, float x_target, float
   const double ln_s = p.s < INFINITY && p.s > 0.0f ? double(ex - 1) * kLn2 + double(logf(mant)) : double(NAN);
   // how far the sums' offset lies from m s
   const double moved = DT != NS_DTYPE_F32 && near ? double(__fmul_rn(p.m, scale)) - double(p.m) * double(scale) : 0.0;
-  // the exponentials are kEx2Mean low on average, all but for the target's own, 2^0 = 1, which is p of S.  A
-  // sequence's reward adds such errors up, a gradient's p divides them out
-  const double ln_all = ln_s + (near ? kEx2Mean * (1.0 - double(1.0f / p.s)) : 0.0);
+  // the exponentials are kEx2Mean low on average, all but for the target's own, 2^0 = 1, which is 1 / S of S as long
+  // as the sums' offset is the target's logit; around 0 the target has no such part, and S may be as small as 2^-60.
+  // A sequence's reward adds such errors up, a gradient's p divides them out
+  const double ln_all = ln_s + (near && p.m == x_target ? kEx2Mean * (1.0 - double(1.0f / p.s)) : 0.0);
   RowResult r;
   r.logprob = ((double(x_target) - double(p.m)) * double(scale) - moved) * kLn2 - ln_all;
   if (r.logprob > 0.0) r.logprob = 0.0;          // a rounding of S
