@@ -9,8 +9,9 @@
 // would do in fp32; the target's is known before the row is read and is the
 // same for every thread and block of the row, so no maximum is kept and no sum
 // is ever rescaled: the exponential's error enters once.  A row whose S leaves
-// [2^-60, 2^100] (a target less likely than 2^-100, or barred) is added up again
-// with a running maximum; there, and for fp32 always, the difference is taken
+// [2^-60, 2^100] (a target less likely than 2^-100, or barred), or whose entropy
+// is less than a 64th of |ln S|, is added up again with a running maximum; there,
+// and for fp32 always, the difference is taken
 // before the scale, so a row whose logits are all the type's lowest value still
 // gets its uniform distribution.  The gradient of a * logprob + h * entropy is
 //   dx_j = (a 1{j = target} - p_j (a + h (ln p_j + H))) / T.
@@ -235,23 +236,42 @@ __device__ __forceinline__ void rescale(Part& p, float m, float scale) {
   p.m = m;
 }
 
-// Adds N values to the part: one comparison of their maximum, one exponential each.
+// One thread's running sums.  S in two parts: beside a row's one likely column,
+// whose 2^t is 1, the others are too small for fp32, and an entropy is made of
+// them.  (The same in 64 bits took a fifth longer.)  That column adds 0 to U.
+struct Running {
+  float m, s, low, u;
+};
+
+// Adds N values to the sums: one comparison of their maximum, one exponential each.
 template <bool ENT, int N>
-__device__ __forceinline__ void add(Part& p, const float (&x)[N], float scale) {
+__device__ __forceinline__ void add(Running& p, const float (&x)[N], float scale) {
   float top = x[0];
 #pragma unroll
   for (int i = 1; i < N; ++i) top = fmaxf(top, x[i]);
-  if (top > p.m) rescale<ENT>(p, top, scale);
+  if (top > p.m) {
+    const float d = fmaxf((p.m - top) * scale, -200.0f);    // as in rescale
+    const float f = ex2_approx(d);
+    if (ENT) p.u = f * fmaf(d, p.s, p.u);
+    p.s *= f;
+    p.low *= f;
+    p.m = top;
+  }
   const float m = p.m == -INFINITY ? 0.0f : p.m;   // -inf - -inf would be NaN
+  float s = 0.0f, u = 0.0f;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const float t = (x[i] - m) * scale;
     const float e = ex2_approx(t);
-    p.s += e;
+    s += e;
     // t is held above -200, where e is 0, so that 0 * -inf does not arise; a
     // NaN t has made e and S NaN
-    if (ENT) p.u = fmaf(e, fmaxf(t, -200.0f), p.u);
+    if (ENT) u = fmaf(e, fmaxf(t, -200.0f), u);
   }
+  const float sum = p.s + s, added = sum - p.s;    // and what the addition lost, exactly
+  p.low += (p.s - (sum - added)) + (s - added);
+  p.s = sum;
+  if (ENT) p.u += u;
 }
 
 template <bool ENT>
@@ -290,26 +310,36 @@ __device__ __forceinline__ Part thread_running(const void* base, int64_t vocab, 
   const Span sp = row_span<E>(row, vocab);
   const int64_t v0 = sp.nv * rank / blocks, v1 = sp.nv * (rank + 1) / blocks;
   const uint4* vec = reinterpret_cast<const uint4*>(row + sp.head);
-  Part p = {-INFINITY, 0.0f, 0.0f};
-  for (int64_t v = v0 + tid; v < v1; v += THREADS) {
-    float x[E];
-    D::unpack(vec[v], x);
-    add<ENT>(p, x, scale);
+  Running p = {-INFINITY, 0.0f, 0.0f, 0.0f};
+  const uint4 none = make_uint4(D::kNegInf2, D::kNegInf2, D::kNegInf2, D::kNegInf2);
+  // loads ahead: with 4 in a warp's rows the compiler gives the whole kernel a slower form
+  constexpr int kAgain = THREADS == kThreads ? 4 : 2;
+  for (int64_t v = v0 + tid; v < v1; v += kAgain * THREADS) {
+    uint4 q[kAgain];
+#pragma unroll
+    for (int k = 0; k < kAgain; ++k) q[k] = v + k * THREADS < v1 ? vec[v + k * THREADS] : none;
+#pragma unroll
+    for (int k = 0; k < kAgain; ++k) {
+      float x[E];
+      D::unpack(q[k], x);
+      add<ENT>(p, x, scale);
+    }
   }
   const int64_t tail = sp.head + sp.nv * E + tid;
   const float x[2] = {rank == 0 && tid < sp.head ? D::load(row + tid) : -INFINITY,
                       rank == blocks - 1 && tail < vocab ? D::load(row + tail) : -INFINITY};
   add<ENT>(p, x, scale);
-  return p;
+  return {p.m, p.s + p.low, p.u};
 }
-template <int DT, bool ENT>
-__device__ __noinline__ Part warp_running(const void* base, int64_t vocab, float scale, int rank, int blocks) {
-  return warp_join<ENT>(thread_running<DT, ENT, 32>(base, vocab, scale, rank, blocks, threadIdx.x & 31), scale);
+// The same joined over each of the warps that hold the THREADS threads.
+template <int DT, bool ENT, int THREADS>
+__device__ __noinline__ Part warp_running(const void* base, int64_t vocab, float scale, int rank, int blocks, int tid) {
+  return warp_join<ENT>(thread_running<DT, ENT, THREADS>(base, vocab, scale, rank, blocks, tid), scale);
 }
 template <int DT, bool ENT>
 __device__ __noinline__ Part block_running(const void* base, int64_t vocab, float scale, int rank, int blocks,
                                            Part* shared) {
-  Part p = warp_join<ENT>(thread_running<DT, ENT, kThreads>(base, vocab, scale, rank, blocks, threadIdx.x), scale);
+  Part p = warp_running<DT, ENT, kThreads>(base, vocab, scale, rank, blocks, threadIdx.x);
   __syncthreads();
   if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = p;
   __syncthreads();
@@ -363,9 +393,18 @@ struct RowShared {
   Part block[kMaxCluster];
 };
 
-// Whether S says that c lies too far from the row's largest logit.  NaN: the
-// row holds one, and no offset helps.
-__device__ __forceinline__ bool sums_far(float s) { return s < 0x1p-60f || s > 0x1p100f; }
+// Whether the row has to be added up around its largest logit: S says that c
+// lies too far from it, or the entropy, ln S - ln2 U / S, is so much smaller
+// than the two that their roundings show.  A target of more than 1/64 is never
+// that far, and of drawn targets one in 64 at most is 64 entropies unlikely.
+// NaN: the row holds one, and no offset helps.
+template <bool ENT>
+__device__ __forceinline__ bool sums_far(const Part& p) {
+  if (p.s < 0x1p-60f || p.s > 0x1p100f) return true;
+  if (!ENT) return false;
+  const float l = __log2f(p.s);
+  return fabsf(l) > 6.0f && 64.0f * fmaf(l, p.s, -p.u) < fabsf(l) * p.s;
+}
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
@@ -458,7 +497,7 @@ __device__ __forceinline__ Part row_sums(const void* base, int64_t vocab, float 
     p.s = warp_sum(lane < blocks ? sh.block[lane].s : 0.0f);
     if (ENT) p.u = warp_sum(lane < blocks ? sh.block[lane].u : 0.0f);
   }
-  near = !sums_far(p.s);             // the same for the whole cluster
+  near = !sums_far<ENT>(p);          // the same for the whole cluster
   if (near) return p;
   p = block_running<DT, ENT>(base, vocab, scale, rank, blocks, sh.warp);
   if (blocks > 1) {
@@ -495,7 +534,10 @@ __device__ __forceinline__ RowResult finish(const Part& p, float x_target, float
   r.logprob = ((double(x_target) - double(p.m)) * double(scale) - moved) * kLn2 - ln_all;
   if (r.logprob > 0.0) r.logprob = 0.0;          // a rounding of S
   r.log2s = float(ln_s * (1.0 / kLn2) + moved);
-  r.entropy = ENT ? float(ln_all) - float(kLn2) * (p.u / p.s) : 0.0f;
+  // a difference of two numbers of the size of ln S, the quotient with its remainder; roundings must not make it negative
+  const float mean = p.u / p.s, rest = __fdividef(fmaf(-mean, p.s, p.u), p.s);
+  const float entropy = ENT ? fmaf(-float(kLn2), rest, float(fma(-kLn2, double(mean), ln_all))) : 0.0f;
+  r.entropy = entropy < 0.0f ? 0.0f : entropy;
   if (isnan(r.logprob)) r.log2s = r.entropy = NAN;
   return r;
 }
@@ -559,7 +601,7 @@ __device__ __forceinline__ bool row_alive(const LossArgs& a, int64_t row, float&
 struct alignas(16) GradRow {
   float c, log2s, scale, ca, cb;
   float at;                  // the value at the target
-  short zero, wide;          // wide: |c s| is too large for one multiply-add
+  bool zero, wide, later;    // wide: |c s| is too large for one multiply-add; later: there is no gradient yet
   int target;                // past the vocabulary: none
 };
 template <int DT, bool ENT>
@@ -581,6 +623,7 @@ __device__ __forceinline__ GradRow grad_row(float c, float log2s, float scale, d
   g.cb = ENT ? -float(double(h) * kLn2 * inv_t) : 0.0f;
   g.at = grad_value<DT, ENT>(g, x_target) + float(double(a) * inv_t);
   g.zero = a == 0.0f && h == 0.0f;
+  g.later = false;
   g.target = int(target < (int64_t(1) << 24) ? target : int64_t(1) << 24);
   return g;
 }
@@ -681,7 +724,7 @@ __device__ __forceinline__ void write_row(const LossArgs& a, int64_t row, const 
 
 // One cluster of blocks per row.
 template <int DT, bool ENT, int OP>
-__global__ void __launch_bounds__(kThreads) forward_kernel(const LossArgs a) {
+__global__ void __launch_bounds__(kThreads, 5) forward_kernel(const LossArgs a) {
   if (OP != kLogprob) let_next_start();
   using D = Elem<DT>;
   using T = typename D::T;
@@ -730,8 +773,8 @@ __global__ void __launch_bounds__(kThreads) forward_rows_kernel(const LossArgs a
   Part p = thread_sums<DT, ENT, 32>(x, a.vocab, c, scale, 0, 1, lane);
   p.s = warp_sum(p.s);
   if (ENT) p.u = warp_sum(p.u);
-  const bool near = !sums_far(p.s);
-  if (!near) p = warp_running<DT, ENT>(x, a.vocab, scale, 0, 1);
+  const bool near = !sums_far<ENT>(p);
+  if (!near) p = warp_running<DT, ENT, 32>(x, a.vocab, scale, 0, 1, lane);
   if (lane == 0) write_row<DT, ENT, OP>(a, row, p, x_target, scale, w, near);
 }
 
@@ -950,10 +993,10 @@ struct RowInfo {
 struct HeldShared {
   uint64_t full[16], empty[16];    // of the ring's chunks
   uint64_t bar[2];                 // sums of the cluster's blocks, by turn
-  uint64_t far_bar;                // the same for a row that is added up again
   float2 part[2][kMaxCluster];     // (S, U) of each block
-  float4 far_part[kMaxCluster];    // (m, S, U)
   float2 warp_part[16];
+  Part again_part[16];             // of the warps, for a row that was put off
+  bool rows_left;                  // whether there are such rows
   RowInfo info[16];                // of the row whose first chunk lies in the slot
   GradRow coef;
 };
@@ -1053,6 +1096,74 @@ __device__ __forceinline__ Share row_share(const void* base, int vocab, int rank
   return s;
 }
 
+// A row's sums turned into its results and its gradient's constants (one thread).
+template <int DT, bool ENT>
+__device__ __forceinline__ void finish_policy_row(const LossArgs& a, int64_t row, const Part& p, const RowInfo& info,
+                                                  bool near, bool write, GradRow& coef) {
+  const RowResult r = finish<DT, ENT>(p, info.x_target, info.scale, near);
+  const PolicyRow l = policy_row(a, info.in, r.logprob, r.entropy);
+  coef = grad_row<DT, ENT>(p.m, r.log2s, info.scale, info.inv_t, l.a, l.h, r.entropy, info.target, info.x_target);
+  if (write) {
+    a.logprobs[row] = float(r.logprob);
+    if (ENT) a.entropy[row] = r.entropy;
+    a.stats[2 * row] = p.m;
+    a.stats[2 * row + 1] = r.log2s;
+    write_policy_row(a, row, l);
+  }
+}
+
+// The rows whose sums have to be taken around their largest logit, read again
+// by a cluster's first block when the others are done: a target that is all but
+// impossible, one that is unlikely in a row of little entropy, or 16-bit logits
+// past kNearOffset, which a low temperature makes of all rows.  They are marked
+// by a log2 S that no row has.  It is a call of its own so that the registers
+// of the others' loop are not shared with it.
+constexpr float kPutOff = -INFINITY;
+template <int DT, bool ENT, int SHAPE>
+__device__ __noinline__ void put_off_rows(const LossArgs& a, HeldShared& sh, unsigned cluster, unsigned clusters) {
+  using D = Elem<DT>;
+  using T = typename D::T;
+  constexpr int kRowWarps = HeldShape<SHAPE>::kRowWarps, kRowThreads = HeldShape<SHAPE>::kRowThreads;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  RowWalk walk;
+  while (walk.base < a.rows) {
+    walk.step(a, cluster, clusters);
+    for (uint32_t mine = walk.mine & walk.mine_alive; mine; mine &= mine - 1) {
+      const int64_t row = walk.base - 32 + __ffs(mine) - 1;
+      if (a.stats[2 * row + 1] != kPutOff) continue;
+      const T* x = static_cast<const T*>(a.logits) + row * a.row_stride;
+      T* out = static_cast<T*>(a.grad_logits) + row * a.grad_stride;
+      RowInfo info;
+      info.target = a.targets[row];
+      info.x_target = info.target < a.vocab ? D::load(x + info.target) : NAN;
+      info.in = policy_in(a, row, a.weights ? a.weights[row] : 1.0f / float(a.rows));
+      row_scale(a, row, info.scale, info.inv_t);
+      Part p = warp_running<DT, ENT, kRowThreads>(x, a.vocab, info.scale, 0, 1, tid);
+      if (lane == 0) sh.again_part[warp] = p;
+      row_barrier<kRowThreads>();             // and every thread has read the mark
+      if (warp == 0) {
+        p = warp_join<ENT>(lane < kRowWarps ? sh.again_part[lane] : Part{-INFINITY, 0.0f, 0.0f}, info.scale);
+        if (lane == 0) finish_policy_row<DT, ENT>(a, row, p, info, false, true, sh.coef);
+      }
+      row_barrier<kRowThreads>();
+      const GradRow g = sh.coef;
+      if (g.zero) {
+        write_zeros<DT, kRowThreads>(out, a.vocab, 0, 1);
+        continue;
+      }
+      constexpr int kEach = 8;                // elements ahead: in place, no store may be passed by a later load
+      for (int64_t j = tid; j < a.vocab; j += kEach * kRowThreads) {
+        float v[kEach];
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) v[i] = j + i * kRowThreads < a.vocab ? D::load(x + j + i * kRowThreads) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+          if (j + i * kRowThreads < a.vocab) grad_element<DT, ENT>(g, v[i], out, j + i * kRowThreads);
+      }
+    }
+  }
+}
+
 template <int DT, bool ENT, int SHAPE>
 __global__ void __launch_bounds__(HeldShape<SHAPE>::kThreads, HeldShape<SHAPE>::kBlocks)
     policy_kernel(const __grid_constant__ LossArgs a) {
@@ -1075,7 +1186,7 @@ __global__ void __launch_bounds__(HeldShape<SHAPE>::kThreads, HeldShape<SHAPE>::
   if (tid == 0) {
     mbar_init(&sh.bar[0], 1);
     mbar_init(&sh.bar[1], 1);
-    mbar_init(&sh.far_bar, 1);
+    sh.rows_left = false;
   }
   fence_mbar_init();
   __syncthreads();
@@ -1142,7 +1253,7 @@ __global__ void __launch_bounds__(HeldShape<SHAPE>::kThreads, HeldShape<SHAPE>::
   } else {
     // --------------------------------------------------------------- row warps
     bool bad = false;
-    uint32_t joined = 0, far_phase = 0, phase = 0;
+    uint32_t joined = 0, phase = 0;
     int slot = 0;
     uint4 held[kHold ? kHold : 1][kLaneVecs];
     // Rows whose stride is whole vectors all start at the same phase: the share is looked up anew only for another.
@@ -1242,11 +1353,8 @@ __global__ void __launch_bounds__(HeldShape<SHAPE>::kThreads, HeldShape<SHAPE>::
       }
       // ---- joined, and turned into the row's numbers, by the first warp
       if (warp == 0) {
-        Part p;
-        {
-          const float2 v = lane < kRowWarps ? sh.warp_part[lane] : make_float2(0.0f, 0.0f);
-          p = {c, warp_sum(v.x), ENT ? warp_sum(v.y) : 0.0f};
-        }
+        float2 v = lane < kRowWarps ? sh.warp_part[lane] : make_float2(0.0f, 0.0f);
+        Part p = {c, warp_sum(v.x), ENT ? warp_sum(v.y) : 0.0f};
         if (blocks > 1) {
           // a peer may be one join ahead of this block, never two: two barriers take turns
           const int turn = int(joined & 1);
@@ -1255,47 +1363,24 @@ __global__ void __launch_bounds__(HeldShape<SHAPE>::kThreads, HeldShape<SHAPE>::
           if (lane < blocks) send(peer_addr(&sh.part[turn][rank], lane), p.s, p.u, peer_addr(&sh.bar[turn], lane));
           if (!bad) bad = __any_sync(~0u, !mbar_wait_bounded(&sh.bar[turn], (joined >> 1) & 1));
           ++joined;
-          const float2 v = lane < blocks ? sh.part[turn][lane] : make_float2(0.0f, 0.0f);
+          v = lane < blocks ? sh.part[turn][lane] : make_float2(0.0f, 0.0f);
           p.s = warp_sum(v.x);
           if (ENT) p.u = warp_sum(v.y);
         }
         if (bad) p.s = NAN;             // a wait ran out: the row has no result
-        const bool near = !sums_far(p.s);
-        if (!near) {
-          // one warp of a block: a row whose target is all but impossible is rare
-          p = warp_running<DT, ENT>(x, a.vocab, scale, rank, blocks);
-          if (blocks > 1) {
-            if (lane == 0) mbar_arrive_expect_tx(&sh.far_bar, uint32_t(blocks) * 16);
-            __syncwarp();
-            if (lane < blocks) {
-              const uint32_t dst = peer_addr(&sh.far_part[rank], lane), bar = peer_addr(&sh.far_bar, lane);
-              send(dst, p.m, p.s, bar);
-              send(dst + 8, p.u, 0.0f, bar);
-            }
-            bad = __any_sync(~0u, !mbar_wait_bounded(&sh.far_bar, far_phase));
-            far_phase ^= 1;
-            const float4 v = lane < blocks ? sh.far_part[lane] : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
-            p = warp_join<ENT>(Part{v.x, v.y, v.z}, scale);
-            if (bad) p.s = NAN;
-          }
-        }
         if (lane == 0) {
-          const RowResult r = finish<DT, ENT>(p, info.x_target, info.scale, near);
-          const PolicyRow l = policy_row(a, info.in, r.logprob, r.entropy);
-          sh.coef = grad_row<DT, ENT>(p.m, r.log2s, info.scale, info.inv_t, l.a, l.h, r.entropy, info.target, info.x_target);
-          if (rank == 0) {
-            a.logprobs[row] = float(r.logprob);
-            if (ENT) a.entropy[row] = r.entropy;
-            a.stats[2 * row] = p.m;
-            a.stats[2 * row + 1] = r.log2s;
-            write_policy_row(a, row, l);
+          if (sums_far<ENT>(p)) {       // the same for the whole cluster
+            sh.coef.later = sh.rows_left = true;
+            if (rank == 0) a.stats[2 * row + 1] = kPutOff;
+          } else {
+            finish_policy_row<DT, ENT>(a, row, p, info, true, rank == 0, sh.coef);
           }
         }
       }
       row_barrier<kRowThreads>();
       // ---- its gradient; every chunk goes to the next row as it is done
       const GradRow g = sh.coef;
-      if (edge_at >= 0) {
+      if (edge_at >= 0 && !g.later) {
         if (g.zero)
           D::store(out + edge_at, 0.0f);
         else
@@ -1321,7 +1406,9 @@ __global__ void __launch_bounds__(HeldShape<SHAPE>::kThreads, HeldShape<SHAPE>::
       uint4* dst = reinterpret_cast<uint4*>(mine);
       const GradPairs<DT> pairs(g);
       const bool same = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
-      if (!same || (DT != NS_DTYPE_F32 && g.wide)) {
+      if (g.later) {
+        write([](const uint4&, int) {});
+      } else if (!same || (DT != NS_DTYPE_F32 && g.wide)) {
         // the rows start on different 16-byte phases, or the row is wide: element by element
         write([&](const uint4& q, int v) {
           float f[E];
@@ -1336,8 +1423,9 @@ __global__ void __launch_bounds__(HeldShape<SHAPE>::kThreads, HeldShape<SHAPE>::
       }
       // the target's value over its vector, by the thread that wrote it
       const unsigned target = unsigned(g.target - s.head) - unsigned(s.v0) * E;
-      if (!g.zero && target < unsigned(s.n) * E && int(target / E) % kRowThreads == tid) D::store(mine + target, g.at);
+      if (!g.zero && !g.later && target < unsigned(s.n) * E && int(target / E) % kRowThreads == tid) D::store(mine + target, g.at);
     }
+    if (!bad && rank == 0 && sh.rows_left) put_off_rows<DT, ENT, SHAPE>(a, sh, blockIdx.x >> shift, gridDim.x >> shift);
     // rows are left over, and with them there is no loss
     if (bad)
       for (int64_t i = tid; i < a.rows; i += kRowThreads) a.row_loss[i] = a.logprobs[i] = NAN;

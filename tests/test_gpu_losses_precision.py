@@ -1,5 +1,5 @@
 """Rows whose values are easily lost in the operators on sampled tokens' logits:
-barred targets among low logits.  Against the 64-bit oracle, within bounds
+barred targets among low logits, one likely column.  Against the 64-bit oracle, within bounds
 counted from the kernels' roundings (u = 2^-24)."""
 import math
 
@@ -16,6 +16,13 @@ HALVES = [torch.bfloat16, torch.float16]
 TYPES = [torch.float32, *HALVES]
 # rows of one block's first vectors, and rows that policy_kernel holds on chip
 VOCABS = [1003, 32000]
+
+
+def _joins(vocab):
+    """Additions of a sum after its largest term has joined it, at most: 3 in the term's vector, its thread's further
+    vectors (a block's 256 threads add up 2 x 2 elements a turn at the least), 4 that end the thread's part, 5 of a
+    warp's lanes, 5 of a block's warps, 3 of a cluster."""
+    return 3 + vocab / (256 * 4) + 4 + 13
 
 
 def _normal(seed, *shape, scale=1.0):
@@ -77,3 +84,108 @@ def test_barred_targets_among_shifted_logits(dtype, mask, shift, vocab):
         close(got.loss, want["loss"], 2 * total + 4 * U * (1 + want["loss"].abs()), "preference loss")
         a_off = want["a"].abs() * 8 * U + 0.01 / 2 * 2 * total
         close(grad, want["grad"], off(want["grad"], want["a"], zero, a_off), "preference grad")
+
+
+# --------------------------------------------------------------------- peaked rows
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [40, 1003, 32000, 50257])
+@pytest.mark.parametrize("rows", [1, 300])
+def test_entropy_does_not_depend_on_the_target(dtype, vocab, rows):
+    """One likely column and a target far below it: the entropy is a property of the row, not negative, and its error
+    stays that of sums around the row's largest logit.  A target less than 6 bits away, or than 64 entropies, may
+    serve as the sums' offset: U is then a sum around 6 bits or 64 H.  Through each way that rows are added up."""
+    cases = [(q, d) for q in (1e-3, 1e-5, 1e-7) for d in (1.0, 2.5, 7.0, 16.0, 20.0, 40.0, 61.0, 80.0)]
+    cases = cases if rows > 1 else cases[3::5]
+    q, d = (torch.tensor(c)[:, None] for c in zip(*cases))
+    x = _normal(vocab, len(cases), vocab, scale=0.5) + torch.log(q / vocab) + 10.0
+    at = torch.randint(0, vocab, (len(cases),), generator=torch.Generator().manual_seed(2))
+    here = torch.arange(len(cases))
+    targets = (at + 1) % vocab
+    x[here, at] = 10.0
+    x[here, targets] = 10.0 - d[:, 0]
+    turn = (torch.arange(rows) % len(cases)) if rows > 1 else None
+    for part in ([turn] if rows > 1 else [torch.tensor([i]) for i in range(len(cases))]):
+        z, tg = x[part].to(dtype).cuda(), targets[part].cuda()
+        one = torch.arange(min(len(part), len(cases)))         # the rows repeat: the oracle sees each once
+        ln_p, lp, ent, alive, t = O.rows(z[one], tg[one])
+        # the offset's distance from the largest logit, in nats
+        far = torch.minimum(lp.abs(), torch.maximum(torch.full_like(ent, 6 * math.log(2)), 64 * ent))
+        zz = (ln_p - ln_p.max(1, keepdim=True).values).abs() + far[:, None]
+        p = ln_p.exp()
+        mean, square = (p * zz).sum(1), (p * zz * zz).sum(1)
+        n = _joins(vocab)
+        # S and U are off by a rounding an addition and by each term's: 4 u of the exponential, 3 u |z| of its argument
+        bound = U * ((n + 8) * (1 + 2 * mean) + 3 * (mean + square) + 4 * (1 - p.max(1).values) + 4 * ent)
+        bound = bound[turn % len(cases)] if rows > 1 else bound
+        want = ent[turn % len(cases)] if rows > 1 else ent
+        got = token_logprobs(z, tg, entropy=True)[1]
+        close(got, want, bound, "entropy")
+        assert (got >= 0).all()
+        old, adv = torch.zeros(len(part), device="cuda"), torch.zeros(len(part), device="cuda")
+        got, grad = policy_loss_and_grad(z, tg, old, adv, entropy_coef=1.0, weights=torch.ones(len(part), device="cuda"))
+        close(got.entropy, want, bound, "policy entropy")
+        assert (got.entropy >= 0).all()
+        g = O.gradient(ln_p, ent, alive, t, tg[one], torch.zeros_like(ent), -torch.ones_like(ent))
+        off = grad_bound(ln_p, -far, t, ent, tg[one].cpu(), g, torch.zeros_like(ent), torch.zeros_like(ent),
+                         torch.ones_like(ent), dtype)
+        off = off + p * bound[one][:, None]
+        close(grad[one], g, off, "policy grad")
+
+
+@pytest.mark.parametrize("rows,vocab,dtype", [
+    (40, 32000, torch.bfloat16), (40, 64007, torch.float16), (500, 100003, torch.bfloat16), (420, 170000, torch.float16),
+    (30, 400000, torch.bfloat16), (40, 32000, torch.float32), (30, 151936, torch.float32), (6, 600000, torch.float32)])
+@pytest.mark.parametrize("entropy", [0.0, 0.01])
+def test_rows_that_are_added_up_again(rows, vocab, dtype, entropy):
+    """Targets 80 nats below their row's largest logit, and 16-bit logits at a temperature that puts them past 1024,
+    among ordinary rows and rows without a token: on every way that policy_kernel holds a row, into a new gradient, one
+    of another stride, and the logits' place."""
+    alive = torch.randperm(rows, generator=torch.Generator().manual_seed(rows))[:min(rows, 9)].sort().values.cuda()
+    n = len(alive)
+    part = _normal(vocab, n, vocab, scale=2.0)
+    targets = torch.randint(0, vocab, (n,), generator=torch.Generator().manual_seed(3))
+    temperature = torch.ones(n)
+    for i in range(n):
+        if i % 3 == 0:                  # all but impossible
+            part[i, targets[i]] = -75.0
+            part[i, (targets[i] + 7) % vocab] = 15.0
+        elif i % 3 == 1:                # cold
+            temperature[i] = 0.02
+            part[i] += 30.0
+            targets[i] = part[i].argmax()
+    x = torch.full((rows, vocab), math.nan, dtype=dtype, device="cuda")
+    x[alive] = part.to(dtype).cuda()
+    every = torch.full((rows,), -1, device="cuda")
+    every[alive] = targets.cuda()
+    part = x[alive].clone()
+    ln_p, lp, ent, _, t = O.rows(part, targets, temperature)
+    old = torch.zeros(rows, device="cuda")
+    # a ratio of 1.1 in an ordinary row, 1 in a cold one; one that no fp32 of either probability would hold is left out
+    old[alive] = torch.where(lp > -60, lp - 0.1 * (torch.arange(n) % 3 == 2), torch.full_like(lp, -60.0)).float().cuda()
+    adv, w = torch.full((rows,), -1.5, device="cuda"), torch.full((rows,), 0.25, device="cuda")
+    temps = torch.ones(rows, device="cuda")
+    temps[alive] = temperature.cuda()
+    want = O.policy(part, targets, old[alive], adv[alive], None, w[alive], temperature, 0.2, 0.2, 0.0, entropy)
+
+    def run(z, out):
+        return policy_loss_and_grad(z, every, old, adv, weights=w, temperature=temps, entropy_coef=entropy, out=out)
+    got, grad = run(x, None)
+    assert (grad[every < 0] == 0).all()
+    n_add = _joins(vocab) + 8
+    close(got.logprobs[alive], lp, U * (n_add + 8 * lp.abs() + 3 * ent + 16), "logprobs")
+    mean = (ln_p.exp() * (ln_p - ln_p.max(1, keepdim=True).values).nan_to_num(neginf=0.0).abs()).sum(1) + lp.abs().clamp(max=40)
+    ent_off = U * (n_add * (1 + 2 * mean) + 8 * (mean + 1) ** 2)
+    if entropy:
+        close(got.entropy[alive], ent, ent_off, "entropy")
+    # e^lp: relative errors of the sums and of the offset, which is at most 69 nats away
+    rel = U * (n_add + 8 * lp.abs() + 3 * ent + 32)
+    bound = grad_bound(ln_p, lp, t, ent, targets, want["grad"], want["a"], rel * want["a"].abs(), want["h"], dtype)
+    bound = bound + ln_p.exp() * (want["h"].abs() * ent_off)[:, None] / t[:, None]
+    close(grad[alive], want["grad"], bound, "grad")
+    wide = torch.full((rows, vocab + 3), 5.0, dtype=dtype, device="cuda")
+    moved = run(x, wide[:, 1:1 + vocab])[1]
+    assert torch.equal(moved, grad) and (wide[:, 0] == 5).all() and (wide[:, 1 + vocab:] == 5).all()
+    again, same = run(x, x)
+    assert same.data_ptr() == x.data_ptr() and torch.equal(same, grad)
+    for u, v in zip(got, again):
+        assert v is None and u is None or torch.equal(u, v)
