@@ -153,10 +153,10 @@ __device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
 
 // t = (x - c) s for pairs of logits.  fp32: difference, then product.  16-bit
 // logits: one multiply-add x s - fl(c s); the rounding of c s moves every t of
-// the row alike and is taken into account exactly, and while |c s| is below
-// kNearOffset the gradient's offset c s + log2 S rounds to less than 2^-14, and
-// so moves a value by less than a twentieth of fp16's half step.  Rows beyond
-// that go the way of `sums_far`.
+// the row alike and is taken into account exactly, as is that of the gradient's
+// offset c s + log2 S.  Rows whose |c s| is not below kNearOffset, where that is
+// at most 2^-14, are added up around 0, most of them in vain, and go the way of
+// `sums_far`: they are cold (|logit| / T past 710).
 constexpr float kNearOffset = 1024.0f;
 template <int DT>
 struct ScaledPairs {
@@ -606,8 +606,7 @@ struct alignas(16) GradRow {
 };
 template <int DT, bool ENT>
 __device__ __forceinline__ float grad_value(const GradRow& g, float x) {
-  const float t = DT == NS_DTYPE_F32 || g.wide ? fmaf(x - g.c, g.scale, -g.log2s)
-                                               : fmaf(x, g.scale, -fmaf(g.c, g.scale, g.log2s));
+  const float t = fmaf(x - g.c, g.scale, -g.log2s);
   return ex2_approx(t) * (ENT ? fmaf(g.cb, fmaxf(t, -200.0f), g.ca) : g.ca);
 }
 // a and h: dloss/dlogprob and dloss/dentropy of the row
@@ -618,17 +617,33 @@ __device__ __forceinline__ GradRow grad_row(float c, float log2s, float scale, d
   g.c = c == -INFINITY ? 0.0f : c;      // no distribution: log2 S is NaN
   g.log2s = log2s;
   g.scale = scale;
-  g.wide = !(fabsf(g.c * scale) < kNearOffset);
+  g.wide = DT != NS_DTYPE_F32 && !(fabsf(g.c * scale) < kNearOffset);
+  // at the target a (1 - p) - h p (ln p + H): where p is near 1, 1 - p must come from ln p, and that from the difference
+  // (a - a: an infinite coefficient has no gradient here, as it has none where p is 0)
+  const float t = fmaf(x_target - g.c, scale, -log2s);
+  const float ln_p = t > 0.0f ? 0.0f : t * float(kLn2);      // above 0 by a rounding of S
+  const float at = -a * expm1f(ln_p) + (a - a) - (ENT ? h * ex2_approx(t) * (fmaxf(ln_p, -200.0f) + entropy) : 0.0f);
+  g.at = float(double(at) * inv_t);
   g.ca = -float((double(a) + (ENT ? double(h) * double(entropy) : 0.0)) * inv_t);
   g.cb = ENT ? -float(double(h) * kLn2 * inv_t) : 0.0f;
-  g.at = grad_value<DT, ENT>(g, x_target) + float(double(a) * inv_t);
+  if (DT != NS_DTYPE_F32 && !g.wide) {
+    // One multiply-add to t' = x s - fl(c s + log2 S).  What the product and the sum leave out, d, is a factor of the
+    // row's p: 2^(t' - d) (A + B (t' - d)).  It is below 2^-13, so that 2^-d is 1 - d ln2 to 2^-27.
+    const float off = __fmul_rn(g.c, scale), whole = __fadd_rn(off, log2s), added = __fsub_rn(whole, off);
+    const float d = fmaf(g.c, scale, -off) + __fadd_rn(__fsub_rn(off, __fsub_rn(whole, added)), __fsub_rn(log2s, added));
+    const float f = fmaf(-d, float(kLn2), 1.0f);
+    g.c = 0.0f;
+    g.log2s = whole;
+    g.ca = f * (ENT ? fmaf(-g.cb, d, g.ca) : g.ca);
+    g.cb *= f;
+  }
   g.zero = a == 0.0f && h == 0.0f;
   g.later = false;
   g.target = int(target < (int64_t(1) << 24) ? target : int64_t(1) << 24);
   return g;
 }
-// The same for a vector; the constants of the row are in pairs.  16-bit rows
-// that are not wide take one multiply-add to log2 p.
+// The same for a vector; the constants of the row are in pairs.  c is 0 in
+// 16-bit rows that are not wide: one multiply-add to log2 p.
 template <int DT>
 struct GradPairs {
   F2 a, b, l, ca, cb;
@@ -636,8 +651,7 @@ struct GradPairs {
     if constexpr (DT == NS_DTYPE_F32) {
       a = f2(-g.c, -g.c), b = f2(g.scale, g.scale), l = f2(-g.log2s, -g.log2s);
     } else {
-      const float off = -fmaf(g.c, g.scale, g.log2s);
-      a = f2(g.scale, g.scale), b = f2(off, off), l = 0;
+      a = f2(g.scale, g.scale), b = f2(-g.log2s, -g.log2s), l = 0;
     }
   }
   __device__ __forceinline__ F2 operator()(F2 x) const {

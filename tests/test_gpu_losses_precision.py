@@ -1,6 +1,6 @@
 """Rows whose values are easily lost in the operators on sampled tokens' logits:
-barred targets among low logits, one likely column.  Against the 64-bit oracle, within bounds
-counted from the kernels' roundings (u = 2^-24)."""
+barred targets among low logits, one likely column, confident tokens.  Against
+the 64-bit oracle, within bounds counted from the kernels' roundings (u = 2^-24)."""
 import math
 
 import pytest
@@ -189,3 +189,76 @@ def test_rows_that_are_added_up_again(rows, vocab, dtype, entropy):
     assert same.data_ptr() == x.data_ptr() and torch.equal(same, grad)
     for u, v in zip(got, again):
         assert v is None and u is None or torch.equal(u, v)
+
+
+# ------------------------------------------------------------------- confident tokens
+def _peaked(dtype, vocab, peaks, rest, seed=7):
+    """Rows of one likely column: its logit is peaks[i], and the others share about rest[i] times its mass."""
+    n = len(peaks)
+    peak, rest = torch.tensor(peaks)[:, None], torch.tensor(rest)[:, None]
+    x = peak + torch.log(rest / (vocab - 1)) + _normal(seed, n, vocab, scale=0.5)
+    at = torch.randint(0, vocab, (n,), generator=torch.Generator().manual_seed(seed))
+    x[torch.arange(n), at] = peak[:, 0]
+    return x.to(dtype).cuda(), at.cuda()
+
+
+PEAKS = [20.0, 30.0, 38.5, 64.0, 90.0, 130.0, 300.0, 420.0, 640.0]
+REST = [1e-3, 1e-4, 1e-5, 1e-6]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("temperature", [1.0, 0.7])
+@pytest.mark.parametrize("vocab", VOCABS)
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_gradient_at_a_confident_token(dtype, temperature, vocab, sign):
+    """a (1 - p) of a target with p near 1 keeps what S, a sum near 1, can tell of it: S is off by a rounding an
+    addition and by the exponential's 2^-22 = 4 u, and the rest by its own relative error."""
+    peaks = [p * s for p in PEAKS for s in (temperature, -1.0)]
+    peaks, rest = [p for p in peaks for _ in REST], REST * len(peaks)
+    x, targets = _peaked(dtype, vocab, peaks, rest)
+    n = len(peaks)
+    x = x if temperature == 1.0 else ((x.float() - torch.tensor(peaks).cuda()[:, None]) * temperature
+                                      + torch.tensor(peaks).cuda()[:, None]).to(dtype)
+    a = sign * (1 + torch.rand(n, generator=torch.Generator().manual_seed(1))).cuda()
+    ln_p, lp, ent, alive, t = O.rows(x, targets, temperature)
+    off = U * (_joins(vocab) + 4 + 2) - torch.expm1(lp) * U * 64
+    info, here = torch.finfo(dtype), torch.arange(n)
+
+    def check(grad, a, rel, what):                  # rel: the coefficient's relative error
+        a = a.cpu().double()
+        want = O.gradient(ln_p, ent, alive, t, targets, a)
+        bound = grad_bound(ln_p, lp, t, ent, targets.cpu(), want, a, rel * a.abs(), torch.zeros_like(a), dtype)
+        at = want[here, targets.cpu()]
+        bound[here, targets.cpu()] = (a.abs() / t * off + at.abs() * (info.eps / 2 + rel + 4 * U)
+                                      + info.smallest_normal * info.eps)
+        close(grad, want, bound, what)
+    leaf = x.clone().requires_grad_()
+    (grad,) = torch.autograd.grad(token_logprobs(leaf, targets, temperature=temperature), [leaf], [a])
+    check(grad, a, 0.0, "token_logprobs")
+    # from the policy loss: without a drift the coefficient is -A w
+    old, w = lp.float().cuda(), torch.ones(n, device="cuda")
+    got, grad = policy_loss_and_grad(x, targets, old, -a, weights=w, temperature=temperature)
+    want = O.policy(x, targets, old, -a, None, w, temperature)
+    check(grad, want["a"], U * (_joins(vocab) + 16), "policy_loss_and_grad")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", VOCABS)
+def test_entropy_gradient_at_the_peak(dtype, vocab):
+    """-h p (ln p + H) at a likely column, where ln p + H cancels: as exact as H itself."""
+    peaks, rest = [p * s for p in PEAKS for s in (1.0, -1.0)], [1e-3]
+    x, targets = _peaked(dtype, vocab, peaks, rest * len(peaks))
+    n = len(peaks)
+    ln_p, lp, ent, alive, t = O.rows(x, targets)
+    h, zero = torch.linspace(0.5, 2.0, n).cuda(), torch.zeros(n, dtype=torch.float64)
+    leaf = x.clone().requires_grad_()
+    _, got = token_logprobs(leaf, targets, entropy=True)
+    (grad,) = torch.autograd.grad(got, [leaf], [h])
+    hh = h.cpu().double()
+    want = O.gradient(ln_p, ent, alive, t, targets, zero, hh)
+    bound = grad_bound(ln_p, lp, t, ent, targets.cpu(), want, zero, zero, hh, dtype)
+    # at the peak: ln p and H are off by S's error and by that of the small terms of U
+    at, info = want[torch.arange(n), targets.cpu()], torch.finfo(dtype)
+    off = U * (_joins(vocab) + 6) * 2 + ent * U * (_joins(vocab) + 64)
+    bound[torch.arange(n), targets.cpu()] = hh * off + at.abs() * (info.eps / 2 + 4 * U) + info.smallest_normal * info.eps
+    close(grad, want, bound, "grad")
