@@ -22,7 +22,9 @@
  *   - T: temperature fp32 [rows], or NULL and every row uses temperature_all.
  *     0 (a greedy row) stands for 1: a greedy draw is scored under the
  *     unscaled logits.  A temperature that is negative, infinite or NaN makes
- *     the row's results NaN (temperature_all: NS_ERR_INVALID_ARGUMENT).
+ *     the row's results NaN (temperature_all: NS_ERR_INVALID_ARGUMENT).  Where
+ *     T is so small that a coefficient / T passes 2^127 (an entropy's 2^119),
+ *     that is what it counts as in the columns other than the target.
  *   - -inf logits have probability 0.  A row that holds a NaN, a +inf or
  *     nothing but -inf has no distribution; its results are NaN.
  *   - Gradients have the logits' dtype and are `grad_stride` elements from row

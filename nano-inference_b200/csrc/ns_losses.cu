@@ -609,6 +609,13 @@ __device__ __forceinline__ float grad_value(const GradRow& g, float x) {
   const float t = fmaf(x - g.c, g.scale, -g.log2s);
   return ex2_approx(t) * (ENT ? fmaf(g.cb, fmaxf(t, -200.0f), g.ca) : g.ca);
 }
+// A coefficient over T, held at `most` where a small T would take it past fp32:
+// 0 times infinity must not arise in a column without probability (A + B log2 p is
+// A - 200 B there).
+__device__ __forceinline__ float held(double v, double inv_t, float most) {
+  const float f = float(v * inv_t);
+  return fabsf(f) > most && !isinf(v) ? copysignf(most, f) : f;
+}
 // a and h: dloss/dlogprob and dloss/dentropy of the row
 template <int DT, bool ENT>
 __device__ __forceinline__ GradRow grad_row(float c, float log2s, float scale, double inv_t, float a, float h,
@@ -624,8 +631,8 @@ __device__ __forceinline__ GradRow grad_row(float c, float log2s, float scale, d
   const float ln_p = t > 0.0f ? 0.0f : t * float(kLn2);      // above 0 by a rounding of S
   const float at = -a * expm1f(ln_p) + (a - a) - (ENT ? h * ex2_approx(t) * (fmaxf(ln_p, -200.0f) + entropy) : 0.0f);
   g.at = float(double(at) * inv_t);
-  g.ca = -float((double(a) + (ENT ? double(h) * double(entropy) : 0.0)) * inv_t);
-  g.cb = ENT ? -float(double(h) * kLn2 * inv_t) : 0.0f;
+  g.ca = -held(double(a) + (ENT ? double(h) * double(entropy) : 0.0), inv_t, 0x1p127f);
+  g.cb = ENT ? -held(double(h) * kLn2, inv_t, 0x1p119f) : 0.0f;
   if (DT != NS_DTYPE_F32 && !g.wide) {
     // One multiply-add to t' = x s - fl(c s + log2 S).  What the product and the sum leave out, d, is a factor of the
     // row's p: 2^(t' - d) (A + B (t' - d)).  It is below 2^-13, so that 2^-d is 1 - d ln2 to 2^-27.

@@ -1,6 +1,7 @@
 """Rows whose values are easily lost in the operators on sampled tokens' logits:
-barred targets among low logits, one likely column, confident tokens.  Against
-the 64-bit oracle, within bounds counted from the kernels' roundings (u = 2^-24)."""
+barred targets among low logits, one likely column, confident tokens, vanishing
+temperatures.  Against the 64-bit oracle, within bounds counted from the kernels'
+roundings (u = 2^-24)."""
 import math
 
 import pytest
@@ -262,3 +263,29 @@ def test_entropy_gradient_at_the_peak(dtype, vocab):
     off = U * (_joins(vocab) + 6) * 2 + ent * U * (_joins(vocab) + 64)
     bound[torch.arange(n), targets.cpu()] = hh * off + at.abs() * (info.eps / 2 + 4 * U) + info.smallest_normal * info.eps
     close(grad, want, bound, "grad")
+
+
+# ------------------------------------------------------------------ low temperatures
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("temperature", [1e-30, 1e-37, 1e-39, 1e-44])
+@pytest.mark.parametrize("vocab", VOCABS)
+def test_gradients_at_vanishing_temperatures(dtype, temperature, vocab):
+    """The distribution is the largest logit's alone; a / T may be past fp32, but a column without probability has
+    no gradient, and neither has a certain target."""
+    x = _normal(3, 4, vocab, scale=3.0).to(dtype).cuda()
+    x[:, 5] = 40.0
+    targets = torch.tensor([5, 5, 5, -1]).cuda()
+    each = torch.full((4,), temperature, device="cuda")
+    leaf = x.clone().requires_grad_()
+    lp, ent = token_logprobs(leaf, targets, temperature=each, entropy=True)
+    (grad,) = torch.autograd.grad([lp, ent], [leaf], [torch.ones_like(lp), torch.ones_like(ent)])
+    assert (lp == 0).all() and (ent == 0).all() and (grad == 0).all()
+    ones = torch.ones(4, device="cuda")
+    for kw in (dict(), dict(entropy_coef=0.1)):
+        got, grad = policy_loss_and_grad(x, targets, 0 * ones, ones, temperature=each, **kw)
+        assert (got.logprobs == 0).all() and (grad == 0).all()
+    # targets without probability: the gradient is a / T at them, or infinite
+    targets = torch.tensor([7, 8, 9, -1]).cuda()
+    (grad,) = torch.autograd.grad(token_logprobs(leaf, targets, temperature=each), [leaf], [ones * 1e-30])
+    assert (grad[:3, 10:] == 0).all() and (grad[3] == 0).all() and (grad[torch.arange(3), targets[:3]] > 0).all()
+    assert not torch.isnan(grad).any()
