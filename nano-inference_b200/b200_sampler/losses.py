@@ -27,6 +27,7 @@ counterpart (its sampler returns ids alone, ``sampling/sampler.py:36-91``).
 """
 from __future__ import annotations
 
+import ctypes
 import math
 from typing import NamedTuple, Optional, Tuple, Union
 
@@ -38,6 +39,7 @@ _DTYPES = {torch.float32: _lib.NS_DTYPE_F32, torch.bfloat16: _lib.NS_DTYPE_BF16,
            torch.float16: _lib.NS_DTYPE_F16}
 
 Temperature = Union[float, torch.Tensor]
+_LEAST = 2.0 ** -149      # of fp32's values above 0
 
 
 class PolicyLoss(NamedTuple):
@@ -70,10 +72,16 @@ def _rows(logits: torch.Tensor, targets: torch.Tensor, temperature: Temperature)
         raise TypeError("targets must be int64")
     _check("targets", targets, n, logits.device)
     if isinstance(temperature, torch.Tensor):
-        return logits, targets.contiguous(), _vector("temperature", temperature, n, logits.device), 1.0
+        each = _vector("temperature", temperature, n, logits.device)
+        if temperature.dtype is torch.float64:
+            # what fp32 rounds to 0 is no greedy row: its least value stands for it
+            least = torch.copysign(torch.full_like(temperature, _LEAST), temperature).float()
+            each = torch.where((each == 0) & (temperature != 0), least, each)
+        return logits, targets.contiguous(), each, 1.0
     temperature = float(temperature)
-    if not 0.0 <= temperature < math.inf:
-        raise ValueError("temperature must be finite and not negative")
+    rounded = ctypes.c_float(temperature).value
+    if not 0.0 <= rounded < math.inf or (rounded == 0.0 and temperature != 0.0):
+        raise ValueError("temperature must be finite and not negative, and 0 or at least 1e-45 (it is held in fp32)")
     return logits, targets.contiguous(), None, temperature
 
 
