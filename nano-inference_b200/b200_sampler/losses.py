@@ -161,13 +161,22 @@ def _grad_out(logits: torch.Tensor, given: torch.Tensor, out: Optional[torch.Ten
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors [rows, vocab] of one type share an element.  Of
+    different strides, whether their ranges do."""
     def span(t):
         if t.numel() == 0:
             return t.data_ptr(), t.data_ptr()
         last = sum((n - 1) * abs(s) for n, s in zip(t.shape, t.stride()))
         return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
     (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
+    if not (a0 < b1 and b0 < a1):
+        return False
+    if a.shape[0] == 1 or a.stride() != b.stride() or a.stride(1) != 1:
+        return True
+    # side by side in one buffer's rows: how far the one's columns lie behind the other's
+    apart = (a0 - b0) % (a.stride(0) * a.element_size())
+    width = a.shape[1] * a.element_size()
+    return apart < width or apart + width > a.stride(0) * a.element_size()
 
 
 def _gradient(logits, targets, temperature, temperature_all, stats, entropy, a, h):

@@ -25,3 +25,58 @@ def test_a_row_of_small_temperature_is_not_greedy():
     each = losses._rows(X, T, t)[2]
     assert each.dtype == torch.float32
     assert each.tolist() == [2.0 ** -149, 0.0, torch.tensor(0.7).item(), -2.0 ** -149]
+
+
+# ------------------------------------------------------------------------ out
+GRADS = [lambda x, out: losses.policy_loss_and_grad(x, T, F, F, out=out),
+         lambda x, out: losses.preference_loss_and_grad(x, T, OFFSETS, out=out)]
+
+
+@pytest.mark.parametrize("call", GRADS)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("at", [10, 11, 12])
+def test_out_beside_the_logits_in_the_same_rows_is_taken(call, dtype, at):
+    """Columns of one buffer that do not overlap: what is refused here is the CPU's tensors, after out's checks."""
+    buf = torch.zeros(4, 22, dtype=dtype)
+    with pytest.raises(ValueError, match="CUDA"):
+        call(buf[:, :10], buf[:, at:at + 10])
+    with pytest.raises(ValueError, match="CUDA"):
+        call(buf[:, at:at + 10], buf[:, :10])
+
+
+@pytest.mark.parametrize("call", GRADS)
+@pytest.mark.parametrize("first,second", [(0, 1), (0, 9), (9, 0), (3, 12)])
+def test_out_over_some_of_the_logits_is_refused(call, first, second):
+    buf = torch.zeros(5, 22)
+    with pytest.raises(ValueError, match="overlap"):
+        call(buf[:4, first:first + 10], buf[:4, second:second + 10])
+    # the columns of the next rows
+    with pytest.raises(ValueError, match="overlap"):
+        call(buf[:4, first:first + 10], buf[1:, second:second + 10])
+    # another stride: by their ranges
+    with pytest.raises(ValueError, match="overlap"):
+        call(buf[:4, first:first + 10], buf.view(-1)[:80].view(4, 20)[:, 10:])
+    flat = torch.zeros(200)
+    with pytest.raises(ValueError, match="overlap"):
+        call(flat.as_strided((4, 10), (22, 1), first), flat.as_strided((4, 10), (22, 1), second + 22))
+
+
+def test_out_behind_the_logits_across_the_end_of_a_row():
+    """22 apart, 15 and 7 behind: the columns 15 to 24 reach into the next row's first 3, which are not among 5 to 14."""
+    flat = torch.zeros(200)
+    with pytest.raises(ValueError, match="CUDA"):
+        GRADS[0](flat.as_strided((4, 10), (22, 1), 5), flat.as_strided((4, 10), (22, 1), 15))
+    with pytest.raises(ValueError, match="overlap"):
+        GRADS[0](flat.as_strided((4, 10), (22, 1), 2), flat.as_strided((4, 10), (22, 1), 15))
+
+
+def test_out_of_a_single_row():
+    """One row's stride says nothing, 0 as little as any other."""
+    x, one, flat = torch.zeros(1, 10), torch.zeros(1), torch.zeros(40)
+    t = torch.zeros(1, dtype=torch.int64)
+    for stride in (0, 5, 22):
+        a, b = flat.as_strided((1, 10), (stride, 1), 0), flat.as_strided((1, 10), (stride, 1), 10)
+        with pytest.raises(ValueError, match="CUDA"):
+            losses.policy_loss_and_grad(a, t, one, one, out=b)
+        with pytest.raises(ValueError, match="overlap"):
+            losses.policy_loss_and_grad(a, t, one, one, out=flat.as_strided((1, 10), (stride, 1), 9))
