@@ -1,9 +1,11 @@
 """Arguments of the operators on sampled tokens' logits that have to be refused
 or taken as they are before anything is launched (no GPU needed)."""
+import os
+
 import pytest
 import torch
 
-from b200_sampler import losses
+from b200_sampler import _lib, losses
 
 X, T = torch.zeros(4, 10), torch.zeros(4, dtype=torch.int64)
 F, OFFSETS = torch.zeros(4), torch.tensor([0, 2, 4])
@@ -80,3 +82,23 @@ def test_out_of_a_single_row():
             losses.policy_loss_and_grad(a, t, one, one, out=b)
         with pytest.raises(ValueError, match="overlap"):
             losses.policy_loss_and_grad(a, t, one, one, out=flat.as_strided((1, 10), (stride, 1), 9))
+
+
+# ------------------------------------------------------------------- decode loop
+def test_device_batch_scores_no_host_tensors():
+    """Nothing reaches the C entry: a kernel must not be given an address of the host."""
+    from b200_sampler import SamplingParams
+    from b200_sampler.sampler import DeviceBatch
+
+    class Library:
+        def __getattr__(self, name):
+            raise RuntimeError(name + " was called")
+
+    class Stream:
+        cuda_stream = 0
+    if not os.path.exists(_lib.LIB_PATH):
+        pytest.skip("library not built")
+    batch = DeviceBatch(None, [SamplingParams()] * 4, "cpu")
+    batch.lib = Library()
+    with pytest.raises(AssertionError):
+        batch.logprobs(X, T, F, stream=Stream())
