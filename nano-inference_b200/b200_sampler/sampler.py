@@ -416,6 +416,9 @@ class DeviceBatch:
         assert ids.dtype == torch.int64 and out.dtype == torch.float32 and ids.is_contiguous() and out.is_contiguous()
         # an address of the host, or of another device, must not reach the kernel
         assert logits.is_cuda and logits.device == ids.device == out.device == self.params.device
+        if logits.device.index != torch.cuda.current_device():     # the call launches on the current one
+            with torch.cuda.device(logits.device):
+                return self.logprobs(logits, ids, out, stream)
         s = stream if stream is not None else torch.cuda.current_stream(self.device)
         return self.lib.ns_token_logprobs(
             logits.data_ptr(), _DTYPES[logits.dtype], B, V, int(logits.stride(0)) if B > 1 else V,

@@ -102,3 +102,52 @@ def test_device_batch_scores_no_host_tensors():
     batch.lib = Library()
     with pytest.raises(AssertionError):
         batch.logprobs(X, T, F, stream=Stream())
+
+
+def test_device_batch_scores_on_its_own_device(monkeypatch):
+    """With another device current, the call is made with the tensors' device current, on that one's stream."""
+    from b200_sampler.sampler import DeviceBatch
+    current, calls = [0], []
+
+    class Tensor:
+        device, is_cuda, shape = torch.device("cuda", 1), True, (4, 10)
+
+        def __init__(self, dtype):
+            self.dtype = dtype
+
+        def stride(self, i):
+            return (10, 1)[i]
+
+        def numel(self):
+            return 4
+
+        def is_contiguous(self):
+            return True
+
+        def data_ptr(self):
+            return 1
+
+    class Device:
+        def __init__(self, device):
+            self.index = torch.device(device).index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *_):
+            current[0] = self.before
+
+    class Library:
+        def ns_token_logprobs(self, *args):
+            calls.append((current[0], args[-1]))
+            return 0
+
+    class Stream:
+        cuda_stream = 7
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: Stream())
+    batch = DeviceBatch.__new__(DeviceBatch)
+    batch.batch, batch.device, batch.params, batch.lib = 4, Tensor.device, Tensor(torch.float32), Library()
+    assert batch.logprobs(Tensor(torch.float32), Tensor(torch.int64), Tensor(torch.float32)) == 0
+    assert calls == [(1, 7)] and current == [0]
