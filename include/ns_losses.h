@@ -91,6 +91,22 @@ int ns_policy_loss(const void* logits, int dtype, int64_t rows, int64_t vocab, i
                    float* row_grad, void* grad_logits, int64_t grad_stride, ns_stream_t stream);
 
 /*
+ * ns_policy_loss in which one wait inside the kernel that holds rows on chip
+ * counts as run out at row `give_up`: for tests of what a call leaves then.  A
+ * wait runs out after 200 ms, which takes a fault elsewhere.  The rows of the
+ * blocks concerned that hold a token are then NaN in all results, and so is the
+ * loss.  Without grad_logits, or with rows too short or too long to be held,
+ * there are no such waits, and the results are ns_policy_loss's.
+ */
+int ns_policy_loss_debug(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t row_stride,
+                         const int64_t* targets, const float* temperature, float temperature_all,
+                         const float* old_logprobs, const float* ref_logprobs, const float* advantages,
+                         const float* weights, float clip_low, float clip_high, float kl_coef, float entropy_coef,
+                         float* loss, float* row_loss, float* logprobs, float* entropy, float* kl, float* stats,
+                         float* row_grad, void* grad_logits, int64_t grad_stride, int64_t give_up,
+                         ns_stream_t stream);
+
+/*
  * Preference loss on pairs of sequences whose tokens are packed row after row:
  * sequence s holds rows [seq_offsets[s], seq_offsets[s + 1]) (int64 [2 pairs +
  * 1], ascending, within rows); 2 p is pair p's chosen sequence and 2 p + 1 the

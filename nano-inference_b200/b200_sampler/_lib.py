@@ -114,6 +114,12 @@ PROTOTYPES = {
         _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp,    # loss, row_loss, logprobs, entropy, kl, stats
         _c_vp, _c_vp, _c_i64, _c_vp,                 # row_grad, grad_logits, grad_stride, stream
     ]),
+    "ns_policy_loss_debug": (_c_int, [
+        *_ROWS, _c_vp, _c_vp, _c_vp, _c_vp,          # old_logprobs, ref_logprobs, advantages, weights
+        _c_f32, _c_f32, _c_f32, _c_f32,              # clip_low, clip_high, kl_coef, entropy_coef
+        _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp,    # loss, row_loss, logprobs, entropy, kl, stats
+        _c_vp, _c_vp, _c_i64, _c_i64, _c_vp,         # row_grad, grad_logits, grad_stride, give_up, stream
+    ]),
     "ns_preference_loss": (_c_int, [
         *_ROWS, _c_vp, _c_i64, _c_vp,                # seq_offsets, pairs, ref_logprobs
         _c_f32, _c_f32, _c_int,                      # beta, label_smoothing, average

@@ -195,6 +195,7 @@ struct LossArgs {
   const float *old_logprobs, *ref_logprobs, *advantages, *weights;
   float clip_low, clip_high, kl_coef, entropy_coef;
   float *row_loss, *kl, *row_grad;
+  int64_t give_up;          // the row at which a wait counts as run out (tests); kGiveUpNever
   // preference
   const int64_t* seq_offsets;
   int64_t pairs;
@@ -216,6 +217,8 @@ __device__ __forceinline__ void row_scale(float t, float& s, double& inv_t) {
 __device__ __forceinline__ void row_scale(const LossArgs& a, int64_t row, float& s, double& inv_t) {
   row_scale(a.temperature ? a.temperature[row] : a.temperature_all, s, inv_t);
 }
+
+constexpr int64_t kGiveUpNever = -2;     // -1 ends a block's rows
 
 // Running (m, S, U) of a part of a row.  m = -inf: nothing but -inf so far.
 // Sums around the target's logit have it, or 0, as m.
@@ -1185,6 +1188,35 @@ __device__ __noinline__ void put_off_rows(const LossArgs& a, HeldShared& sh, uns
   }
 }
 
+// A wait of the block's ran out: rows of its cluster are left over, and may be
+// half written.  All of them that hold a token become NaN, and so does the loss.
+template <int DT, int SHAPE>
+__device__ __noinline__ void void_rows(const LossArgs& a, unsigned cluster, unsigned clusters) {
+  using T = typename Elem<DT>::T;
+  constexpr int kRowThreads = HeldShape<SHAPE>::kRowThreads;
+  RowWalk walk;
+  while (walk.base < a.rows) {
+    walk.step(a, cluster, clusters);
+    for (uint32_t mine = walk.mine; mine; mine &= mine - 1) {
+      const int i = __ffs(mine) - 1;
+      const int64_t row = walk.base - 32 + i;
+      T* out = static_cast<T*>(a.grad_logits) + row * a.grad_stride;
+      if (!((walk.mine_alive >> i) & 1)) {
+        if (threadIdx.x == 0) write_dead_row<kPolicy>(a, row);
+        write_zeros<DT, kRowThreads>(out, a.vocab, 0, 1);
+        continue;
+      }
+      if (threadIdx.x == 0) {
+        a.logprobs[row] = a.row_loss[row] = a.row_grad[row] = a.row_grad[a.rows + row] = NAN;
+        a.stats[2 * row] = a.stats[2 * row + 1] = NAN;
+        if (a.entropy) a.entropy[row] = NAN;
+        if (a.kl) a.kl[row] = NAN;
+      }
+      for (int64_t j = threadIdx.x; j < a.vocab; j += kRowThreads) Elem<DT>::store(out + j, NAN);
+    }
+  }
+}
+
 template <int DT, bool ENT, int SHAPE>
 __global__ void __launch_bounds__(HeldShape<SHAPE>::kThreads, HeldShape<SHAPE>::kBlocks)
     policy_kernel(const __grid_constant__ LossArgs a) {
@@ -1214,13 +1246,13 @@ __global__ void __launch_bounds__(HeldShape<SHAPE>::kThreads, HeldShape<SHAPE>::
   if (blocks > 1) cluster.sync();       // the peers' barriers exist
   const auto logits_row = [&](int64_t row) { return static_cast<const T*>(a.logits) + row * a.row_stride; };
 
+  bool bad = false;               // a wait ran out: the same in every row warp once they have left their loop
   if (warp == kRowWarps) {
     // ------------------------------------------------------------ producer warp
     const uint64_t policy = l2_policy_evict_first();
     RowWalk walk;
     int slot = 0;
     uint32_t phase = 1;                 // the first round finds the slots empty
-    bool bad = false;
     RowInfo mine = {};                  // lane i: of the i-th of 32 rows
     for (bool end = false; !end && !bad;) {
       while (walk.mine == 0 && walk.base < a.rows) {
@@ -1268,12 +1300,10 @@ __global__ void __launch_bounds__(HeldShape<SHAPE>::kThreads, HeldShape<SHAPE>::
         }
       } while (at < s.n);
     }
-    // the copies end before the block does
-    if (bad)
-      for (int i = 0; i < kSlots; ++i) mbar_wait_bounded(&sh.full[i], phase ^ 1);
+    // the copies end before the block does: those of this round, and of the last in the slots from `slot` on
+    for (int i = 0; i < kSlots; ++i) mbar_wait_bounded(&sh.full[i], i < slot ? phase ^ 1 : phase);
   } else {
     // --------------------------------------------------------------- row warps
-    bool bad = false;
     uint32_t joined = 0, phase = 0;
     int slot = 0;
     uint4 held[kHold ? kHold : 1][kLaneVecs];
@@ -1288,8 +1318,9 @@ __global__ void __launch_bounds__(HeldShape<SHAPE>::kThreads, HeldShape<SHAPE>::
       if (!bad) bad = !mbar_wait_bounded(&sh.full[slot], phase);
       bad = __any_sync(~0u, bad);
       const int64_t row = bad ? -1 : sh.info[first_slot].row;
-      if (row < 0) {              // the rows are done, or a wait ran out: all warps leave at the same barrier
-        row_barrier_any<kRowThreads>(true);
+      if (row == a.give_up && warp == kRowWarps - 1 && rank == blocks - 1) bad = true;
+      if (row < 0 || bad) {       // the rows are done, or a wait ran out: all warps leave at the same barrier
+        bad = row_barrier_any<kRowThreads>(bad);
         break;
       }
       const T* x = logits_row(row);
@@ -1447,11 +1478,9 @@ __global__ void __launch_bounds__(HeldShape<SHAPE>::kThreads, HeldShape<SHAPE>::
       if (!g.zero && !g.later && target < unsigned(s.n) * E && int(target / E) % kRowThreads == tid) D::store(mine + target, g.at);
     }
     if (!bad && rank == 0 && sh.rows_left) put_off_rows<DT, ENT, SHAPE>(a, sh, blockIdx.x >> shift, gridDim.x >> shift);
-    // rows are left over, and with them there is no loss
-    if (bad)
-      for (int64_t i = tid; i < a.rows; i += kRowThreads) a.row_loss[i] = a.logprobs[i] = NAN;
   }
   if (blocks > 1) cluster.sync();        // no block leaves while a peer may still write to it
+  if (bad && warp < kRowWarps) void_rows<DT, SHAPE>(a, blockIdx.x >> shift, gridDim.x >> shift);
 }
 
 // ---------------------------------------------------------------------------
@@ -1658,6 +1687,55 @@ bool grad_ok(const void* logits, int64_t row_stride, const void* grad, int64_t g
   return grad_stride >= vocab && (grad != logits || grad_stride == row_stride);
 }
 
+int policy_loss(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t row_stride,
+                const int64_t* targets, const float* temperature, float temperature_all,
+                const float* old_logprobs, const float* ref_logprobs, const float* advantages,
+                const float* weights, float clip_low, float clip_high, float kl_coef, float entropy_coef,
+                float* loss, float* row_loss, float* logprobs, float* entropy, float* kl, float* stats,
+                float* row_grad, void* grad_logits, int64_t grad_stride, int64_t give_up, ns_stream_t stream) {
+  if (const int rc = check_rows(dtype, rows, vocab, row_stride, temperature, temperature_all)) return rc;
+  if (!(clip_low >= 0.0f && clip_low <= 1.0f) || !(clip_high >= 0.0f && clip_high < INFINITY) ||
+      !std::isfinite(kl_coef) || !std::isfinite(entropy_coef))
+    return NS_ERR_INVALID_ARGUMENT;
+  if (!loss || (grad_logits && grad_stride < vocab)) return NS_ERR_INVALID_ARGUMENT;
+  const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (rows == 0) return cudaMemsetAsync(loss, 0, sizeof(float), s) == cudaSuccess ? NS_OK : NS_ERR_CUDA;
+  if (!logits || !targets || !old_logprobs || !advantages || !row_loss || !logprobs || !stats || !row_grad)
+    return NS_ERR_INVALID_ARGUMENT;
+  if ((kl_coef != 0.0f || kl) && !ref_logprobs) return NS_ERR_INVALID_ARGUMENT;
+  if (entropy_coef != 0.0f && !entropy) return NS_ERR_INVALID_ARGUMENT;
+  if (grad_logits && !grad_ok(logits, row_stride, grad_logits, grad_stride, vocab)) return NS_ERR_INVALID_ARGUMENT;
+  LossArgs a = row_args(logits, rows, vocab, row_stride, targets, temperature, temperature_all);
+  a.logprobs = logprobs;
+  a.entropy = entropy;
+  a.stats = stats;
+  a.old_logprobs = old_logprobs;
+  a.ref_logprobs = ref_logprobs;
+  a.advantages = advantages;
+  a.weights = weights;
+  a.clip_low = clip_low;
+  a.clip_high = clip_high;
+  a.kl_coef = kl_coef;
+  a.entropy_coef = entropy_coef;
+  a.row_loss = row_loss;
+  a.kl = kl;
+  a.row_grad = row_grad;
+  a.grad_logprobs = row_grad;
+  a.grad_entropy = entropy_coef != 0.0f ? row_grad + rows : nullptr;
+  a.grad_logits = grad_logits;
+  a.grad_stride = grad_stride;
+  a.give_up = give_up;
+  bool held = false;
+  if (grad_logits)
+    if (const int rc = policy_held(a, dtype, s, &held)) return rc;
+  if (!held) {
+    if (const int rc = forward<kPolicy>(a, dtype, s)) return rc;
+    if (grad_logits)
+      if (const int rc = gradient(a, dtype, true, s)) return rc;
+  }
+  return launch(policy_sum_kernel, 1, 1024, 1, 0, true, s, a, loss);
+}
+
 }  // namespace
 }  // namespace ns
 
@@ -1701,46 +1779,22 @@ int ns_policy_loss(const void* logits, int dtype, int64_t rows, int64_t vocab, i
                    const float* weights, float clip_low, float clip_high, float kl_coef, float entropy_coef,
                    float* loss, float* row_loss, float* logprobs, float* entropy, float* kl, float* stats,
                    float* row_grad, void* grad_logits, int64_t grad_stride, ns_stream_t stream) {
-  if (const int rc = ns::check_rows(dtype, rows, vocab, row_stride, temperature, temperature_all)) return rc;
-  if (!(clip_low >= 0.0f && clip_low <= 1.0f) || !(clip_high >= 0.0f && clip_high < INFINITY) ||
-      !std::isfinite(kl_coef) || !std::isfinite(entropy_coef))
-    return NS_ERR_INVALID_ARGUMENT;
-  if (!loss || (grad_logits && grad_stride < vocab)) return NS_ERR_INVALID_ARGUMENT;
-  const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (rows == 0) return cudaMemsetAsync(loss, 0, sizeof(float), s) == cudaSuccess ? NS_OK : NS_ERR_CUDA;
-  if (!logits || !targets || !old_logprobs || !advantages || !row_loss || !logprobs || !stats || !row_grad)
-    return NS_ERR_INVALID_ARGUMENT;
-  if ((kl_coef != 0.0f || kl) && !ref_logprobs) return NS_ERR_INVALID_ARGUMENT;
-  if (entropy_coef != 0.0f && !entropy) return NS_ERR_INVALID_ARGUMENT;
-  if (grad_logits && !ns::grad_ok(logits, row_stride, grad_logits, grad_stride, vocab)) return NS_ERR_INVALID_ARGUMENT;
-  ns::LossArgs a = ns::row_args(logits, rows, vocab, row_stride, targets, temperature, temperature_all);
-  a.logprobs = logprobs;
-  a.entropy = entropy;
-  a.stats = stats;
-  a.old_logprobs = old_logprobs;
-  a.ref_logprobs = ref_logprobs;
-  a.advantages = advantages;
-  a.weights = weights;
-  a.clip_low = clip_low;
-  a.clip_high = clip_high;
-  a.kl_coef = kl_coef;
-  a.entropy_coef = entropy_coef;
-  a.row_loss = row_loss;
-  a.kl = kl;
-  a.row_grad = row_grad;
-  a.grad_logprobs = row_grad;
-  a.grad_entropy = entropy_coef != 0.0f ? row_grad + rows : nullptr;
-  a.grad_logits = grad_logits;
-  a.grad_stride = grad_stride;
-  bool held = false;
-  if (grad_logits)
-    if (const int rc = ns::policy_held(a, dtype, s, &held)) return rc;
-  if (!held) {
-    if (const int rc = ns::forward<ns::kPolicy>(a, dtype, s)) return rc;
-    if (grad_logits)
-      if (const int rc = ns::gradient(a, dtype, true, s)) return rc;
-  }
-  return ns::launch(ns::policy_sum_kernel, 1, 1024, 1, 0, true, s, a, loss);
+  return ns::policy_loss(logits, dtype, rows, vocab, row_stride, targets, temperature, temperature_all, old_logprobs,
+                         ref_logprobs, advantages, weights, clip_low, clip_high, kl_coef, entropy_coef, loss, row_loss,
+                         logprobs, entropy, kl, stats, row_grad, grad_logits, grad_stride, ns::kGiveUpNever, stream);
+}
+
+int ns_policy_loss_debug(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t row_stride,
+                         const int64_t* targets, const float* temperature, float temperature_all,
+                         const float* old_logprobs, const float* ref_logprobs, const float* advantages,
+                         const float* weights, float clip_low, float clip_high, float kl_coef, float entropy_coef,
+                         float* loss, float* row_loss, float* logprobs, float* entropy, float* kl, float* stats,
+                         float* row_grad, void* grad_logits, int64_t grad_stride, int64_t give_up,
+                         ns_stream_t stream) {
+  if (give_up < 0) return NS_ERR_INVALID_ARGUMENT;
+  return ns::policy_loss(logits, dtype, rows, vocab, row_stride, targets, temperature, temperature_all, old_logprobs,
+                         ref_logprobs, advantages, weights, clip_low, clip_high, kl_coef, entropy_coef, loss, row_loss,
+                         logprobs, entropy, kl, stats, row_grad, grad_logits, grad_stride, give_up, stream);
 }
 
 int ns_preference_loss(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t row_stride,

@@ -151,3 +151,12 @@ def test_device_batch_scores_on_its_own_device(monkeypatch):
     batch.batch, batch.device, batch.params, batch.lib = 4, Tensor.device, Tensor(torch.float32), Library()
     assert batch.logprobs(Tensor(torch.float32), Tensor(torch.int64), Tensor(torch.float32)) == 0
     assert calls == [(1, 7)] and current == [0]
+
+
+@pytest.mark.skipif(not os.path.exists(_lib.LIB_PATH), reason="library not built")
+def test_the_debug_entry_wants_a_row():
+    args = [1, 0, 4, 10, 10, 1, None, 1.0, 1, None, 1, None, 0.2, 0.2, 0.0, 0.0, 1, 1, 1, None, None, 1, 1, 2, 10]
+    lib = _lib.load()
+    assert lib.ns_policy_loss_debug(*args, -1, None) == _lib.NS_ERR_INVALID_ARGUMENT
+    args[3] = 0
+    assert lib.ns_policy_loss_debug(*args, 1, None) == _lib.NS_ERR_INVALID_ARGUMENT
