@@ -1036,6 +1036,20 @@ __device__ __forceinline__ void send(uint32_t dst, float a, float b, uint32_t ba
                "f"(b), "r"(bar)
                : "memory");
 }
+// mbar_wait_bounded, whose limit is wall time, in the time that the kernel runs:
+// a poll counts for a millisecond at most, so that a context that was suspended
+// for long does not find its waits run out.
+__device__ __forceinline__ bool mbar_wait_running(uint64_t* bar, uint32_t parity) {
+  if (mbar_try_wait(bar, parity)) return true;
+  uint64_t last = global_timer_ns(), waited = 0;
+  while (!mbar_try_wait(bar, parity)) {
+    const uint64_t now = global_timer_ns();
+    waited += min(now - last, uint64_t(1000000));
+    last = now;
+    if (waited > kWaitTimeoutNs) return false;
+  }
+  return true;
+}
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
@@ -1281,7 +1295,7 @@ __global__ void __launch_bounds__(HeldShape<SHAPE>::kThreads, HeldShape<SHAPE>::
       }
       int at = 0;
       do {                              // a row has one chunk at least: it carries the row's numbers
-        bad = __any_sync(~0u, !mbar_wait_bounded(&sh.empty[slot], phase));
+        bad = __any_sync(~0u, !mbar_wait_running(&sh.empty[slot], phase));
         if (bad) break;
         if (at == 0 && lane == of) {
           sh.info[slot] = mine;
@@ -1301,7 +1315,7 @@ __global__ void __launch_bounds__(HeldShape<SHAPE>::kThreads, HeldShape<SHAPE>::
       } while (at < s.n);
     }
     // the copies end before the block does: those of this round, and of the last in the slots from `slot` on
-    for (int i = 0; i < kSlots; ++i) mbar_wait_bounded(&sh.full[i], i < slot ? phase ^ 1 : phase);
+    for (int i = 0; i < kSlots; ++i) mbar_wait_running(&sh.full[i], i < slot ? phase ^ 1 : phase);
   } else {
     // --------------------------------------------------------------- row warps
     uint32_t joined = 0, phase = 0;
@@ -1315,7 +1329,7 @@ __global__ void __launch_bounds__(HeldShape<SHAPE>::kThreads, HeldShape<SHAPE>::
       // ---- the row's sums, chunk after chunk as they land
       const int first_slot = slot;
       F2 sum[2] = {0, 0}, u[2] = {0, 0};
-      if (!bad) bad = !mbar_wait_bounded(&sh.full[slot], phase);
+      if (!bad) bad = !mbar_wait_running(&sh.full[slot], phase);
       bad = __any_sync(~0u, bad);
       const int64_t row = bad ? -1 : sh.info[first_slot].row;
       if (row == a.give_up && warp == kRowWarps - 1 && rank == blocks - 1) bad = true;
@@ -1350,7 +1364,7 @@ __global__ void __launch_bounds__(HeldShape<SHAPE>::kThreads, HeldShape<SHAPE>::
       RowInfo info;
       if (warp == 0) info = sh.info[first_slot];
       const auto take = [&](int at, uint4 (&q)[kLaneVecs]) {      // the chunk at vector `at` of the share
-        if (at > 0 && !bad) bad = !mbar_wait_bounded(&sh.full[slot], phase);
+        if (at > 0 && !bad) bad = !mbar_wait_running(&sh.full[slot], phase);
         const uint4* src = ring + slot * kChunkVecs + tid;
         if (at + kChunkVecs <= s.n) {
 #pragma unroll
@@ -1413,7 +1427,7 @@ __global__ void __launch_bounds__(HeldShape<SHAPE>::kThreads, HeldShape<SHAPE>::
           if (lane == 0) mbar_arrive_expect_tx(&sh.bar[turn], uint32_t(blocks) * 8);
           __syncwarp();
           if (lane < blocks) send(peer_addr(&sh.part[turn][rank], lane), p.s, p.u, peer_addr(&sh.bar[turn], lane));
-          if (!bad) bad = __any_sync(~0u, !mbar_wait_bounded(&sh.bar[turn], (joined >> 1) & 1));
+          if (!bad) bad = __any_sync(~0u, !mbar_wait_running(&sh.bar[turn], (joined >> 1) & 1));
           ++joined;
           v = lane < blocks ? sh.part[turn][lane] : make_float2(0.0f, 0.0f);
           p.s = warp_sum(v.x);
