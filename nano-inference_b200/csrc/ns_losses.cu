@@ -10,8 +10,8 @@
 // same for every thread and block of the row, so no maximum is kept and no sum
 // is ever rescaled: the exponential's error enters once.  A row whose S leaves
 // [2^-60, 2^100] (a target less likely than 2^-100, or barred), or whose entropy
-// is less than a 64th of |ln S|, is added up again with a running maximum; there,
-// and for fp32 always, the difference is taken
+// is less than a 1024th of |ln S|, is added up again with a running maximum;
+// there, and for fp32 always, the difference is taken
 // before the scale, so a row whose logits are all the type's lowest value still
 // gets its uniform distribution.  The gradient of a * logprob + h * entropy is
 //   dx_j = (a 1{j = target} - p_j (a + h (ln p_j + H))) / T.
@@ -316,7 +316,7 @@ __device__ __forceinline__ Part thread_running(const void* base, int64_t vocab, 
   Running p = {-INFINITY, 0.0f, 0.0f, 0.0f};
   const uint4 none = make_uint4(D::kNegInf2, D::kNegInf2, D::kNegInf2, D::kNegInf2);
   // loads ahead: with 4 in a warp's rows the compiler gives the whole kernel a slower form
-  constexpr int kAgain = THREADS == kThreads ? 4 : 2;
+  constexpr int kAgain = THREADS == 32 ? 2 : 4;
   for (int64_t v = v0 + tid; v < v1; v += kAgain * THREADS) {
     uint4 q[kAgain];
 #pragma unroll
@@ -398,15 +398,16 @@ struct RowShared {
 
 // Whether the row has to be added up around its largest logit: S says that c
 // lies too far from it, or the entropy, ln S - ln2 U / S, is so much smaller
-// than the two that their roundings show.  A target of more than 1/64 is never
-// that far, and of drawn targets one in 64 at most is 64 entropies unlikely.
-// NaN: the row holds one, and no offset helps.
+// than the two that their roundings, 8e-8 of |ln S|, show: 5e-7 or 8e-5 of it
+// are left.  A target of more than 2^-10 is never that far, and of drawn targets
+// one in 1024 at most is 1024 entropies unlikely; with 2^-6 and 64, rows of most
+// calls were.  NaN: the row holds one, and no offset helps.
 template <bool ENT>
 __device__ __forceinline__ bool sums_far(const Part& p) {
   if (p.s < 0x1p-60f || p.s > 0x1p100f) return true;
   if (!ENT) return false;
   const float l = __log2f(p.s);
-  return fabsf(l) > 6.0f && 64.0f * fmaf(l, p.s, -p.u) < fabsf(l) * p.s;
+  return fabsf(l) > 10.0f && 1024.0f * fmaf(l, p.s, -p.u) < fabsf(l) * p.s;
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -1014,13 +1015,14 @@ struct RowInfo {
   float x_target, scale;
   PolicyIn in;
 };
+constexpr int kPutOffList = 32;
 struct HeldShared {
   uint64_t full[16], empty[16];    // of the ring's chunks
   uint64_t bar[2];                 // sums of the cluster's blocks, by turn
   float2 part[2][kMaxCluster];     // (S, U) of each block
   float2 warp_part[16];
   Part again_part[16];             // of the warps, for a row that was put off
-  bool rows_left;                  // whether there are such rows
+  int put_off, put_off_row[kPutOffList];    // how many rows were, and the first of them
   RowInfo info[16];                // of the row whose first chunk lies in the slot
   GradRow coef;
 };
@@ -1150,54 +1152,85 @@ __device__ __forceinline__ void finish_policy_row(const LossArgs& a, int64_t row
   }
 }
 
-// The rows whose sums have to be taken around their largest logit, read again
-// by a cluster's first block when the others are done: a target that is all but
-// impossible, one that is unlikely in a row of little entropy, or 16-bit logits
-// past kNearOffset, which a low temperature makes of all rows.  They are marked
-// by a log2 S that no row has.  It is a call of its own so that the registers
-// of the others' loop are not shared with it.
+// A row whose sums have to be taken around its largest logit, read again by the
+// row warps of its cluster's first block.
+template <int DT, bool ENT, int SHAPE>
+__device__ __noinline__ void put_off_row(const LossArgs& a, HeldShared& sh, int64_t row) {
+  using D = Elem<DT>;
+  using T = typename D::T;
+  constexpr int E = D::E, kRowWarps = HeldShape<SHAPE>::kRowWarps, kRowThreads = HeldShape<SHAPE>::kRowThreads;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const T* x = static_cast<const T*>(a.logits) + row * a.row_stride;
+  T* out = static_cast<T*>(a.grad_logits) + row * a.grad_stride;
+  RowInfo info;
+  row_scale(a, row, info.scale, info.inv_t);
+  Part p = warp_running<DT, ENT, kRowThreads>(x, a.vocab, info.scale, 0, 1, tid);
+  if (lane == 0) sh.again_part[warp] = p;
+  row_barrier<kRowThreads>();
+  if (warp == 0) {
+    p = warp_join<ENT>(lane < kRowWarps ? sh.again_part[lane] : Part{-INFINITY, 0.0f, 0.0f}, info.scale);
+    if (lane == 0) {
+      info.target = a.targets[row];
+      info.x_target = info.target < a.vocab ? D::load(x + info.target) : NAN;
+      info.in = policy_in(a, row, a.weights ? a.weights[row] : 1.0f / float(a.rows));
+      finish_policy_row<DT, ENT>(a, row, p, info, false, true, sh.coef);
+    }
+  }
+  row_barrier<kRowThreads>();
+  const GradRow g = sh.coef;
+  if (g.zero) {
+    write_zeros<DT, kRowThreads>(out, a.vocab, 0, 1);
+    return;
+  }
+  if (((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(out)) & 15) != 0) {
+    write_elements<DT, ENT, kRowThreads>(g, x, out, a.vocab, 0, 1);
+    return;
+  }
+  const Span sp = row_span<E>(x, a.vocab);
+  const uint4* src = reinterpret_cast<const uint4*>(x + sp.head);
+  uint4* dst = reinterpret_cast<uint4*>(out + sp.head);
+  const int nv = int(sp.nv), at = int(g.target - sp.head);
+  constexpr int kEach = 4;                // vectors ahead: in place, no load may be moved before a store
+#pragma unroll 1
+  for (int v = tid; v < nv; v += kEach * kRowThreads) {
+    uint4 q[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) q[i] = src[min(v + i * kRowThreads, nv - 1)];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      if (v + i * kRowThreads >= nv) break;
+      float f[E];
+      D::unpack(q[i], f);
+#pragma unroll
+      for (int j = 0; j < E; ++j) f[j] = (v + i * kRowThreads) * E + j == at ? g.at : grad_value<DT, ENT>(g, f[j]);
+      dst[v + i * kRowThreads] = D::pack(f);
+    }
+  }
+  const int64_t tail = sp.head + sp.nv * E + tid;
+  if (tid < sp.head) grad_element<DT, ENT>(g, D::load(x + tid), out, tid);
+  if (tail < a.vocab) grad_element<DT, ENT>(g, D::load(x + tail), out, tail);
+}
+
+// Those rows, when the others are done: a target that is all but impossible, one
+// that is unlikely in a row of little entropy, or 16-bit logits past kNearOffset,
+// which a low temperature makes of all rows.  The first of them are listed, and
+// all are marked by a log2 S that no row has.  Calls of their own, so that the
+// registers of the row loop are not shared with them.
 constexpr float kPutOff = -INFINITY;
 template <int DT, bool ENT, int SHAPE>
 __device__ __noinline__ void put_off_rows(const LossArgs& a, HeldShared& sh, unsigned cluster, unsigned clusters) {
-  using D = Elem<DT>;
-  using T = typename D::T;
-  constexpr int kRowWarps = HeldShape<SHAPE>::kRowWarps, kRowThreads = HeldShape<SHAPE>::kRowThreads;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int count = sh.put_off;
+  if (count <= kPutOffList) {
+    for (int i = 0; i < count; ++i) put_off_row<DT, ENT, SHAPE>(a, sh, sh.put_off_row[i]);
+    return;
+  }
   RowWalk walk;
   while (walk.base < a.rows) {
     walk.step(a, cluster, clusters);
     for (uint32_t mine = walk.mine & walk.mine_alive; mine; mine &= mine - 1) {
       const int64_t row = walk.base - 32 + __ffs(mine) - 1;
-      if (a.stats[2 * row + 1] != kPutOff) continue;
-      const T* x = static_cast<const T*>(a.logits) + row * a.row_stride;
-      T* out = static_cast<T*>(a.grad_logits) + row * a.grad_stride;
-      RowInfo info;
-      info.target = a.targets[row];
-      info.x_target = info.target < a.vocab ? D::load(x + info.target) : NAN;
-      info.in = policy_in(a, row, a.weights ? a.weights[row] : 1.0f / float(a.rows));
-      row_scale(a, row, info.scale, info.inv_t);
-      Part p = warp_running<DT, ENT, kRowThreads>(x, a.vocab, info.scale, 0, 1, tid);
-      if (lane == 0) sh.again_part[warp] = p;
-      row_barrier<kRowThreads>();             // and every thread has read the mark
-      if (warp == 0) {
-        p = warp_join<ENT>(lane < kRowWarps ? sh.again_part[lane] : Part{-INFINITY, 0.0f, 0.0f}, info.scale);
-        if (lane == 0) finish_policy_row<DT, ENT>(a, row, p, info, false, true, sh.coef);
-      }
-      row_barrier<kRowThreads>();
-      const GradRow g = sh.coef;
-      if (g.zero) {
-        write_zeros<DT, kRowThreads>(out, a.vocab, 0, 1);
-        continue;
-      }
-      constexpr int kEach = 8;                // elements ahead: in place, no store may be passed by a later load
-      for (int64_t j = tid; j < a.vocab; j += kEach * kRowThreads) {
-        float v[kEach];
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) v[i] = j + i * kRowThreads < a.vocab ? D::load(x + j + i * kRowThreads) : 0.0f;
-#pragma unroll
-        for (int i = 0; i < kEach; ++i)
-          if (j + i * kRowThreads < a.vocab) grad_element<DT, ENT>(g, v[i], out, j + i * kRowThreads);
-      }
+      // every thread reads the mark before the first of the row's barriers, behind which it goes
+      if (a.stats[2 * row + 1] == kPutOff) put_off_row<DT, ENT, SHAPE>(a, sh, row);
     }
   }
 }
@@ -1253,7 +1286,7 @@ __global__ void __launch_bounds__(HeldShape<SHAPE>::kThreads, HeldShape<SHAPE>::
   if (tid == 0) {
     mbar_init(&sh.bar[0], 1);
     mbar_init(&sh.bar[1], 1);
-    sh.rows_left = false;
+    sh.put_off = 0;
   }
   fence_mbar_init();
   __syncthreads();
@@ -1436,8 +1469,10 @@ __global__ void __launch_bounds__(HeldShape<SHAPE>::kThreads, HeldShape<SHAPE>::
         if (bad) p.s = NAN;             // a wait ran out: the row has no result
         if (lane == 0) {
           if (sums_far<ENT>(p)) {       // the same for the whole cluster
-            sh.coef.later = sh.rows_left = true;
+            sh.coef.later = true;
             if (rank == 0) a.stats[2 * row + 1] = kPutOff;
+            if (sh.put_off < kPutOffList) sh.put_off_row[sh.put_off] = int(row);
+            ++sh.put_off;
           } else {
             finish_policy_row<DT, ENT>(a, row, p, info, true, rank == 0, sh.coef);
           }
@@ -1491,7 +1526,7 @@ __global__ void __launch_bounds__(HeldShape<SHAPE>::kThreads, HeldShape<SHAPE>::
       const unsigned target = unsigned(g.target - s.head) - unsigned(s.v0) * E;
       if (!g.zero && !g.later && target < unsigned(s.n) * E && int(target / E) % kRowThreads == tid) D::store(mine + target, g.at);
     }
-    if (!bad && rank == 0 && sh.rows_left) put_off_rows<DT, ENT, SHAPE>(a, sh, blockIdx.x >> shift, gridDim.x >> shift);
+    if (!bad && rank == 0 && sh.put_off) put_off_rows<DT, ENT, SHAPE>(a, sh, blockIdx.x >> shift, gridDim.x >> shift);
   }
   if (blocks > 1) cluster.sync();        // no block leaves while a peer may still write to it
   if (bad && warp < kRowWarps) void_rows<DT, SHAPE>(a, blockIdx.x >> shift, gridDim.x >> shift);
