@@ -568,7 +568,11 @@ __device__ __forceinline__ PolicyRow policy_row(const LossArgs& a, const PolicyI
   if (a.ref_logprobs) {
     const float d = float(double(in.ref) - logprob);
     const float g = expm1f(d);
-    r.kl = g - d;
+    // e^d - 1 - d: near 0 by its series, d^2 / 2 (1 + d / 3 (1 + d / 4 (...))), whose next term is 2^-28 at 1/2
+    float series = 1.0f;
+#pragma unroll
+    for (int i = 9; i > 2; --i) series = fmaf(d * (1.0f / float(i)), series, 1.0f);
+    r.kl = fabsf(d) < 0.5f ? 0.5f * d * d * series : g - d;
     if (a.kl_coef != 0.0f) {
       r.loss = fmaf(a.kl_coef, r.kl, r.loss);
       r.a = fmaf(-a.kl_coef, g, r.a);

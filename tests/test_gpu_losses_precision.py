@@ -309,3 +309,25 @@ def test_log_probabilities_have_no_mean_error(dtype, vocab):
         want = z.gather(1, targets[:, None])[:, 0] - torch.logsumexp(z, 1)
         mean += (token_logprobs(x, targets).double() - want).sum().item() / rows
     assert abs(mean) < 2e-8
+
+
+# ------------------------------------------------------------------- the KL term
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [1, 32000])
+def test_kl_near_zero(dtype, vocab):
+    """exp(d) - d - 1 of small d, at a column that has all of the probability (its logit 0: ln p is 0, and d is the
+    reference's number).  Where the three are added up, from 1/2 on, a last place of e^d - 1 is at most 4.4 of their
+    sum above 0 and 3.7 below, and d's rounding is none: 16 u in all.  Below, the series has 10 roundings."""
+    d = torch.tensor([s * v for v in (1e-30, 1e-8, 1e-5, 1e-3, 0.03, 0.2, 0.4999, 0.5, 0.7, 1.5, 20.0) for s in (1, -1)])
+    n = len(d)
+    x = torch.full((n, vocab), -INF, dtype=dtype, device="cuda")
+    targets = (torch.arange(n) * 31 % vocab).cuda()
+    x[torch.arange(n), targets] = 0.0
+    want = torch.expm1(d.double()) - d.double()
+    series = sum(d.double() ** k / math.factorial(k) for k in range(2, 14))
+    want = torch.where(d.abs() < 0.1, series, want)          # 64 bits cancel too
+    zero = torch.zeros(n, device="cuda")
+    got, _ = policy_loss_and_grad(x, targets, zero, zero, ref_logprobs=d.cuda(), kl_coef=1.0)
+    assert (got.logprobs == 0).all() and (got.kl >= 0).all()
+    close(got.kl, want, 16 * U * want + 2.0 ** -149, "kl")
+    close(got.row_loss, want, 17 * U * want + 2.0 ** -149, "row_loss")
