@@ -10,10 +10,10 @@
 // same for every thread and block of the row, so no maximum is kept and no sum
 // is ever rescaled: the exponential's error enters once.  A row whose S leaves
 // [2^-60, 2^100] (a target less likely than 2^-100, or barred), or whose entropy
-// is less than a 1024th of |ln S|, is added up again with a running maximum;
-// there, and for fp32 always, the difference is taken
-// before the scale, so a row whose logits are all the type's lowest value still
-// gets its uniform distribution.  The gradient of a * logprob + h * entropy is
+// is less than a 256th of |ln S|, is added up again with a running maximum;
+// there, and for fp32 always, the difference is taken before the scale, so a row
+// whose logits are all the type's lowest value still gets its uniform
+// distribution.  The gradient of a * logprob + h * entropy is
 //   dx_j = (a 1{j = target} - p_j (a + h (ln p_j + H))) / T.
 //
 // Bound: HBM.  A forward reads the logits once, a gradient reads them and
@@ -398,16 +398,16 @@ struct RowShared {
 
 // Whether the row has to be added up around its largest logit: S says that c
 // lies too far from it, or the entropy, ln S - ln2 U / S, is so much smaller
-// than the two that their roundings, 8e-8 of |ln S|, show: 5e-7 or 8e-5 of it
-// are left.  A target of more than 2^-10 is never that far, and of drawn targets
-// one in 1024 at most is 1024 entropies unlikely; with 2^-6 and 64, rows of most
-// calls were.  NaN: the row holds one, and no offset helps.
+// than the two that their roundings show (2e-7 of |ln S| as a root mean square,
+// 4e-7 beside many small terms).  A target of more than 2^-8 is never that far,
+// and of drawn targets one in 256 at most is 256 entropies unlikely.  With 2^-6
+// and 64, rows of most calls were.  NaN: the row holds one, and no offset helps.
 template <bool ENT>
 __device__ __forceinline__ bool sums_far(const Part& p) {
   if (p.s < 0x1p-60f || p.s > 0x1p100f) return true;
   if (!ENT) return false;
   const float l = __log2f(p.s);
-  return fabsf(l) > 10.0f && 1024.0f * fmaf(l, p.s, -p.u) < fabsf(l) * p.s;
+  return fabsf(l) > 8.0f && 256.0f * fmaf(l, p.s, -p.u) < fabsf(l) * p.s;
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -518,7 +518,7 @@ __device__ __forceinline__ Part row_sums(const void* base, int64_t vocab, float 
 // reference's log-probability keep their digits.  The target's t uses the same
 // rounded scale, and `near` the same rounded offset, as the sums.  The
 // logarithm is split as exponent * ln2 + ln(mantissa), whose second part lies
-// in [0, ln2) and is exact to 2^-25.
+// in [0, ln2) and is off by 2^-24 at most.
 struct RowResult {
   double logprob;
   float entropy, log2s;      // log2 S around m s, not rounded
