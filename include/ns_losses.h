@@ -32,7 +32,9 @@
  *     stride): the gradient then takes their place.  No other overlap.  The
  *     columns past vocab are left as they are.
  *   - Sums are fp32 per thread and joined in a fixed order: equal inputs give
- *     equal bits.  No call needs a workspace or leaves state for the next.
+ *     equal bits (of rows that start on the same 16-byte boundaries; others are
+ *     added up in another order).  No call needs a workspace or leaves state
+ *     for the next.
  *
  *   stats fp32 [rows][2], written by the forward calls and read by the
  *   gradient: an offset c (a logit of the row) and log2 of sum exp((x - c) / T).
