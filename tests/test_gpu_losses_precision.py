@@ -331,3 +331,37 @@ def test_kl_near_zero(dtype, vocab):
     assert (got.logprobs == 0).all() and (got.kl >= 0).all()
     close(got.kl, want, 16 * U * want + 2.0 ** -149, "kl")
     close(got.row_loss, want, 17 * U * want + 2.0 ** -149, "row_loss")
+
+
+def test_more_rows_added_up_again_than_a_block_lists():
+    """16500 cold rows on some 444 clusters, a few of them without a token: each cluster has over 32 to add up again,
+    and finds them by their marks."""
+    rows, vocab, t = 16500, 14400, 0.02
+    g = torch.Generator("cuda").manual_seed(1)
+    x = torch.empty(rows, vocab, dtype=torch.bfloat16, device="cuda")
+    for i in range(0, rows, 1500):
+        x[i:i + 1500] = (torch.randn(1500, vocab, device="cuda", generator=g) + 30).bfloat16()
+    targets = torch.where(torch.arange(rows, device="cuda") % 3 > 0, x.argmax(1), torch.arange(rows, device="cuda") % vocab)
+    targets[5::97] = -1
+    zero, adv = torch.zeros(rows, device="cuda"), torch.randn(rows, device="cuda", generator=g)
+    lp = torch.empty(rows, dtype=torch.float64, device="cuda")
+    for i in range(0, rows, 1500):
+        z = x[i:i + 1500].double() / t
+        lp[i:i + 1500] = z.gather(1, targets[i:i + 1500].clamp(min=0)[:, None])[:, 0] - torch.logsumexp(z, 1)
+    old = torch.where(targets >= 0, lp, torch.zeros_like(lp)).clamp(min=-60).float()
+    w = torch.full((rows,), 1.0, device="cuda")
+    got, grad = policy_loss_and_grad(x, targets, old, adv, weights=w, temperature=t)
+    alive = targets >= 0
+    # S has a rounding an addition and the exponentials' 4 u; the value's own rounding and the scale's
+    close(got.logprobs, torch.where(alive, lp, torch.zeros_like(lp)).cpu(), U * (_joins(vocab) + 12 + 6 * lp.abs().cpu()), "logprobs")
+    pick = torch.cat([torch.arange(0, rows, 271), torch.arange(rows - 40, rows)]).cuda()
+    want = O.policy(x[pick], targets[pick], old[pick], adv[pick], None, w[pick], t)
+    rel = U * (_joins(vocab) + 32 + 8 * want["logprobs"].abs())
+    none = torch.zeros(len(pick), dtype=torch.float64)
+    bound = grad_bound(want["ln_p"], want["logprobs"], want["t"], want["entropy"], targets[pick].cpu(), want["grad"], want["a"],
+                       rel * want["a"].abs(), none, x.dtype)
+    close(grad[pick], want["grad"], bound, "grad")
+    assert (grad[~alive] == 0).all() and torch.isfinite(got.loss)
+    for i in range(0, rows, 1500):      # no row is left as its memory was: a row's gradient sums to nothing beside its parts
+        part = grad[i:i + 1500].double()
+        assert (part.sum(1).abs() <= part.abs().sum(1) * 2.0 ** -7 + 1e-4).all()
